@@ -85,6 +85,8 @@ enum BtKernelId {
     BTK_SUM_PARTIALS,
     BTK_SIGMOID_MSE,
     BTK_ADAMW,
+    BTK_POLICY,
+    BTK_AFFINE,
     BTK_COUNT
 };
 int bt_prof_register(const char *kernel_expr);  // -> profiler id of the kernel spelled `kernel_expr`

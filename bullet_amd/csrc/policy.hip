@@ -1,0 +1,703 @@
+// Losses of a policy head over masked moves, each with its gradient: the clipped policy loss with a KL term and the
+// preference loss over pairs of lines of moves.
+//
+// Both are bound by the bytes of the logits: one group of lanes owns a row, keeps it in registers between the softmax
+// statistics and the gradient, and so reads every logit once and writes every gradient once. Per-row scalars (log-sum,
+// log-probability, ratio, losses) are computed in 64 bits from the row's 32-bit sum: they cost one evaluation a row and
+// keep the rounding of values near 7 out of differences that may be near 0.
+#include <type_traits>
+
+#include "common.h"
+
+namespace {
+
+constexpr float NEG_INF = -__builtin_huge_valf();
+
+template <typename T>
+struct Row {
+    static constexpr int V = 16 / sizeof(T);  // elements of a 16-byte chunk
+    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+    typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint64_t>::type bytes;  // one mask byte per element
+};
+
+// exp(x) for x <= 0 with the rounding of x * log2(e) carried along (x to -100 would lose 7 bits otherwise); below -150 it
+// is 0 in 32 bits, and the select keeps -infinity out of the correction but lets NaN pass
+__device__ __forceinline__ float exp_neg(float x) {
+    const float c = x < -150.0f ? -150.0f : x;
+    const float t = c * 1.44269502f;
+    const float lo = fmaf(c, 1.92596303e-8f, fmaf(c, 1.44269502f, -t));  // c * log2(e) - t
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, lo * 0.693147182f, e);
+}
+
+// a launch holds less than 2^32 threads a dimension: many rows fold into the grid's second one
+__device__ __forceinline__ long long row_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 row_grid(long long blocks) {
+    constexpr long long W = 1 << 22;
+    return blocks <= W ? dim3((unsigned)blocks) : dim3((unsigned)W, (unsigned)((blocks + W - 1) / W));
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+// Reductions over the G lanes that own a row: 8 lanes (short rows, eight rows a wave), a wave, or a workgroup of 256.
+// The order is fixed. Lane exchanges inside 16 lanes are DPP moves, no LDS.
+template <int G>
+struct Group {
+    template <typename F>
+    static __device__ __forceinline__ float reduce(float v, F f, float *red) {
+        v = f(v, dpp<0xB1>(v));   // lane ^ 1
+        v = f(v, dpp<0x4E>(v));   // lane ^ 2
+        v = f(v, dpp<0x141>(v));  // mirrored within 8
+        if (G == 8) return v;
+        v = f(v, dpp<0x140>(v));  // mirrored within 16
+        v = f(f(lane_value(v, 0), lane_value(v, 16)), f(lane_value(v, 32), lane_value(v, 48)));
+        if (G == 64) return v;
+        __syncthreads();  // the previous reduction's values have been read
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return f(f(red[0], red[1]), f(red[2], red[3]));
+    }
+    static __device__ __forceinline__ float max(float v, float *red) {
+        return reduce(v, [](float a, float b) { return fmaxf(a, b); }, red);
+    }
+    static __device__ __forceinline__ float sum(float v, float *red) {
+        return reduce(v, [](float a, float b) { return a + b; }, red);
+    }
+    static __device__ double sum64(double v, double *red) {
+        for (int o = 1; o < (G < 64 ? G : 64); o <<= 1) v += __shfl_xor(v, o, 64);
+        if (G <= 64) return v;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return (red[0] + red[1]) + (red[2] + red[3]);
+    }
+};
+
+// one mask byte per element of the chunk that starts at element e0: 0 where there is no element or no legal move
+template <typename T>
+__device__ __forceinline__ typename Row<T>::bytes legal_bytes(const uint8_t *mask, int e0, int width) {
+    typedef typename Row<T>::bytes B;
+    constexpr int V = Row<T>::V;
+    const int n = width - e0;
+    if (n <= 0) return 0;
+    if (!mask) return n >= V ? (B)0x0101010101010101ull : (B)0x0101010101010101ull & (((B)1 << (8 * n)) - 1);
+    B b = 0;
+    if (n >= V) {
+        __builtin_memcpy(&b, mask + e0, V);
+    } else {
+        for (int j = 0; j < n; j++) b |= (B)mask[e0 + j] << (8 * j);
+    }
+    return b;
+}
+template <typename B>
+__device__ __forceinline__ bool legal_at(B b, int j) {
+    return (b >> (8 * j)) & 0xff;
+}
+// the chunk's elements that the mask leaves (a chunk it leaves empty is not read), -infinity elsewhere
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T *row, int e0, int width, typename Row<T>::bytes b, typename Row<T>::vec &v) {
+    constexpr int V = Row<T>::V;
+    if (b) {
+        if (width - e0 >= V) {
+            __builtin_memcpy(&v, row + e0, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (j < width - e0) v[j] = row[e0 + j];
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void keep_legal(typename Row<T>::bytes b, typename Row<T>::vec &v) {
+#pragma unroll
+    for (int j = 0; j < Row<T>::V; j++) v[j] = legal_at(b, j) ? v[j] : (T)NEG_INF;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T *row, int e0, int width, typename Row<T>::vec v) {
+    constexpr int V = Row<T>::V;
+    if (width - e0 >= V) {
+        __builtin_memcpy(row + e0, &v, 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j++)
+            if (j < width - e0) row[e0 + j] = v[j];
+    }
+}
+
+// Softmax statistics of one row, and what the KL over the whole policy needs beside them.
+struct RowStats {
+    float top, sum;       // largest legal logit, sum of exp(z - top)
+    float ref_top, ref_sum;
+    float cross;          // sum of exp(z - top) (z - q)
+};
+
+// What a row's element needs for its gradient: p = exp(z - top) inv;
+//   g = -ca p (+ ca for the action taken), and for the full KL + ck p (z - q - shift)
+struct RowGrad {
+    float top, inv, ca, ck, shift;
+};
+template <bool FULL>
+__device__ __forceinline__ float row_grad(float e, float z, float q, const RowGrad &r) {
+    const float p = e * r.inv;
+    float g = -r.ca * p;
+    if (FULL) g = fmaf(r.ck * p, (z - q) - r.shift, g);
+    return e == 0.0f ? 0.0f : g;  // masked (and vanishing) places have no share, whatever the row's scalars are
+}
+
+struct PolicyArgs {
+    const void *z, *ref;
+    const uint8_t *mask;
+    const int32_t *actions;
+    const float *old_logp, *advantages, *weights;
+    void *grad;
+    float *row_loss, *row_logp, *row_kl;
+    bt_policy_desc d;
+};
+
+// The whole of one row once its statistics are known: losses, row outputs and the coefficients of its gradient.
+// `near` is set when the ratio stands so close to a clipping border that the row's 32-bit sum cannot say on which side:
+// the caller then sums again in 64 bits and asks once more (sum64 > 0).
+struct PolicyRow {
+    float za, qa;    // logit (and reference logit) of the action taken
+    bool counted;
+};
+__device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, const PolicyRow &pr, const RowStats &st, double sum64,
+                                               bool full, RowGrad &g, double &logp, double &kl, float &loss, float &grad_taken) {
+    const bt_policy_desc &d = a.d;
+    const double logsum = log(sum64 > 0.0 ? sum64 : (double)st.sum);
+    logp = ((double)pr.za - (double)st.top) - logsum;
+    const double adv = a.advantages[row], w = a.weights ? (double)a.weights[row] : 1.0;
+    const double r = exp(logp - (double)a.old_logp[row]);
+    const double lo = 1.0 - (double)d.clip_low, hi = 1.0 + (double)d.clip_high;
+    // a 32-bit sum of up to 2^24 terms is off by less than 1e-5 of itself
+    const bool near = fabs(r - lo) < 1e-5 * lo || fabs(r - hi) < 1e-5 * hi;
+    const double free_gain = r * adv, held_gain = fmin(fmax(r, lo), hi) * adv;
+    double slope = free_gain <= held_gain || free_gain != free_gain ? -free_gain : 0.0;
+    kl = 0.0;
+    g.ck = 0.0f;
+    g.shift = 0.0f;
+    if (d.kl == BT_KL_TAKEN) {
+        const double x = (double)((const float *)a.ref)[row] - logp;
+        const double em1 = expm1(x);
+        kl = em1 - x;
+        slope -= (double)d.kl_weight * em1;
+    } else if (full) {
+        const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log((double)st.ref_sum));
+        kl = (double)st.cross / (double)st.sum - dl;
+        g.ck = (float)(w * (double)d.kl_weight);
+        g.shift = (float)(dl + kl);
+    }
+    loss = (float)(w * ((double)d.kl_weight * kl - (free_gain != free_gain ? free_gain : fmin(free_gain, held_gain))));
+    g.top = st.top;
+    g.inv = (float)(1.0 / (double)st.sum);
+    g.ca = (float)(w * slope);
+    const double pa = exp(logp);
+    grad_taken = (float)(w * slope * (1.0 - pa));
+    if (full && pa > 0.0) grad_taken += (float)((double)g.ck * pa * (((double)pr.za - (double)pr.qa) - (double)g.shift));
+    return near;
+}
+
+template <typename T>
+__device__ __forceinline__ PolicyRow policy_row_begin(const PolicyArgs &a, const T *z, const T *q, const uint8_t *mask, int row,
+                                                      bool full) {
+    PolicyRow pr{0.0f, 0.0f, false};
+    const int act = a.actions[row];
+    pr.counted = act >= 0 && act < a.d.width && (!mask || mask[act]);
+    if (pr.counted) {
+        pr.za = (float)z[act];
+        if (full) pr.qa = (float)q[act];
+    }
+    return pr;
+}
+__device__ __forceinline__ void policy_row_out(const PolicyArgs &a, int row, bool counted, float loss, double logp, double kl) {
+    a.row_loss[row] = counted ? loss : 0.0f;
+    if (a.row_logp) a.row_logp[row] = counted ? (float)logp : 0.0f;
+    if (a.row_kl) a.row_kl[row] = counted ? (float)kl : 0.0f;
+}
+
+// this lane's share of the row's sum, from memory and in 64 bits (rare: see policy_scalars)
+template <typename T, int G>
+__device__ __noinline__ double sum_again(const T *z, const uint8_t *mask, int width, int lane, float top) {
+    double s = 0.0;
+    for (long long e = lane; e < width; e += G)
+        if (!mask || mask[e]) s += exp((double)(float)z[e] - (double)top);
+    return s;
+}
+
+// One group of G lanes per row, at most K chunks a lane, all in registers.
+template <typename T, int G, int K, bool FULL>
+__global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
+    constexpr int V = Row<T>::V;
+    typedef typename Row<T>::vec vec;
+    typedef typename Row<T>::bytes bytes;
+    __shared__ float red[4];
+    __shared__ double red64[4];
+    const int lane = threadIdx.x % G;
+    const long long row64 = row_block() * (256 / G) + threadIdx.x / G;
+    if (row64 >= a.d.batch) return;  // (whole groups)
+    const int row = (int)row64;
+    const int width = a.d.width;
+    const T *z = (const T *)a.z + (size_t)row * a.d.ld;
+    const T *q = FULL ? (const T *)a.ref + (size_t)row * a.d.ld : nullptr;
+    const uint8_t *mask = a.mask ? a.mask + (size_t)row * a.d.mask_ld : nullptr;
+    const PolicyRow pr = policy_row_begin(a, z, q, mask, row, FULL);
+
+    bytes b[K];
+    vec zc[K], qc[FULL ? K : 1];
+#pragma unroll
+    for (int k = 0; k < K; k++) b[k] = legal_bytes<T>(mask, (lane + k * G) * V, width);
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        load_chunk<T>(z, (lane + k * G) * V, width, b[k], zc[k]);
+        if (FULL) load_chunk<T>(q, (lane + k * G) * V, width, b[k], qc[FULL ? k : 0]);
+    }
+    float top = NEG_INF, ref_top = NEG_INF;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        keep_legal<T>(b[k], zc[k]);
+#pragma unroll
+        for (int j = 0; j < V; j++) top = fmaxf(top, (float)zc[k][j]);
+        if (FULL) {
+            keep_legal<T>(b[k], qc[FULL ? k : 0]);
+#pragma unroll
+            for (int j = 0; j < V; j++) ref_top = fmaxf(ref_top, (float)qc[FULL ? k : 0][j]);
+        }
+    }
+    RowStats st;
+    st.top = Group<G>::max(top, red);
+    st.ref_top = FULL ? Group<G>::max(ref_top, red) : 0.0f;
+    const float base = st.top == NEG_INF ? 0.0f : st.top;  // (nothing left: every term is exp(-infinity) = 0)
+    float e[K][V], s = 0.0f, sq = 0.0f, cross = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float zv = (float)zc[k][j];
+            e[k][j] = exp_neg(zv - base);
+            s += e[k][j];
+            if (FULL) {
+                const float qv = (float)qc[FULL ? k : 0][j];
+                sq += exp_neg(qv - st.ref_top);
+                cross += e[k][j] == 0.0f ? 0.0f : e[k][j] * (zv - qv);
+            }
+        }
+    st.sum = Group<G>::sum(s, red);
+    st.ref_sum = FULL ? Group<G>::sum(sq, red) : 1.0f;
+    st.cross = FULL ? Group<G>::sum(cross, red) : 0.0f;
+    const bool counted = pr.counted && st.top > NEG_INF;
+
+    T *grad = a.grad ? (T *)a.grad + (size_t)row * a.d.ld : nullptr;
+    if (!counted) {
+        if (lane == 0) policy_row_out(a, row, false, 0.0f, 0.0, 0.0);
+        if (grad) {
+            vec zero = {};
+#pragma unroll
+            for (int k = 0; k < K; k++) store_chunk<T>(grad, (lane + k * G) * V, width, zero);
+        }
+        return;
+    }
+    RowGrad g;
+    double logp, kl;
+    float loss, grad_taken;
+    if (policy_scalars(a, row, pr, st, 0.0, FULL, g, logp, kl, loss, grad_taken)) {
+        const double s64 = Group<G>::sum64(sum_again<T, G>(z, mask, width, lane, st.top), red64);
+        policy_scalars(a, row, pr, st, s64, FULL, g, logp, kl, loss, grad_taken);
+    }
+    if (lane == 0) policy_row_out(a, row, true, loss, logp, kl);
+    if (!grad) return;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        vec out;
+#pragma unroll
+        for (int j = 0; j < V; j++)
+            out[j] = (T)row_grad<FULL>(e[k][j], FULL ? (float)zc[k][j] : 0.0f, FULL ? (float)qc[FULL ? k : 0][j] : 0.0f, g);
+        store_chunk<T>(grad, (lane + k * G) * V, width, out);
+    }
+    // the action taken: written again by the lane that wrote its chunk
+    const int act = a.actions[row];
+    if (lane == (act / V) % G) grad[act] = (T)grad_taken;
+}
+
+// Rows too wide for the registers of a workgroup: running maximum and sums in one pass, the gradient in a second one.
+template <typename T, bool FULL>
+__global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
+    constexpr int V = Row<T>::V;
+    typedef typename Row<T>::vec vec;
+    typedef typename Row<T>::bytes bytes;
+    __shared__ float red[4];
+    __shared__ double red64[4];
+    const long long row64 = row_block();
+    if (row64 >= a.d.batch) return;
+    const int row = (int)row64, lane = threadIdx.x, width = a.d.width;
+    const T *z = (const T *)a.z + (size_t)row * a.d.ld;
+    const T *q = FULL ? (const T *)a.ref + (size_t)row * a.d.ld : nullptr;
+    const uint8_t *mask = a.mask ? a.mask + (size_t)row * a.d.mask_ld : nullptr;
+    const PolicyRow pr = policy_row_begin(a, z, q, mask, row, FULL);
+    float top = NEG_INF, s = 0.0f, ref_top = NEG_INF, sq = 0.0f, cross = 0.0f;
+    for (long long e0 = (long long)lane * V; e0 < width; e0 += 256 * V) {
+        const bytes b = legal_bytes<T>(mask, (int)e0, width);
+        vec zc, qc;
+        load_chunk<T>(z, (int)e0, width, b, zc);
+        keep_legal<T>(b, zc);
+        if (FULL) {
+            load_chunk<T>(q, (int)e0, width, b, qc);
+            keep_legal<T>(b, qc);
+        }
+        float m = top, mq = ref_top;
+        for (int j = 0; j < V; j++) {
+            m = fmaxf(m, (float)zc[j]);
+            if (FULL) mq = fmaxf(mq, (float)qc[j]);
+        }
+        if (m > top) {
+            const float f = exp_neg(top - m);
+            s *= f, cross *= f, top = m;
+        }
+        if (FULL && mq > ref_top) sq *= exp_neg(ref_top - mq), ref_top = mq;
+        const float base = top == NEG_INF ? 0.0f : top;
+        for (int j = 0; j < V; j++) {
+            const float zv = (float)zc[j], e = exp_neg(zv - base);
+            s += e;
+            if (FULL) {
+                const float qv = (float)qc[j];
+                sq += exp_neg(qv - (ref_top == NEG_INF ? 0.0f : ref_top));
+                cross += e == 0.0f ? 0.0f : e * (zv - qv);
+            }
+        }
+    }
+    RowStats st;
+    st.top = Group<256>::max(top, red);
+    const float f = top == NEG_INF ? 0.0f : exp_neg(top - st.top);
+    st.sum = Group<256>::sum(top == NEG_INF ? s : s * f, red);  // (s without a finite maximum: 0 or NaN)
+    st.ref_top = FULL ? Group<256>::max(ref_top, red) : 0.0f;
+    st.ref_sum = FULL ? Group<256>::sum(ref_top == NEG_INF ? sq : sq * exp_neg(ref_top - st.ref_top), red) : 1.0f;
+    st.cross = FULL ? Group<256>::sum(top == NEG_INF ? cross : cross * f, red) : 0.0f;
+    const bool counted = pr.counted && st.top > NEG_INF;
+    T *grad = a.grad ? (T *)a.grad + (size_t)row * a.d.ld : nullptr;
+    RowGrad g;
+    double logp = 0.0, kl = 0.0;
+    float loss = 0.0f, grad_taken = 0.0f;
+    if (counted && policy_scalars(a, row, pr, st, 0.0, FULL, g, logp, kl, loss, grad_taken)) {
+        const double s64 = Group<256>::sum64(sum_again<T, 256>(z, mask, width, lane, st.top), red64);
+        policy_scalars(a, row, pr, st, s64, FULL, g, logp, kl, loss, grad_taken);
+    }
+    if (lane == 0) policy_row_out(a, row, counted, loss, logp, kl);
+    if (!grad) return;
+    for (long long e0 = (long long)lane * V; e0 < width; e0 += 256 * V) {
+        vec out = {};
+        if (counted) {
+            const bytes b = legal_bytes<T>(mask, (int)e0, width);
+            vec zc, qc;
+            load_chunk<T>(z, (int)e0, width, b, zc);
+            keep_legal<T>(b, zc);
+            if (FULL) {
+                load_chunk<T>(q, (int)e0, width, b, qc);
+                keep_legal<T>(b, qc);
+            }
+            for (int j = 0; j < V; j++) {
+                const float zv = (float)zc[j];
+                out[j] = (T)row_grad<FULL>(exp_neg(zv - g.top), zv, FULL ? (float)qc[j] : 0.0f, g);
+            }
+        }
+        store_chunk<T>(grad, (int)e0, width, out);
+    }
+    const int act = a.actions[row];
+    if (counted && lane == (act / V) % 256) grad[act] = (T)grad_taken;
+}
+
+// loss_sum = sum of the rows' losses, in 64 bits and a fixed order
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float *__restrict__ rows, int n, float *__restrict__ out) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (long long i = threadIdx.x; i < n; i += 1024) s += (double)rows[i];
+    for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; i++) s += red[i];
+        out[0] = (float)s;
+    }
+}
+
+// ---- preference loss: row statistics -> pairs -> gradient rows
+struct PrefArgs {
+    const void *z;
+    const uint8_t *mask;
+    const int32_t *actions, *offsets;
+    const float *ref, *weights;
+    void *grad;
+    float *pair_loss, *line_logp;
+    double *logp;  // [rows] log-probability of the action taken, 0 where the row is not counted
+    float *top;    // [rows] largest legal logit
+    float *inv;    // [rows] 1 / sum of exp(z - top), 0 where the row is not counted
+    float *slope;  // [pairs] d loss / d s of the preferred line
+    bt_preference_desc d;
+};
+__device__ __forceinline__ int pref_offset(const PrefArgs &a, int k) { return min(max(a.offsets[k], 0), a.d.rows); }
+
+__device__ __forceinline__ void pref_row_out(const PrefArgs &a, int row, bool counted, float za, float top, float sum) {
+    a.logp[row] = counted ? ((double)za - (double)top) - log((double)sum) : 0.0;
+    a.top[row] = top;
+    a.inv[row] = counted ? (float)(1.0 / (double)sum) : 0.0f;
+}
+
+template <typename T, int G, int K>
+__global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
+    constexpr int V = Row<T>::V;
+    __shared__ float red[4];
+    const int lane = threadIdx.x % G;
+    const long long row64 = row_block() * (256 / G) + threadIdx.x / G;
+    if (row64 < pref_offset(a, 0) || row64 >= pref_offset(a, 2 * a.d.pairs)) return;
+    const int row = (int)row64;
+    const int width = a.d.width;
+    const T *z = (const T *)a.z + (size_t)row * a.d.ld;
+    const uint8_t *mask = a.mask ? a.mask + (size_t)row * a.d.mask_ld : nullptr;
+    const int act = a.actions[row];
+    const bool can = act >= 0 && act < width && (!mask || mask[act]);
+    const float za = can ? (float)z[act] : 0.0f;
+    float top = NEG_INF, s = 0.0f;
+    if (K > 0) {
+        typename Row<T>::bytes b[K ? K : 1];
+        typename Row<T>::vec zc[K ? K : 1];
+#pragma unroll
+        for (int k = 0; k < K; k++) b[k] = legal_bytes<T>(mask, (lane + k * G) * V, width);
+#pragma unroll
+        for (int k = 0; k < K; k++) load_chunk<T>(z, (lane + k * G) * V, width, b[k], zc[k]);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            keep_legal<T>(b[k], zc[k]);
+#pragma unroll
+            for (int j = 0; j < V; j++) top = fmaxf(top, (float)zc[k][j]);
+        }
+        top = Group<G>::max(top, red);
+        const float base = top == NEG_INF ? 0.0f : top;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int j = 0; j < V; j++) s += exp_neg((float)zc[k][j] - base);
+        s = Group<G>::sum(s, red);
+    } else {  // any width: running maximum and sum
+        for (long long e0 = (long long)lane * V; e0 < width; e0 += G * V) {
+            const typename Row<T>::bytes b = legal_bytes<T>(mask, (int)e0, width);
+            typename Row<T>::vec zc;
+            load_chunk<T>(z, (int)e0, width, b, zc);
+            keep_legal<T>(b, zc);
+            float m = top;
+            for (int j = 0; j < V; j++) m = fmaxf(m, (float)zc[j]);
+            if (m > top) s *= exp_neg(top - m), top = m;
+            const float base = top == NEG_INF ? 0.0f : top;
+            for (int j = 0; j < V; j++) s += exp_neg((float)zc[j] - base);
+        }
+        const float all = Group<G>::max(top, red);
+        s = Group<G>::sum(top == NEG_INF ? s : s * exp_neg(top - all), red);
+        top = all;
+    }
+    if (lane == 0) pref_row_out(a, row, can && top > NEG_INF, za, top, s);
+}
+
+// one wave per pair
+__global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
+    const long long p64 = row_block() * 4 + (threadIdx.x >> 6);
+    const int p = (int)p64, lane = threadIdx.x & 63;
+    if (p64 >= a.d.pairs) return;
+    double s[2];
+    for (int h = 0; h < 2; h++) {
+        const int r1 = pref_offset(a, 2 * p + h + 1);
+        double v = 0.0;
+        for (long long r = pref_offset(a, 2 * p + h) + lane; r < r1; r += 64) v += a.logp[r];
+        for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+        s[h] = v;
+    }
+    if (lane) return;
+    const double beta = a.d.beta, eps = a.d.smoothing, w = a.weights ? (double)a.weights[p] : 1.0;
+    const double x = beta * ((s[0] - (double)a.ref[2 * p]) - (s[1] - (double)a.ref[2 * p + 1]));
+    const double soft = log1p(exp(-fabs(x)));  // -log sigmoid(x) = soft - min(x, 0)
+    a.pair_loss[p] = (float)(w * ((1.0 - eps) * (soft - fmin(x, 0.0)) + eps * (soft + fmax(x, 0.0))));
+    // sigmoid(x) - (1 - eps), written so that nothing cancels for large x
+    a.slope[p] = (float)(w * beta * (eps - 1.0 / (1.0 + exp(x))));
+    if (a.line_logp) a.line_logp[2 * p] = (float)s[0], a.line_logp[2 * p + 1] = (float)s[1];
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void pref_grad(PrefArgs a) {
+    constexpr int V = Row<T>::V;
+    const int lane = threadIdx.x % G;
+    const long long row64 = row_block() * (256 / G) + threadIdx.x / G;
+    if (row64 < pref_offset(a, 0) || row64 >= pref_offset(a, 2 * a.d.pairs)) return;
+    const int row = (int)row64;
+    int lo = 0, hi = 2 * a.d.pairs;  // offsets[lo] <= row < offsets[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pref_offset(a, mid) <= row)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const float top = a.top[row], inv = a.inv[row];
+    const float ca = (lo & 1) ? -a.slope[lo >> 1] : a.slope[lo >> 1];
+    const bool counted = inv != 0.0f;
+    const int width = a.d.width;
+    const T *z = (const T *)a.z + (size_t)row * a.d.ld;
+    const uint8_t *mask = a.mask ? a.mask + (size_t)row * a.d.mask_ld : nullptr;
+    T *grad = (T *)a.grad + (size_t)row * a.d.ld;
+    const RowGrad g{top, inv, ca, 0.0f, 0.0f};
+    for (long long e0 = (long long)lane * V; e0 < width; e0 += G * V) {
+        typename Row<T>::vec out = {};
+        if (counted) {
+            const typename Row<T>::bytes b = legal_bytes<T>(mask, (int)e0, width);
+            typename Row<T>::vec zc;
+            load_chunk<T>(z, (int)e0, width, b, zc);
+            keep_legal<T>(b, zc);
+#pragma unroll
+            for (int j = 0; j < V; j++) out[j] = (T)row_grad<false>(exp_neg((float)zc[j] - top), 0.0f, 0.0f, g);
+        }
+        store_chunk<T>(grad, (int)e0, width, out);
+    }
+    const int act = a.actions[row];
+    if (counted && lane == (act / V) % G) grad[act] = (T)((double)ca * (1.0 - exp(a.logp[row])));
+}
+
+// ---- host side
+int type_size(int type) { return type == BT_TYPE_F32 ? 4 : 2; }
+bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+int matrix_validate(const char *fn, int type, int width, int ld, int mask_ld, bool mask) {
+    BT_REQUIRE(type == BT_TYPE_F32 || type == BT_TYPE_BF16 || type == BT_TYPE_F16, "%s: unknown element type %d", fn, type);
+    BT_REQUIRE(width > 0, "%s: Mismatched sizes! (width <= 0)", fn);
+    BT_REQUIRE(ld >= width, "%s: Mismatched sizes! (leading dimension %d < width %d)", fn, ld, width);
+    BT_REQUIRE(!mask || mask_ld >= width, "%s: Mismatched sizes! (mask leading dimension %d < width %d)", fn, mask_ld, width);
+    return BT_OK;
+}
+
+// Lanes per row and chunks per lane. A row stays in one wave's registers up to 8 chunks a lane (2048 f32 or 4096 16-bit
+// elements), in a workgroup's up to 4 times that; rows of at most 8 chunks share a wave.
+#define ROW_SHAPES(X)                       \
+    if (chunks <= 8) X(8, 1)                \
+    else if (chunks <= 64) X(64, 1)         \
+    else if (chunks <= 128) X(64, 2)        \
+    else if (chunks <= 256) X(64, 4)        \
+    else if (chunks <= 512) X(64, 8)        \
+    else if (chunks <= 1024) X(256, 4)      \
+    else if (chunks <= 2048) X(256, 8)
+
+template <typename T, bool FULL>
+int policy_launch(hipStream_t s, const PolicyArgs &a) {
+    const int chunks = bt_div_up(a.d.width, Row<T>::V);
+#define POLICY_CASE(G, K) \
+    BT_LAUNCH(BTK_POLICY, s, (policy_rows<T, G, K, FULL>), row_grid(bt_div_up(a.d.batch, 256 / G)), dim3(256), 0, a);
+    ROW_SHAPES(POLICY_CASE)
+    else BT_LAUNCH(BTK_POLICY, s, (policy_rows_long<T, FULL>), row_grid(a.d.batch), dim3(256), 0, a);
+#undef POLICY_CASE
+    BT_LAUNCH_CHECK();
+    return BT_OK;
+}
+template <typename T>
+int policy_launch(hipStream_t s, const PolicyArgs &a) {
+    return a.d.kl == BT_KL_FULL ? policy_launch<T, true>(s, a) : policy_launch<T, false>(s, a);
+}
+
+template <typename T>
+int pref_launch(hipStream_t s, const PrefArgs &a) {
+    const int chunks = bt_div_up(a.d.width, Row<T>::V);
+    if (a.d.rows > 0) {
+#define PREF_CASE(G, K) BT_LAUNCH(BTK_POLICY, s, (pref_rows<T, G, K>), row_grid(bt_div_up(a.d.rows, 256 / G)), dim3(256), 0, a);
+        ROW_SHAPES(PREF_CASE)
+        else BT_LAUNCH(BTK_POLICY, s, (pref_rows<T, 256, 0>), row_grid(a.d.rows), dim3(256), 0, a);
+#undef PREF_CASE
+        BT_LAUNCH_CHECK();
+    }
+    BT_LAUNCH(BTK_POLICY, s, pref_pairs, row_grid(bt_div_up(a.d.pairs, 4)), dim3(256), 0, a);
+    BT_LAUNCH_CHECK();
+    if (a.grad && a.d.rows > 0) {
+        if (chunks <= 8)
+            BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 8>), row_grid(bt_div_up(a.d.rows, 32)), dim3(256), 0, a);
+        else if (chunks <= 512)
+            BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 64>), row_grid(bt_div_up(a.d.rows, 4)), dim3(256), 0, a);
+        else
+            BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 256>), row_grid(a.d.rows), dim3(256), 0, a);
+        BT_LAUNCH_CHECK();
+    }
+    return BT_OK;
+}
+
+int pref_validate(const bt_preference_desc *d, const char *fn, bool mask) {
+    BT_REQUIRE(d, "%s: null pointer", fn);
+    BT_REQUIRE(d->pairs > 0 && d->pairs <= (1 << 29), "%s: Mismatched sizes! (pairs = %d)", fn, d->pairs);
+    BT_REQUIRE(d->rows >= 0, "%s: Mismatched sizes! (rows < 0)", fn);
+    if (int rc = matrix_validate(fn, d->type, d->width, d->ld, d->mask_ld, mask)) return rc;
+    BT_REQUIRE(d->beta >= 0.0f && d->beta <= 3.0e38f, "%s: beta = %g must not be negative", fn, d->beta);
+    BT_REQUIRE(d->smoothing >= 0.0f && d->smoothing < 0.5f, "%s: smoothing = %g is outside [0, 0.5)", fn, d->smoothing);
+    return BT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int bt_policy_loss(void *stream, const bt_policy_desc *d, const void *logits, const uint8_t *mask, const int32_t *actions,
+                   const float *old_logp, const float *advantages, const void *ref, const float *row_weights,
+                   float *loss_sum, void *grad, float *row_loss, float *row_logp, float *row_kl) {
+    BT_REQUIRE(d, "bt_policy_loss: null pointer");
+    BT_REQUIRE(d->batch > 0, "bt_policy_loss: Mismatched sizes! (batch <= 0)");
+    if (int rc = matrix_validate("bt_policy_loss", d->type, d->width, d->ld, d->mask_ld, mask)) return rc;
+    BT_REQUIRE(d->kl == BT_KL_NONE || d->kl == BT_KL_TAKEN || d->kl == BT_KL_FULL, "bt_policy_loss: unknown KL kind %d", d->kl);
+    BT_REQUIRE(d->clip_low >= 0.0f && d->clip_low <= 1.0f && d->clip_high >= 0.0f && d->clip_high <= 3.0e38f,
+               "bt_policy_loss: clipping range (%g, %g) is not one", d->clip_low, d->clip_high);
+    BT_REQUIRE(d->kl_weight >= 0.0f && d->kl_weight <= 3.0e38f, "bt_policy_loss: kl_weight = %g must not be negative",
+               d->kl_weight);
+    BT_REQUIRE(logits && actions && old_logp && advantages && loss_sum && row_loss, "bt_policy_loss: null pointer");
+    BT_REQUIRE(d->kl == BT_KL_NONE || ref, "bt_policy_loss: this KL term needs the reference policy");
+    const size_t es = type_size(d->type);
+    BT_REQUIRE(aligned(logits, es) && aligned(grad, es) && (d->kl == BT_KL_NONE || aligned(ref, d->kl == BT_KL_FULL ? es : 4)),
+               "bt_policy_loss: a buffer is not aligned to its element type");
+    BT_REQUIRE(d->kl != BT_KL_FULL || ref != grad || !grad, "bt_policy_loss: grad must not be the reference logits");
+    PolicyArgs a{logits, ref, mask, actions, old_logp, advantages, row_weights, grad, row_loss, row_logp, row_kl, *d};
+    hipStream_t s = bt_stream(stream);
+    if (int rc = d->type == BT_TYPE_F32    ? policy_launch<float>(s, a)
+                 : d->type == BT_TYPE_BF16 ? policy_launch<__bf16>(s, a)
+                                           : policy_launch<_Float16>(s, a))
+        return rc;
+    BT_LAUNCH(BTK_POLICY, s, loss_sum_kernel, dim3(1), dim3(1024), 0, row_loss, d->batch, loss_sum);
+    BT_LAUNCH_CHECK();
+    return BT_OK;
+}
+
+size_t bt_preference_loss_workspace_bytes(const bt_preference_desc *d) {
+    if (pref_validate(d, "bt_preference_loss_workspace_bytes", false)) return 0;
+    return bt_align((size_t)d->rows * 8) + 2 * bt_align((size_t)d->rows * 4) + bt_align((size_t)d->pairs * 4);
+}
+
+int bt_preference_loss(void *stream, const bt_preference_desc *d, const void *logits, const uint8_t *mask,
+                       const int32_t *actions, const int32_t *offsets, const float *ref_logp, const float *pair_weights,
+                       float *loss_sum, void *grad, float *pair_loss, float *line_logp, void *workspace,
+                       size_t workspace_bytes) {
+    if (int rc = pref_validate(d, "bt_preference_loss", mask)) return rc;
+    BT_REQUIRE(offsets && ref_logp && loss_sum && pair_loss && workspace, "bt_preference_loss: null pointer");
+    BT_REQUIRE(d->rows == 0 || (logits && actions), "bt_preference_loss: null pointer");
+    BT_REQUIRE(workspace_bytes >= bt_preference_loss_workspace_bytes(d), "bt_preference_loss: workspace too small");
+    BT_REQUIRE(aligned(workspace, 8), "bt_preference_loss: workspace is not aligned to 8 bytes");
+    const size_t es = type_size(d->type);
+    BT_REQUIRE(aligned(logits, es) && aligned(grad, es), "bt_preference_loss: a buffer is not aligned to its element type");
+    char *ws = static_cast<char *>(workspace);
+    PrefArgs a{logits, mask, actions, offsets, ref_logp, pair_weights, grad, pair_loss, line_logp, nullptr, nullptr, nullptr,
+               nullptr, *d};
+    a.logp = reinterpret_cast<double *>(ws), ws += bt_align((size_t)d->rows * 8);
+    a.top = reinterpret_cast<float *>(ws), ws += bt_align((size_t)d->rows * 4);
+    a.inv = reinterpret_cast<float *>(ws), ws += bt_align((size_t)d->rows * 4);
+    a.slope = reinterpret_cast<float *>(ws);
+    hipStream_t s = bt_stream(stream);
+    if (int rc = d->type == BT_TYPE_F32    ? pref_launch<float>(s, a)
+                 : d->type == BT_TYPE_BF16 ? pref_launch<__bf16>(s, a)
+                                           : pref_launch<_Float16>(s, a))
+        return rc;
+    BT_LAUNCH(BTK_POLICY, s, loss_sum_kernel, dim3(1), dim3(1024), 0, pair_loss, d->pairs, loss_sum);
+    BT_LAUNCH_CHECK();
+    return BT_OK;
+}
+
+}  // extern "C"

@@ -26,6 +26,20 @@ class DenseDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("batch", "in_", "out", "buckets", "act")]
 
 
+class PolicyDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("batch", "width", "type", "ld", "mask_ld", "kl")] + \
+               [(n, C.c_float) for n in ("clip_low", "clip_high", "kl_weight")]
+
+
+class PreferenceDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("pairs", "rows", "width", "type", "ld", "mask_ld")] + \
+               [(n, C.c_float) for n in ("beta", "smoothing")]
+
+
+TYPE = {"f32": 0, "bf16": 1, "f16": 2}
+KL = {"none": 0, "taken": 1, "full": 2}
+
+
 class AdamwTensor(C.Structure):
     _fields_ = [("grad", C.c_void_p), ("param", C.c_void_p), ("momentum", C.c_void_p), ("velocity", C.c_void_p),
                 ("n", C.c_size_t), ("decay", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float),
@@ -156,6 +170,7 @@ SYMBOLS = [
     "bt_dense_forward", "bt_dense_backward_workspace_bytes", "bt_dense_backward", "bt_dense_backward_static",
     "bt_sigmoid_mse", "bt_loss", "bt_adamw", "bt_radam", "bt_lookahead", "bt_weight_clip", "bt_weight_decay",
     "bt_clip_pass_through", "bt_faux_quantise",
+    "bt_policy_loss", "bt_preference_loss_workspace_bytes", "bt_preference_loss",
     "bt_net_set_optimiser",
     "bt_net_param_count", "bt_net_num_tensors", "bt_net_tensor_size", "bt_net_tensor_offset", "bt_net_create",
     "bt_net_destroy", "bt_net_params", "bt_net_grads", "bt_net_momentum", "bt_net_velocity", "bt_net_set_adamw",
@@ -189,6 +204,7 @@ def load():
     L.bt_profile_set_filter.argtypes = [C.c_ulonglong]
     L.bt_profile_stop.argtypes = [C.POINTER(C.c_int), C.POINTER(C.c_double), C.c_int]
     for f in ("bt_ft_backward_workspace_bytes", "bt_dense_backward_workspace_bytes", "bt_net_param_count",
+              "bt_preference_loss_workspace_bytes",
               "bt_net_tensor_size", "bt_net_tensor_offset", "bt_net_flat_size"):
         getattr(L, f).restype = C.c_size_t
     for f in ("bt_net_params", "bt_net_grads", "bt_net_momentum", "bt_net_velocity"):
@@ -240,6 +256,9 @@ def load():
     L.bt_sigmoid_mse.argtypes = [C.c_void_p, C.c_int] + [C.c_void_p] * 5
     L.bt_loss.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_float,
                           C.c_void_p, C.c_void_p]
+    L.bt_policy_loss.argtypes = [C.c_void_p, C.POINTER(PolicyDesc)] + [C.c_void_p] * 12
+    L.bt_preference_loss_workspace_bytes.argtypes = [C.POINTER(PreferenceDesc)]
+    L.bt_preference_loss.argtypes = [C.c_void_p, C.POINTER(PreferenceDesc)] + [C.c_void_p] * 11 + [C.c_size_t]
     L.bt_weight_clip.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_float, C.c_float]
     L.bt_weight_decay.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_float, C.c_void_p]
     L.bt_clip_pass_through.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_float, C.c_float]

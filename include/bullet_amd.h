@@ -264,6 +264,72 @@ int bt_clip_pass_through(void *stream, const float *x, float *y, size_t n, float
 int bt_faux_quantise(void *stream, const float *x, float *y, size_t n, float value, int round);
 
 /* ------------------------------------------------------------------------------------------
+ * 2b. Policy heads (no counterpart in the reference, whose nets end in 1 or 3 outputs): two losses on the move logits,
+ *     each with its gradient, and the wide layer that makes the logits.
+ *
+ * Element types of the matrices: f32, bf16 or f16. Sums, softmax statistics and losses are always held in 32 bits or
+ * more. Matrices are row-major with a leading dimension in elements (rows `ld` apart, ld >= width); elements between two
+ * rows are neither used nor written. Buffers need the alignment of their element type only; 16-byte aligned buffers with
+ * leading dimensions that are multiples of 16 bytes are faster. All calls are enqueue-only on `stream`, allocate nothing
+ * and may be captured into a graph. Results are the same from run to run.
+ * ------------------------------------------------------------------------------------------ */
+enum { BT_TYPE_F32 = 0, BT_TYPE_BF16 = 1, BT_TYPE_F16 = 2 };
+
+/* Clipped policy loss with a KL term. Row b holds the logits of one position's moves; p = softmax over its legal moves,
+ * l = log p, a = actions[b], r = exp(l[a] - old_logp[b]), A = advantages[b]:
+ *   row_loss[b] = weight[b] * ( -min(r A, min(max(r, 1 - clip_low), 1 + clip_high) A) + kl_weight * KL )
+ *   loss_sum[0] = sum over rows of row_loss;   grad = d loss_sum / d logits
+ *   BT_KL_NONE   KL = 0 (ref is ignored)
+ *   BT_KL_TAKEN  KL = exp(d) - d - 1, d = ref[b] - l[a]; ref: F32[batch] log-probability of a under the reference policy
+ *   BT_KL_FULL   KL = sum over legal moves j of p[j] (l[j] - lref[j]); ref: the reference policy's logits, same type, ld
+ *                and mask as `logits` (lref: their log-softmax over the legal moves); no gradient goes into it
+ * mask: U8[batch*mask_ld], non-zero = legal, or NULL = every move is legal. What stands in masked places (infinities, NaN)
+ * has no effect. actions: I32[batch]. A row is not counted (loss, gradient, row outputs all exactly 0) if its action is
+ * outside [0, width) (-1 marks padding), is masked, or if no legal logit is above -infinity. grad of masked places is 0.
+ * The gradient passes where r A is not above its clipped value. NaN or +infinity in a legal place makes its row's loss NaN,
+ * and so do reference logits that leave a counted row nothing above -infinity.
+ * row_weights F32[batch] or NULL = 1. Outputs: loss_sum F32[1] (overwritten, un-normalised, as bt_loss); grad (type and
+ * ld of logits; may be the logits themselves, or NULL = loss only); row_loss F32[batch]; row_logp (l[a]) and row_kl (KL):
+ * F32[batch] or NULL. */
+enum { BT_KL_NONE = 0, BT_KL_TAKEN = 1, BT_KL_FULL = 2 };
+typedef struct {
+    int batch;   /* rows */
+    int width;   /* moves per row, legal or not */
+    int type;    /* BT_TYPE_* of logits, reference logits, grad */
+    int ld;      /* elements from row to row of logits, reference logits and grad (>= width) */
+    int mask_ld; /* bytes from row to row of mask (>= width; ignored without a mask) */
+    int kl;      /* BT_KL_* */
+    float clip_low, clip_high; /* >= 0, clip_low <= 1 */
+    float kl_weight;           /* >= 0 */
+} bt_policy_desc;
+int bt_policy_loss(void *stream, const bt_policy_desc *desc, const void *logits, const uint8_t *mask, const int32_t *actions,
+                   const float *old_logp, const float *advantages, const void *ref, const float *row_weights,
+                   float *loss_sum, void *grad, float *row_loss, float *row_logp, float *row_kl);
+
+/* Preference loss over pairs of lines of moves. Line k (0 <= k < 2*pairs) is the rows offsets[k] <= row < offsets[k+1];
+ * line 2p is the preferred one of pair p, line 2p+1 the other. With l as above, s_k = sum over line k's counted rows of
+ * l[a] (a row whose action is outside [0, width) or masked, or without a legal move, adds nothing and gets no gradient) and
+ *   d = beta * ((s_2p - ref_2p) - (s_2p+1 - ref_2p+1)),  ref_logp F32[2*pairs]: the lines' s under the reference policy
+ *   pair_loss[p] = weight[p] * ( -(1 - smoothing) log sigmoid(d) - smoothing log sigmoid(-d) )
+ *   loss_sum[0] = sum of pair_loss;   grad = d loss_sum / d logits
+ * offsets: I32[2*pairs + 1] on the device, not decreasing, within [0, rows] (values outside are taken as the nearest
+ * bound). Rows in front of the first line and behind the last are neither read nor written: `grad` keeps what it held.
+ * pair_weights F32[pairs] or NULL = 1; grad may be the logits themselves, or NULL; pair_loss F32[pairs]; line_logp (s):
+ * F32[2*pairs] or NULL. */
+typedef struct {
+    int pairs;
+    int rows;    /* rows of logits, mask, actions and grad */
+    int width, type, ld, mask_ld; /* as in bt_policy_desc */
+    float beta;
+    float smoothing; /* 0 <= smoothing < 0.5 */
+} bt_preference_desc;
+size_t bt_preference_loss_workspace_bytes(const bt_preference_desc *desc);
+int bt_preference_loss(void *stream, const bt_preference_desc *desc, const void *logits, const uint8_t *mask,
+                       const int32_t *actions, const int32_t *offsets, const float *ref_logp, const float *pair_weights,
+                       float *loss_sum, void *grad, float *pair_loss, float *line_logp, void *workspace,
+                       size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------------------------
  * 3. The lowered training step for the ValueTrainerBuilder net family
  *    (crates/bullet_lib/src/value/builder.rs:118-181; step = run.rs:185-221)
  * ------------------------------------------------------------------------------------------ */
