@@ -26,6 +26,10 @@ class DenseDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("batch", "in_", "out", "buckets", "act")]
 
 
+class AffineDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("batch", "in_", "out", "act", "type", "w_type", "w_ld", "x_ld", "y_ld")]
+
+
 class PolicyDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("batch", "width", "type", "ld", "mask_ld", "kl")] + \
                [(n, C.c_float) for n in ("clip_low", "clip_high", "kl_weight")]
@@ -170,6 +174,7 @@ SYMBOLS = [
     "bt_dense_forward", "bt_dense_backward_workspace_bytes", "bt_dense_backward", "bt_dense_backward_static",
     "bt_sigmoid_mse", "bt_loss", "bt_adamw", "bt_radam", "bt_lookahead", "bt_weight_clip", "bt_weight_decay",
     "bt_clip_pass_through", "bt_faux_quantise",
+    "bt_affine_forward_workspace_bytes", "bt_affine_forward", "bt_affine_backward_workspace_bytes", "bt_affine_backward",
     "bt_policy_loss", "bt_preference_loss_workspace_bytes", "bt_preference_loss",
     "bt_net_set_optimiser",
     "bt_net_param_count", "bt_net_num_tensors", "bt_net_tensor_size", "bt_net_tensor_offset", "bt_net_create",
@@ -204,7 +209,8 @@ def load():
     L.bt_profile_set_filter.argtypes = [C.c_ulonglong]
     L.bt_profile_stop.argtypes = [C.POINTER(C.c_int), C.POINTER(C.c_double), C.c_int]
     for f in ("bt_ft_backward_workspace_bytes", "bt_dense_backward_workspace_bytes", "bt_net_param_count",
-              "bt_preference_loss_workspace_bytes",
+              "bt_preference_loss_workspace_bytes", "bt_affine_forward_workspace_bytes",
+              "bt_affine_backward_workspace_bytes",
               "bt_net_tensor_size", "bt_net_tensor_offset", "bt_net_flat_size"):
         getattr(L, f).restype = C.c_size_t
     for f in ("bt_net_params", "bt_net_grads", "bt_net_momentum", "bt_net_velocity"):
@@ -256,6 +262,10 @@ def load():
     L.bt_sigmoid_mse.argtypes = [C.c_void_p, C.c_int] + [C.c_void_p] * 5
     L.bt_loss.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_float,
                           C.c_void_p, C.c_void_p]
+    L.bt_affine_forward_workspace_bytes.argtypes = [C.POINTER(AffineDesc)]
+    L.bt_affine_backward_workspace_bytes.argtypes = [C.POINTER(AffineDesc)]
+    L.bt_affine_forward.argtypes = [C.c_void_p, C.POINTER(AffineDesc)] + [C.c_void_p] * 7 + [C.c_size_t]
+    L.bt_affine_backward.argtypes = [C.c_void_p, C.POINTER(AffineDesc)] + [C.c_void_p] * 8 + [C.c_size_t]
     L.bt_policy_loss.argtypes = [C.c_void_p, C.POINTER(PolicyDesc)] + [C.c_void_p] * 12
     L.bt_preference_loss_workspace_bytes.argtypes = [C.POINTER(PreferenceDesc)]
     L.bt_preference_loss.argtypes = [C.c_void_p, C.POINTER(PreferenceDesc)] + [C.c_void_p] * 11 + [C.c_size_t]

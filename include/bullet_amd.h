@@ -275,6 +275,35 @@ int bt_faux_quantise(void *stream, const float *x, float *y, size_t n, float val
  * ------------------------------------------------------------------------------------------ */
 enum { BT_TYPE_F32 = 0, BT_TYPE_BF16 = 1, BT_TYPE_F16 = 2 };
 
+/* Wide affine layer: y = act(x W^T + bias) + residual, and its gradients, on the matrix cores with 32-bit sums. (Layers of
+ * a few outputs per bucket, f32: bt_dense_*.)
+ * w: column-major as everywhere here, w[o + w_ld*i] is the weight of input i for output o; F32 or `type` (w_type). f32
+ * weights of a 16-bit layer are rounded to `type` (to nearest even) before they are used, so a caller may pass the
+ * optimiser's own copy. bias: F32[out] or NULL. x, grad_x: rows x_ld apart; residual, y, saved, out, grad_y: rows y_ld
+ * apart. residual may be NULL, and y may be the residual's own buffer. saved (NULL allowed) receives act(x W^T + bias), what
+ * the backward pass needs where a residual was added. Each output is rounded once, from 32 bits.
+ * A workspace is needed for some shapes (bt_affine_forward_workspace_bytes says how much; 0: may be NULL). */
+typedef struct {
+    int batch, in, out;
+    int act;    /* BT_ACT_* */
+    int type;   /* BT_TYPE_* of x, residual, y, saved, out, grad_y, grad_x */
+    int w_type; /* BT_TYPE_F32 or `type` */
+    int w_ld;   /* elements from input to input of w and dw (>= out) */
+    int x_ld;   /* elements from row to row (>= in) */
+    int y_ld;   /* elements from row to row (>= out) */
+} bt_affine_desc;
+size_t bt_affine_forward_workspace_bytes(const bt_affine_desc *desc);
+int bt_affine_forward(void *stream, const bt_affine_desc *desc, const void *w, const float *bias, const void *x,
+                      const void *residual, void *y, void *saved, void *workspace, size_t workspace_bytes);
+/* gz = grad_y * act'(.), the derivative taken from `out`, the activation's output (y, or saved if there was a residual;
+ * ignored and NULL allowed for BT_ACT_IDENTITY); dw = sum over rows of gz x, dbias = sum of gz, grad_x = gz W. A residual's
+ * gradient is grad_y itself. dw: F32, layout of w, dbias: F32[out] (for bt_adamw; both overwritten); each of dw, dbias,
+ * grad_x may be NULL. 16-bit layers keep gz in 16 bits where that loses nothing (the derivative is 0 or 1) and as a pair
+ * of 16-bit numbers where it would (SCReLU, squared ReLU); squared ReLU of f16 is refused, since gz can leave its range. */
+size_t bt_affine_backward_workspace_bytes(const bt_affine_desc *desc);
+int bt_affine_backward(void *stream, const bt_affine_desc *desc, const void *w, const void *x, const void *out,
+                       const void *grad_y, float *dw, float *dbias, void *grad_x, void *workspace, size_t workspace_bytes);
+
 /* Clipped policy loss with a KL term. Row b holds the logits of one position's moves; p = softmax over its legal moves,
  * l = log p, a = actions[b], r = exp(l[a] - old_logp[b]), A = advantages[b]:
  *   row_loss[b] = weight[b] * ( -min(r A, min(max(r, 1 - clip_low), 1 + clip_high) A) + kl_weight * KL )
