@@ -86,7 +86,7 @@ struct Tile {
 
 // An operand in memory: `rows` rows of `len` contiguous elements, `ld` apart.
 struct Operand {
-    const void *p[2];  // two summands of one product (the pair a 16-bit gradient may be kept in), or the same twice
+    const void *p[3];  // the summands that a 16-bit gradient may be kept as, or the same matrix three times
     long long ld;
     int rows, len;
     int aligned;  // every chunk of every row starts on 16 bytes
@@ -145,12 +145,24 @@ __device__ __forceinline__ void finish4(const Epilogue &e, int row, int c, int n
         store4<T>((T *)e.out + at, v * e.alpha, n);
     } else {
         if (e.bias) {
+            v4f b = {0, 0, 0, 0};
+            if (n >= 4) {
+                __builtin_memcpy(&b, e.bias + c, 16);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j < n) v[j] += e.bias[c + j];
+                for (int j = 0; j < 4; j++)
+                    if (j < n) b[j] = e.bias[c + j];
+            }
+            v += b;
         }
+        // bt_act_fwd without its branches: this is unrolled over a whole tile
+        const float top = e.act == BT_ACT_CRELU || e.act == BT_ACT_SCRELU ? 1.0f : __builtin_huge_valf();
+        const bool clamp = e.act != BT_ACT_IDENTITY, square = e.act == BT_ACT_SCRELU || e.act == BT_ACT_SQRRELU;
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = bt_act_fwd(e.act, v[j]);
+        for (int j = 0; j < 4; j++) {
+            const float a = fminf(fmaxf(v[j], 0.0f), top), b = square ? a * a : a;
+            v[j] = clamp ? b : v[j];
+        }
         if (e.saved) store4<T>((T *)e.saved + at, v, n);
         if (e.residual) {
             const T *r = (const T *)e.residual + at;
@@ -172,7 +184,8 @@ __device__ __forceinline__ void finish4(const Epilogue &e, int row, int c, int n
 struct Product {
     Operand a, b;
     int m, n, k;
-    int passes;          // 1, or 2: both summands of the operands, one after the other
+    int passes;          // summands of the operands, taken one after the other
+    float rescale;       // what the sums of the first summand's products are multiplied by before the next one's
     int tiles_m, tiles_n;
     int splits;          // workgroups that share one tile's k, each leaving its sums in `part`
     float *part;         // [splits][m][part_ld]
@@ -180,21 +193,95 @@ struct Product {
     Epilogue e;
 };
 
-// BM x BN tile by 4 waves of BM/2 x BN/2. Double-buffered LDS: the next tile is on its way while this one is multiplied.
-template <typename T, int BM, int BN, bool AK, bool BKC, int OUT>
-__global__ __launch_bounds__(256) void affine_mm(Product P) {
+// A chunk straight from memory into LDS, 16 bytes a lane: lane l's lands 16 l bytes behind `lds` (the same in all lanes).
+// Written out, since the compiler lets every LDS read wait for all such loads of its own; wait_loads() is the wait, in
+// front of the barrier behind which the chunk is read. The s_nop is the wait state between m0 and its use.
+__device__ __forceinline__ void to_lds(const char *base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" : : "v"(offset), "s"(lds), "s"(base) : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
+}
+
+// One operand's way into LDS, for a workgroup of NT threads. With DMA the chunks of a tile that lies wholly inside the
+// matrix go there directly; a tile that ends with k, or whose span ends inside a chunk, is loaded chunk by chunk with
+// zeros where there is nothing. (Rows of m or n beyond the end are taken from the last row: their sums are not stored.)
+template <typename T, bool KC, int SPAN, int NT, bool DMA>
+struct Stage {
+    typedef Tile<T, KC, SPAN> L;
+    static constexpr int V = Elem<T>::V, BK = Elem<T>::BK, N = L::SLOTS / NT;
+    uint32_t off[DMA ? N : 1];
+    v4u r[DMA ? 1 : N];
+    bool inside;
+    __device__ __forceinline__ void begin(const Operand &o, int s0, int tid) {
+        if constexpr (DMA) {
+            const int left = (KC ? o.rows : o.len) - s0;  // > 0
+            inside = KC || left >= SPAN || o.len % V == 0;
+#pragma unroll
+            for (int q = 0; q < N; q++) {
+                const int s = q * NT + tid;
+                int row = s / L::CPR, c = L::swizzle(row, s % L::CPR);
+                if (KC) row = min(row, left - 1);
+                if (!KC) c = max(min(c, left / V - 1), 0);
+                off[q] = (uint32_t)row * (uint32_t)(o.ld * sizeof(T)) + c * 16;
+            }
+        }
+    }
+    __device__ __forceinline__ v4u chunk(const Operand &o, int pass, int s0, int k0, int s) const {
+        const int row = s / L::CPR, c = L::swizzle(row, s % L::CPR);
+        return load_chunk<T>((const T *)o.p[pass], o, (KC ? s0 : k0) + row, (long long)(KC ? k0 : s0) + c * V);
+    }
+    // issue the tile at k0 of a summand; without DMA it waits in registers until put()
+    __device__ __forceinline__ void get(const Operand &o, int pass, int s0, int k0, int tid, char *lds) {
+        if constexpr (DMA) {
+            if (inside && (KC ? o.len : o.rows) - k0 >= BK) {
+                const char *base = (const char *)o.p[pass] +
+                                   ((KC ? s0 : k0) * (size_t)o.ld + (KC ? k0 : s0)) * sizeof(T);
+                const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (tid & ~63) * 16);
+#pragma unroll
+                for (int q = 0; q < N; q++) to_lds(base, off[q], to + q * NT * 16);
+            } else {
+#pragma unroll 1
+                for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = chunk(o, pass, s0, k0, q * NT + tid);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < N; q++) r[q] = chunk(o, pass, s0, k0, q * NT + tid);
+        }
+    }
+    __device__ __forceinline__ void put(int tid, char *lds) const {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = r[q];
+        }
+    }
+};
+
+// Which tile a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an L2 of its own: every XCD gets a
+// contiguous share of the tiles, and walks it in bands of 8 tiles of m so that what it holds of both operands is reused.
+__device__ __forceinline__ void tile_of(int wg, int wgs, int tiles_m, int tiles_n, int &split, int &tm, int &tn) {
+    const int per = wgs / 8, rest = wgs % 8, xcd = wg % 8;
+    wg = xcd * per + min(xcd, rest) + wg / 8;
+    const int tiles = tiles_m * tiles_n;
+    split = wg / tiles;
+    const int t = wg % tiles, band = t / (8 * tiles_n), in = t % (8 * tiles_n), high = min(8, tiles_m - band * 8);
+    tm = band * 8 + in % high, tn = in / high;
+}
+
+// BM x BN tile by WM x WN waves. Double-buffered LDS: the next tile is on its way while this one is multiplied.
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, bool DMA>
+__global__ __launch_bounds__(64 * WM * WN) void affine_mm(Product P) {
+    constexpr int NT = 64 * WM * WN;
     typedef Tile<T, AK, BM> TA;
     typedef Tile<T, BKC, BN> TB;
-    constexpr int BK = Elem<T>::BK, V = Elem<T>::V;
-    constexpr int FM = BM / 32, FN = BN / 32;
-    constexpr int NA = TA::SLOTS / 256, NB = TB::SLOTS / 256;
-    __shared__ __align__(16) char lds[2][TA::BYTES + TB::BYTES];
+    constexpr int BK = Elem<T>::BK;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    extern __shared__ __align__(16) char lds[];  // 2 x (TA::BYTES + TB::BYTES)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave >> 1, wn = wave & 1;
-    const int tiles = P.tiles_m * P.tiles_n;
-    const int split = blockIdx.x / tiles;
-    int t = blockIdx.x % tiles;
-    const int tm = t / P.tiles_n, tn = t % P.tiles_n;
+    const int wm = wave / WN, wn = wave % WN;
+    int split, tm, tn;
+    tile_of(blockIdx.x, gridDim.x, P.tiles_m, P.tiles_n, split, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int ktiles = (P.k + BK - 1) / BK, all = ktiles * P.passes;
     const int t0 = (int)((long long)all * split / P.splits), t1 = (int)((long long)all * (split + 1) / P.splits);
@@ -204,30 +291,31 @@ __global__ __launch_bounds__(256) void affine_mm(Product P) {
     for (int i = 0; i < FN; i++)
 #pragma unroll
         for (int j = 0; j < FM; j++) acc[i][j] = v4f{0, 0, 0, 0};
-
-    v4u ra[NA], rb[NB];
-    auto load = [&](int kt) {
-        const int pass = kt >= ktiles, k0 = (kt - pass * ktiles) * BK;
+    auto rescale = [&]() {
 #pragma unroll
-        for (int q = 0; q < NA; q++) {
-            const int s = q * 256 + tid, row = s / TA::CPR, c = TA::swizzle(row, s % TA::CPR);
-            ra[q] = load_chunk<T>((const T *)P.a.p[pass], P.a, (AK ? m0 : k0) + row, (long long)(AK ? k0 : m0) + c * V);
-        }
+        for (int i = 0; i < FN; i++)
 #pragma unroll
-        for (int q = 0; q < NB; q++) {
-            const int s = q * 256 + tid, row = s / TB::CPR, c = TB::swizzle(row, s % TB::CPR);
-            rb[q] = load_chunk<T>((const T *)P.b.p[pass], P.b, (BKC ? n0 : k0) + row, (long long)(BKC ? k0 : n0) + c * V);
-        }
+            for (int j = 0; j < FM; j++) acc[i][j] *= P.rescale;
     };
-    if (t0 < t1) load(t0);
+
+    Stage<T, AK, BM, NT, DMA> sa;
+    Stage<T, BKC, BN, NT, DMA> sb;
+    sa.begin(P.a, m0, tid);
+    sb.begin(P.b, n0, tid);
+    auto get = [&](int kt, char *buf) {
+        const int pass = kt / ktiles, k0 = (kt - pass * ktiles) * BK;
+        sa.get(P.a, pass, m0, k0, tid, buf);
+        sb.get(P.b, pass, n0, k0, tid, buf + TA::BYTES);
+    };
+    if (t0 < t1) get(t0, lds);
     for (int kt = t0; kt < t1; kt++) {
-        char *buf = lds[(kt - t0) & 1];
-#pragma unroll
-        for (int q = 0; q < NA; q++) *(v4u *)(buf + (q * 256 + tid) * 16) = ra[q];
-#pragma unroll
-        for (int q = 0; q < NB; q++) *(v4u *)(buf + TA::BYTES + (q * 256 + tid) * 16) = rb[q];
-        __syncthreads();  // (the other buffer's readers passed the barrier of this iteration, too, before it is written again)
-        if (kt + 1 < t1) load(kt + 1);
+        char *buf = lds + ((kt - t0) & 1) * (TA::BYTES + TB::BYTES);
+        sa.put(tid, buf);
+        sb.put(tid, buf + TA::BYTES);
+        if constexpr (DMA) wait_loads();
+        __syncthreads();  // this tile is here, and every wave is done with the other buffer
+        if (kt + 1 < t1) get(kt + 1, lds + ((kt + 1 - t0) & 1) * (TA::BYTES + TB::BYTES));
+        if (kt == ktiles && kt > t0 && P.rescale != 1.0f) rescale();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             typename Elem<T>::frag fa[FM], fb[FN];
@@ -241,20 +329,30 @@ __global__ __launch_bounds__(256) void affine_mm(Product P) {
                 for (int j = 0; j < FM; j++) mma(acc[i][j], fb[i], fa[j]);
         }
     }
-    // lane l holds, of each 16 x 16 block, row m = l % 16 and columns n = 4 (l / 16) .. + 3
+    if (t1 <= ktiles && P.passes > 1 && P.rescale != 1.0f) rescale();
+    // Lane l holds, of each 16 x 16 block, row m = l % 16 and columns n = 4 (l / 16) .. + 3. Every wave turns 16 rows at a
+    // time in its own piece of LDS, so that 16 lanes finish (and load and store) one row's 64 consecutive columns.
+    constexpr int COLS = FN * 16, STRIDE = COLS + 4, LANES = FN * 4, ROWS = 64 / LANES;
+    static_assert(WM * WN * 16 * STRIDE * 4 <= 2 * (TA::BYTES + TB::BYTES), "the waves' strips fit the tiles' LDS");
+    __syncthreads();
+    float *strip = (float *)lds + wave * 16 * STRIDE;
+    const int n = n0 + wn * COLS + (lane % LANES) * 4;
 #pragma unroll
     for (int j = 0; j < FM; j++) {
-        const int m = m0 + (wm * FM + j) * 16 + (lane & 15);
-        if (m >= P.m) continue;
 #pragma unroll
-        for (int i = 0; i < FN; i++) {
-            const int n = n0 + (wn * FN + i) * 16 + (lane >> 4) * 4;
-            if (n >= P.n) continue;
+        for (int i = 0; i < FN; i++) *(v4f *)(strip + (lane & 15) * STRIDE + i * 16 + (lane >> 4) * 4) = acc[i][j];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+        for (int r = lane / LANES; r < 16; r += ROWS) {
+            const int m = m0 + (wm * FM + j) * 16 + r;
+            const v4f v = *(const v4f *)(strip + r * STRIDE + (lane % LANES) * 4);
+            if (m >= P.m || n >= P.n) continue;
             if constexpr (OUT == OUT_PART)
-                *(v4f *)(P.part + ((size_t)split * P.m + m) * P.part_ld + n) = acc[i][j];  // (part_ld: a multiple of 4)
+                *(v4f *)(P.part + ((size_t)split * P.m + m) * P.part_ld + n) = v;  // (part_ld: a multiple of 4)
             else
-                finish4<T, OUT>(P.e, m, n, P.n - n, acc[i][j]);
+                finish4<T, OUT>(P.e, m, n, P.n - n, v);
         }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -288,14 +386,21 @@ __global__ __launch_bounds__(256) void affine_round_w(const float *__restrict__ 
 }
 
 // gz = grad_y act'(out) (half of it where act' carries a factor 2: the products' alpha gives it back, exactly), as one
-// number of the layer's type or as the sum of two, and the column sums of gz over this workgroup's rows.
+// number of the layer's type or, NP > 1, as a sum: each further summand takes what the rounding of those before left over
+// (two of f16: 22 bits, the second one times 2^11 so that it stays clear of the subnormals; three of bf16: 24 bits, two
+// where the product is rounded to bf16 anyway). And the column sums of gz over this workgroup's rows.
 // Thread (c, r) takes column chunk c and every 8th row from r on.
 constexpr int GZ_COLS = 32, GZ_ROWS = 8;
-template <typename T, bool PAIR>
-__global__ __launch_bounds__(256) void affine_gz(const T *__restrict__ gy, const T *__restrict__ out, long long ld, T *__restrict__ hi,
-                                                 T *__restrict__ lo, long long gz_ld, float *__restrict__ part, int batch, int n,
-                                                 int act, int range) {
+constexpr float F16_LIFT = 2048.0f;
+template <typename T>
+struct Summands {
+    T *p[3];  // largest first
+};
+template <typename T, int NP>
+__global__ __launch_bounds__(256) void affine_gz(const T *__restrict__ gy, const T *__restrict__ out, long long ld, Summands<T> gz,
+                                                 long long gz_ld, float *__restrict__ part, int batch, int n, int act, int range) {
     constexpr int V = Elem<T>::V;
+    constexpr float LIFT = std::is_same<T, _Float16>::value ? F16_LIFT : 1.0f;
     typedef typename Elem<T>::frag frag;
     __shared__ float red[GZ_ROWS][GZ_COLS * V];
     const int c = threadIdx.x % GZ_COLS, r = threadIdx.x / GZ_COLS;
@@ -308,7 +413,7 @@ __global__ __launch_bounds__(256) void affine_gz(const T *__restrict__ gy, const
     for (int j = 0; j < V; j++) sum[j] = 0.0f;
     if (left)
         for (long long b = b0 + r; b < b1; b += GZ_ROWS) {
-            frag g = {}, o = {}, h, l;
+            frag g = {}, o = {}, part_of[NP];
             const T *pg = gy + b * ld + e, *po = out ? out + b * ld + e : nullptr;
             if (left == V) {
                 __builtin_memcpy(&g, pg, 16);
@@ -324,11 +429,19 @@ __global__ __launch_bounds__(256) void affine_gz(const T *__restrict__ gy, const
             for (int j = 0; j < V; j++) {
                 const float v = out ? (float)g[j] * (bt_act_deriv(act, (float)o[j]) * half) : (float)g[j];
                 sum[j] += v;
-                h[j] = (T)v;
-                if (PAIR) l[j] = (T)(v - (float)h[j]);
+                float rest = v;
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    part_of[p][j] = (T)rest;
+                    rest = (rest - (float)part_of[p][j]) * LIFT;
+                    if (rest != rest) rest = 0.0f;  // (an infinite gradient stays one)
+                }
             }
-            if (hi) __builtin_memcpy(hi + b * gz_ld + e, &h, 16);  // (gz_ld is a multiple of V: a last chunk is whole)
-            if (PAIR) __builtin_memcpy(lo + b * gz_ld + e, &l, 16);
+            if (gz.p[0]) {
+#pragma unroll
+                for (int p = 0; p < NP; p++)  // (gz_ld is a multiple of V: a last chunk is whole)
+                    __builtin_memcpy(gz.p[p] + b * gz_ld + e, &part_of[p], 16);
+            }
         }
     if (!part) return;
 #pragma unroll
@@ -390,7 +503,7 @@ struct Shape {
 Shape shape_of(int m, int n, int k, int passes, size_t es) {
     Shape s;
     const auto count = [&](int b) { return (long long)bt_div_up(m, b) * bt_div_up(n, b); };
-    s.bm = s.bn = count(128) >= 256 ? 128 : 64;
+    s.bm = s.bn = es == 2 && count(256) >= 200 ? 256 : count(128) >= 256 ? 128 : 64;
     s.tiles_m = bt_div_up(m, s.bm), s.tiles_n = bt_div_up(n, s.bn);
     const long long tiles = count(s.bm), ktiles = (long long)bt_div_up(k, (int)(128 / es)) * passes;
     long long splits = 512 / tiles;
@@ -399,25 +512,38 @@ Shape shape_of(int m, int n, int k, int passes, size_t es) {
     return s;
 }
 
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, bool DMA>
+int mm_launch(hipStream_t st, const Product &P) {
+    const long long blocks = (long long)P.tiles_m * P.tiles_n * P.splits;
+    BT_REQUIRE(blocks < (1 << 22), "bt_affine: Mismatched sizes! (%lld tiles)", blocks);
+    const size_t lds = 2 * (Tile<T, AK, BM>::BYTES + Tile<T, BKC, BN>::BYTES);
+    const auto kernel = affine_mm<T, BM, BN, WM, WN, AK, BKC, OUT, DMA>;
+    if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
+    BT_LAUNCH(BTK_AFFINE, st, (affine_mm<T, BM, BN, WM, WN, AK, BKC, OUT, DMA>), dim3((unsigned)blocks), dim3(64 * WM * WN), lds, P);
+    BT_LAUNCH_CHECK();
+    return BT_OK;
+}
+// the tile sizes shape_of chooses from, with or without direct loads
 template <typename T, bool AK, bool BKC, int OUT>
-int product_launch(hipStream_t st, Product &P, const Shape &s) {
+int tile_launch(hipStream_t st, const Product &P, const Shape &s, bool dma) {
+    if constexpr (sizeof(T) == 2)
+        if (s.bm == 256) return mm_launch<T, 256, 256, 2, 4, AK, BKC, OUT, true>(st, P);
+    if (s.bm == 128)
+        return dma ? mm_launch<T, 128, 128, 2, 2, AK, BKC, OUT, true>(st, P) : mm_launch<T, 128, 128, 2, 2, AK, BKC, OUT, false>(st, P);
+    return dma ? mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT, true>(st, P) : mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT, false>(st, P);
+}
+// direct loads need chunks that start on 16 bytes, and reach rows of one tile through 32-bit offsets
+bool direct(const Operand &o) { return o.aligned && o.ld < (1 << 21); }
+
+template <typename T, bool AK, bool BKC, int OUT>
+int product_launch(hipStream_t st, Product &P, Shape s) {
+    const bool dma = direct(P.a) && direct(P.b);
+    if (s.bm == 256 && !dma) s.bm = s.bn = 128, s.tiles_m = bt_div_up(P.m, 128), s.tiles_n = bt_div_up(P.n, 128);
     P.tiles_m = s.tiles_m, P.tiles_n = s.tiles_n, P.splits = s.splits;
     P.part_ld = (P.n + 3) / 4 * 4;
-    const long long blocks = (long long)s.tiles_m * s.tiles_n * s.splits;
-    BT_REQUIRE(blocks < (1 << 24), "bt_affine: Mismatched sizes! (%lld tiles)", blocks);
-    const dim3 grid((unsigned)blocks), block(256);
-    if (s.splits > 1) {
-        if (s.bm == 128)
-            BT_LAUNCH(BTK_AFFINE, st, (affine_mm<T, 128, 128, AK, BKC, OUT_PART>), grid, block, 0, P);
-        else
-            BT_LAUNCH(BTK_AFFINE, st, (affine_mm<T, 64, 64, AK, BKC, OUT_PART>), grid, block, 0, P);
-        BT_LAUNCH_CHECK();
-        BT_LAUNCH(BTK_AFFINE, st, (affine_join<T, OUT>), dim3(bt_div_up(P.part_ld / 4 * P.m, 256)), block, 0, P);
-    } else if (s.bm == 128) {
-        BT_LAUNCH(BTK_AFFINE, st, (affine_mm<T, 128, 128, AK, BKC, OUT>), grid, block, 0, P);
-    } else {
-        BT_LAUNCH(BTK_AFFINE, st, (affine_mm<T, 64, 64, AK, BKC, OUT>), grid, block, 0, P);
-    }
+    if (s.splits == 1) return tile_launch<T, AK, BKC, OUT>(st, P, s, dma);
+    if (int rc = tile_launch<T, AK, BKC, OUT_PART>(st, P, s, dma)) return rc;
+    BT_LAUNCH(BTK_AFFINE, st, (affine_join<T, OUT>), dim3(bt_div_up(P.part_ld / 4 * P.m, 256)), dim3(256), 0, P);
     BT_LAUNCH_CHECK();
     return BT_OK;
 }
@@ -436,15 +562,15 @@ int make_w(hipStream_t st, const bt_affine_desc *d, const void *w, void *ws, Ope
         BT_LAUNCH(BTK_AFFINE, st, affine_round_w<T>, dim3(bt_div_up(quads, 256)), dim3(256), 0, (const float *)w, (long long)d->w_ld,
                   (T *)ws, ld, d->in, d->out);
         BT_LAUNCH_CHECK();
-        o.p[0] = o.p[1] = ws, o.ld = ld;
+        o.p[0] = o.p[1] = o.p[2] = ws, o.ld = ld;
     } else {
-        o.p[0] = o.p[1] = w, o.ld = d->w_ld;
+        o.p[0] = o.p[1] = o.p[2] = w, o.ld = d->w_ld;
     }
     o.aligned = chunk_aligned(o.p[0], o.ld, sizeof(T));
     return BT_OK;
 }
 Operand matrix(const void *p, long long ld, int rows, int len, size_t es) {
-    return Operand{{p, p}, ld, rows, len, chunk_aligned(p, ld, es)};
+    return Operand{{p, p, p}, ld, rows, len, chunk_aligned(p, ld, es)};
 }
 
 template <typename T>
@@ -454,15 +580,16 @@ int forward(hipStream_t st, const bt_affine_desc *d, const void *w, const float 
     Product P = {};
     if (int rc = make_w<T>(st, d, w, ws, P.b)) return rc;
     P.a = matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
-    P.m = d->batch, P.n = d->out, P.k = d->in, P.passes = 1;
+    P.m = d->batch, P.n = d->out, P.k = d->in, P.passes = 1, P.rescale = 1.0f;
     P.part = (float *)(ws + round_w_bytes(d));
     P.e = Epilogue{bias, residual, y, saved, d->y_ld, d->act, 1.0f};
     return product_launch<T, true, false, OUT_LAYER>(st, P, s);
 }
 
 struct BackwardPlan {
-    bool pair, gz;   // gz kept as two numbers; kept at all (else grad_y is gz)
-    float alpha;
+    bool gz;             // gz is kept (else grad_y is gz)
+    int np_dw, np_dx;    // summands it is kept as for dW (whose outputs are f32), and how many of them grad_x takes
+    float alpha, rescale;
     int range, ranges;
     Shape dw, dx;
     size_t w_bytes, gz_bytes, sum_bytes, part_bytes, total;
@@ -472,19 +599,21 @@ BackwardPlan backward_plan(const bt_affine_desc *d) {
     const size_t es = type_size(d->type);
     const bool root = d->act == BT_ACT_SCRELU || d->act == BT_ACT_SQRRELU;
     p.gz = d->act != BT_ACT_IDENTITY;
-    p.pair = root && es == 2;
+    p.np_dw = !root || es == 4 ? 1 : d->type == BT_TYPE_BF16 ? 3 : 2;
+    p.np_dx = p.np_dw > 2 ? 2 : p.np_dw;
     p.alpha = root ? 2.0f : 1.0f;
+    p.rescale = d->type == BT_TYPE_F16 && root ? 1.0f / F16_LIFT : 1.0f;
     p.range = 128;
     while (bt_div_up(d->batch, p.range) > 1024) p.range *= 2;
     p.ranges = bt_div_up(d->batch, p.range);
-    p.dw = shape_of(d->in, d->out, d->batch, p.pair ? 2 : 1, es);
-    p.dx = shape_of(d->batch, d->in, d->out, p.pair ? 2 : 1, es);
+    p.dw = shape_of(d->in, d->out, d->batch, p.np_dw, es);
+    p.dx = shape_of(d->batch, d->in, d->out, p.np_dx, es);
     p.w_bytes = round_w_bytes(d);
     p.gz_bytes = p.gz ? bt_align((size_t)d->batch * padded(d->out, es) * es) : 0;
     p.sum_bytes = bt_align((size_t)p.ranges * d->out * 4);
     const size_t a = p.dw.part_bytes(d->in, d->out), b = p.dx.part_bytes(d->batch, d->in);
     p.part_bytes = a > b ? a : b;
-    p.total = p.w_bytes + p.gz_bytes * (p.pair ? 2 : 1) + p.sum_bytes + p.part_bytes;
+    p.total = p.w_bytes + p.gz_bytes * p.np_dw + p.sum_bytes + p.part_bytes;
     return p;
 }
 
@@ -492,20 +621,26 @@ template <typename T>
 int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void *x, const void *out, const void *gy, float *dw,
              float *dbias, void *gx, char *ws) {
     const BackwardPlan p = backward_plan(d);
-    char *w16 = ws, *hi = w16 + p.w_bytes, *lo = hi + p.gz_bytes, *sums = hi + p.gz_bytes * (p.pair ? 2 : 1),
-         *part = sums + p.sum_bytes;
+    char *w16 = ws, *kept = w16 + p.w_bytes, *sums = kept + p.gz_bytes * p.np_dw, *part = sums + p.sum_bytes;
     const bool keep = p.gz && (dw || gx);
+    const int np = !keep ? 1 : dw ? p.np_dw : p.np_dx;
     if (keep || dbias) {
         const dim3 grid(bt_div_up(d->out, GZ_COLS * Elem<T>::V), p.ranges);
-        T *h = keep ? (T *)hi : nullptr;
+        Summands<T> gz = {{nullptr, nullptr, nullptr}};
+        for (int i = 0; i < np && keep; i++) gz.p[i] = (T *)(kept + i * p.gz_bytes);
         float *sum = dbias ? (float *)sums : nullptr;
         const T *o = p.gz ? (const T *)out : nullptr;
-        if (keep && p.pair)
-            BT_LAUNCH(BTK_AFFINE, st, (affine_gz<T, true>), grid, dim3(256), 0, (const T *)gy, o, (long long)d->y_ld, h, (T *)lo,
-                      padded(d->out, sizeof(T)), sum, d->batch, d->out, d->act, p.range);
-        else
-            BT_LAUNCH(BTK_AFFINE, st, (affine_gz<T, false>), grid, dim3(256), 0, (const T *)gy, o, (long long)d->y_ld, h,
-                      (T *)nullptr, padded(d->out, sizeof(T)), sum, d->batch, d->out, d->act, p.range);
+        const long long ld = d->y_ld, gz_ld = padded(d->out, sizeof(T));
+#define GZ_CASE(NP)                                                                                                          BT_LAUNCH(BTK_AFFINE, st, (affine_gz<T, NP>), grid, dim3(256), 0, (const T *)gy, o, ld, gz, gz_ld, sum, d->batch, d->out,               d->act, p.range)
+        if (np == 1)
+            GZ_CASE(1);
+        else if constexpr (sizeof(T) == 2) {
+            if (np == 2)
+                GZ_CASE(2);
+            else
+                GZ_CASE(3);
+        }
+#undef GZ_CASE
         BT_LAUNCH_CHECK();
     }
     if (dbias) {
@@ -513,14 +648,17 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
                   p.alpha, dbias);
         BT_LAUNCH_CHECK();
     }
-    Operand gz = p.gz ? matrix(hi, padded(d->out, sizeof(T)), d->batch, d->out, sizeof(T))
-                      : matrix(gy, d->y_ld, d->batch, d->out, sizeof(T));
-    if (p.pair) gz.p[1] = lo;
+    const auto gz_operand = [&](int n) {  // its n largest summands, the smallest of them first
+        if (!p.gz) return matrix(gy, d->y_ld, d->batch, d->out, sizeof(T));
+        Operand o = matrix(kept, padded(d->out, sizeof(T)), d->batch, d->out, sizeof(T));
+        for (int i = 0; i < n; i++) o.p[i] = kept + (n - 1 - i) * p.gz_bytes;
+        return o;
+    };
     if (dw) {
         Product P = {};
         P.a = matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
-        P.b = gz;
-        P.m = d->in, P.n = d->out, P.k = d->batch, P.passes = p.pair ? 2 : 1;
+        P.b = gz_operand(p.np_dw);
+        P.m = d->in, P.n = d->out, P.k = d->batch, P.passes = p.np_dw, P.rescale = p.rescale;
         P.part = (float *)part;
         P.e.out = dw, P.e.ld = d->w_ld, P.e.alpha = p.alpha;
         if (int rc = product_launch<T, false, false, OUT_F32>(st, P, p.dw)) return rc;
@@ -528,8 +666,8 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
     if (gx) {
         Product P = {};
         if (int rc = make_w<T>(st, d, w, w16, P.b)) return rc;
-        P.a = gz;
-        P.m = d->batch, P.n = d->in, P.k = d->out, P.passes = p.pair ? 2 : 1;
+        P.a = gz_operand(p.np_dx);
+        P.m = d->batch, P.n = d->in, P.k = d->out, P.passes = p.np_dx, P.rescale = p.rescale;
         P.part = (float *)part;
         P.e.out = gx, P.e.ld = d->x_ld, P.e.alpha = p.alpha;
         if (int rc = product_launch<T, true, true, OUT_TYPE>(st, P, p.dx)) return rc;

@@ -298,8 +298,9 @@ int bt_affine_forward(void *stream, const bt_affine_desc *desc, const void *w, c
 /* gz = grad_y * act'(.), the derivative taken from `out`, the activation's output (y, or saved if there was a residual;
  * ignored and NULL allowed for BT_ACT_IDENTITY); dw = sum over rows of gz x, dbias = sum of gz, grad_x = gz W. A residual's
  * gradient is grad_y itself. dw: F32, layout of w, dbias: F32[out] (for bt_adamw; both overwritten); each of dw, dbias,
- * grad_x may be NULL. 16-bit layers keep gz in 16 bits where that loses nothing (the derivative is 0 or 1) and as a pair
- * of 16-bit numbers where it would (SCReLU, squared ReLU); squared ReLU of f16 is refused, since gz can leave its range. */
+ * grad_x may be NULL. 16-bit layers keep gz in 16 bits where that loses nothing (the derivative is 0 or 1) and as a sum
+ * of two or three 16-bit numbers where it would (SCReLU, squared ReLU); squared ReLU of f16 is refused, since gz can leave
+ * its range. */
 size_t bt_affine_backward_workspace_bytes(const bt_affine_desc *desc);
 int bt_affine_backward(void *stream, const bt_affine_desc *desc, const void *w, const void *x, const void *out,
                        const void *grad_y, float *dw, float *dbias, void *grad_x, void *workspace, size_t workspace_bytes);

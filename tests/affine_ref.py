@@ -2,8 +2,9 @@
 
 Bounds. A sum of K products in 32 bits, each product exact or rounded once, is off by at most about 6 sqrt(K) 2^-24 of the
 sum of the products' magnitudes (roundings of independent sign; six standard deviations of a bound that already takes every
-rounding at its largest), and never by less than a few 2^-24 of it (the constant 4 for short sums). A gradient kept as two
-16-bit numbers h + l is off by the square of the type's half step; f16 adds half its smallest step.
+rounding at its largest), and never by less than a few 2^-24 of it (the constant 4 for short sums). A gradient kept as n
+16-bit numbers is off by the n-th power of the type's half step: bf16 three times for dw and twice for gx, f16 twice (its
+second number lifted by 2^11, which leaves 2^-11 of half its smallest step).
 """
 import ctypes as C
 
@@ -59,16 +60,15 @@ def forward(kind, w, bias, x, residual):
 def backward(kind, dtype, w, x, out, gy):
     s = slope(kind, out) if out is not None else np.ones_like(gy)
     gz = gy * s
-    pair = 0.0
-    if kind in ("screlu", "sqrrelu"):
-        pair = 4 * U + (0.0 if dtype == "f32" else EPS[dtype] ** 2)
-    tiny = TINY["f16"] if dtype == "f16" and pair else 0.0
-    n = 2 if pair and dtype != "f32" else 1
+    root = kind in ("screlu", "sqrrelu")
+    n_w, n_x = {"f32": (1, 1), "bf16": (3, 2), "f16": (2, 2)}[dtype] if root else (1, 1)
+    e_w, e_x = [4 * U + (0.0 if dtype == "f32" else EPS[dtype] ** n) if root else 0.0 for n in (n_w, n_x)]
+    tiny = TINY["f16"] / 2048 if dtype == "f16" and root else 0.0
     dw, ax = x.T @ gz, np.abs(x)
     gx, aw = gz @ w.T, np.abs(w)
     g = np.abs(gz)
-    ddw = (sums(n * x.shape[0]) + pair) * (ax.T @ g) + 2 * tiny * ax.sum(0)[:, None]
-    dgx = (sums(n * w.shape[1]) + pair) * (g @ aw.T) + 2 * tiny * aw.sum(1)[None, :]
+    ddw = (sums(n_w * x.shape[0]) + e_w) * (ax.T @ g) + 2 * tiny * ax.sum(0)[:, None]
+    dgx = (sums(n_x * w.shape[1]) + e_x) * (g @ aw.T) + 2 * tiny * aw.sum(1)[None, :]
     return dict(dw=dw, dbias=gz.sum(0), gx=gx), dict(dw=ddw, dbias=(sums(x.shape[0]) + 4 * U) * g.sum(0), gx=dgx)
 
 
