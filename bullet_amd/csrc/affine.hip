@@ -26,15 +26,22 @@ struct Elem {
 
 // acc += a b^T over the k of one fragment: lane l holds row l % 16 and, of 16-bit types, k = 8 (l / 16) .. + 7 of 32 (one
 // MFMA), of f32 k = 4 (l / 16) .. + 3 of 16 (four of them, each taking one k from every 16 lanes)
-__device__ __forceinline__ void mma(v4f &acc, const Elem<__bf16>::frag &a, const Elem<__bf16>::frag &b) {
+__device__ __forceinline__ void mma(v4f &acc, const Elem<__bf16>::frag &a, const Elem<__bf16>::frag &b, int) {
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
 }
-__device__ __forceinline__ void mma(v4f &acc, const Elem<_Float16>::frag &a, const Elem<_Float16>::frag &b) {
+__device__ __forceinline__ void mma(v4f &acc, const Elem<_Float16>::frag &a, const Elem<_Float16>::frag &b, int) {
     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0);
 }
-__device__ __forceinline__ void mma(v4f &acc, const Elem<float>::frag &a, const Elem<float>::frag &b) {
+__device__ __forceinline__ void mma(v4f &acc, const Elem<float>::frag &a, const Elem<float>::frag &b, int j) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+}
+// products of one fragment of m with the wave's fragments of n
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void mma_col(v4f (&acc)[FN][FM], int j, const typename Elem<T>::frag (&b)[FN], const typename Elem<T>::frag &a) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+    for (int q = 0; q < (sizeof(T) == 4 ? 4 : 1); q++)  // (f32: four in turn on each block of sums, others in between)
+#pragma unroll
+        for (int i = 0; i < FN; i++) mma(acc[i][j], b[i], a, q);
 }
 
 // One operand's tile. KC: rows of m (or n), contiguous in k; otherwise rows of k, contiguous in m (or n). Slot s of the tile
@@ -54,31 +61,37 @@ struct Tile {
         if (sizeof(T) == 4) return c ^ ((((row >> 2) & 3) << 2) & (CPR - 1));
         return c ^ ((((row & 3) | ((row >> 3) & 1) << 2) << 1) & (CPR - 1));
     }
-    // fragment `f` (16 of SPAN) at k-step s
-    static __device__ __forceinline__ typename Elem<T>::frag read(const char *lds, int f, int s, int lane) {
-        typedef typename Elem<T>::frag frag;
+    // Where lane l's part of fragment f0 (16 of SPAN; a multiple of the wave's number of fragments, a power of two) lies at
+    // k-step 0, and its fragment f0 + f at k-step s from there: the swizzle leaves the rest to a flipped bit or two and
+    // constant distances. LDS addresses; tiles start on 1024 bytes.
+    static __device__ __forceinline__ uint32_t origin(int f0, int lane) {
         const int g = lane >> 4, i = lane & 15;
+        if (KC) return (f0 * 16 + i) * 128 + (g ^ (i & 7)) * 16;
+        if (sizeof(T) == 4) {
+            const int row = g * 4;
+            return (row * CPR + swizzle(row, f0 * 4 + (i >> 2))) * 16 + (i & 3) * 4;
+        }
+        // 16 lanes give the addresses of 4 rows of 16 elements and get 4 rows of one column each
+        const int row = g * 8 + (i >> 2);
+        return (row * CPR + swizzle(row, f0 * 2 + ((i >> 1) & 1))) * 16 + (i & 1) * 8;
+    }
+    static __device__ __forceinline__ typename Elem<T>::frag read(uint32_t at, int f, int s) {
+        typedef typename Elem<T>::frag frag;
         if constexpr (KC) {
-            const int row = f * 16 + i;
-            return *(const frag *)(lds + row * 128 + swizzle(row, s * 4 + g) * 16);
+            return *(const __attribute__((address_space(3))) frag *)(uintptr_t)((at ^ (s * 64)) + f * 2048);
         } else if constexpr (sizeof(T) == 4) {
             frag r;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int row = s * 16 + g * 4 + j, c = f * 4 + (i >> 2);
-                r[j] = *(const float *)(lds + (row * CPR + swizzle(row, c)) * 16 + (i & 3) * 4);
-            }
+            for (int j = 0; j < 4; j++)
+                r[j] = *(const __attribute__((address_space(3))) float *)(uintptr_t)((at ^ (f * 64)) + (s * 16 + j) * CPR * 16);
             return r;
         } else {
             typedef short s4 __attribute__((ext_vector_type(4)));
             s4 h[2];
 #pragma unroll
-            for (int q = 0; q < 2; q++) {
-                // 16 lanes give the addresses of 4 rows of 16 elements and get 4 rows of one column each
-                const int row = s * 32 + g * 8 + q * 4 + (i >> 2), c = f * 2 + ((i >> 1) & 1);
-                const char *p = lds + (row * CPR + swizzle(row, c)) * 16 + (i & 1) * 8;
-                h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p);
-            }
+            for (int q = 0; q < 2; q++)
+                h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s4 *)(uintptr_t)((at ^ (f * 32)) + (s * 32 + q * 4) * CPR * 16));
             return __builtin_bit_cast(frag, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
@@ -181,11 +194,14 @@ __device__ __forceinline__ void finish4(const Epilogue &e, int row, int c, int n
     }
 }
 
+constexpr float F16_LIFT = 2048.0f;  // between the two summands of an f16 gradient (affine_gz)
+
 struct Product {
     Operand a, b;
     int m, n, k;
     int passes;          // summands of the operands, taken one after the other
-    float rescale;       // what the sums of the first summand's products are multiplied by before the next one's
+    int lift;            // the first of two summands is F16_LIFT times too large: one half of the splits takes it, the other
+                         // half the second one, and affine_join puts it right
     int tiles_m, tiles_n;
     int splits;          // workgroups that share one tile's k, each leaving its sums in `part`
     float *part;         // [splits][m][part_ld]
@@ -204,58 +220,46 @@ __device__ __forceinline__ uint32_t lds_address(const char *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
 }
 
-// One operand's way into LDS, for a workgroup of NT threads. With DMA the chunks of a tile that lies wholly inside the
-// matrix go there directly; a tile that ends with k, or whose span ends inside a chunk, is loaded chunk by chunk with
-// zeros where there is nothing. (Rows of m or n beyond the end are taken from the last row: their sums are not stored.)
-template <typename T, bool KC, int SPAN, int NT, bool DMA>
+// One operand's tiles on their way into LDS, for a workgroup of NT threads.
+template <typename T, bool KC, int SPAN, int NT>
 struct Stage {
     typedef Tile<T, KC, SPAN> L;
     static constexpr int V = Elem<T>::V, BK = Elem<T>::BK, N = L::SLOTS / NT;
-    uint32_t off[DMA ? N : 1];
-    v4u r[DMA ? 1 : N];
-    bool inside;
-    __device__ __forceinline__ void begin(const Operand &o, int s0, int tid) {
-        if constexpr (DMA) {
-            const int left = (KC ? o.rows : o.len) - s0;  // > 0
-            inside = KC || left >= SPAN || o.len % V == 0;
-#pragma unroll
-            for (int q = 0; q < N; q++) {
-                const int s = q * NT + tid;
-                int row = s / L::CPR, c = L::swizzle(row, s % L::CPR);
-                if (KC) row = min(row, left - 1);
-                if (!KC) c = max(min(c, left / V - 1), 0);
-                off[q] = (uint32_t)row * (uint32_t)(o.ld * sizeof(T)) + c * 16;
-            }
-        }
-    }
-    __device__ __forceinline__ v4u chunk(const Operand &o, int pass, int s0, int k0, int s) const {
+    // chunk of slot s of the tile at (s0, k0), zeros where the matrix has nothing
+    static __device__ __forceinline__ v4u chunk(const Operand &o, int pass, int s0, int k0, int s) {
         const int row = s / L::CPR, c = L::swizzle(row, s % L::CPR);
         return load_chunk<T>((const T *)o.p[pass], o, (KC ? s0 : k0) + row, (long long)(KC ? k0 : s0) + c * V);
     }
-    // issue the tile at k0 of a summand; without DMA it waits in registers until put()
-    __device__ __forceinline__ void get(const Operand &o, int pass, int s0, int k0, int tid, char *lds) {
-        if constexpr (DMA) {
-            if (inside && (KC ? o.len : o.rows) - k0 >= BK) {
-                const char *base = (const char *)o.p[pass] +
-                                   ((KC ? s0 : k0) * (size_t)o.ld + (KC ? k0 : s0)) * sizeof(T);
-                const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (tid & ~63) * 16);
+    static __device__ __forceinline__ void get(const Operand &o, int pass, int s0, int k0, int tid, v4u (&r)[N]) {
 #pragma unroll
-                for (int q = 0; q < N; q++) to_lds(base, off[q], to + q * NT * 16);
-            } else {
+        for (int q = 0; q < N; q++) r[q] = chunk(o, pass, s0, k0, q * NT + tid);
+    }
+    static __device__ __forceinline__ void put(const v4u (&r)[N], int tid, char *lds) {
+#pragma unroll
+        for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = r[q];
+    }
+    static __device__ __forceinline__ void copy(const Operand &o, int pass, int s0, int k0, int tid, char *lds) {
 #pragma unroll 1
-                for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = chunk(o, pass, s0, k0, q * NT + tid);
-            }
-        } else {
+        for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = chunk(o, pass, s0, k0, q * NT + tid);
+    }
+    // Direct loads: byte offsets of this thread's chunks from the tile's first element, the same for every tile. Rows (or
+    // chunks) of m or n beyond the end are taken from the last one: their sums are not stored.
+    static __device__ __forceinline__ bool inside(const Operand &o, int s0) { return KC || o.len - s0 >= SPAN || o.len % V == 0; }
+    static __device__ __forceinline__ void offsets(const Operand &o, int s0, int tid, uint32_t (&off)[N]) {
+        const int left = (KC ? o.rows : o.len) - s0;  // > 0
 #pragma unroll
-            for (int q = 0; q < N; q++) r[q] = chunk(o, pass, s0, k0, q * NT + tid);
+        for (int q = 0; q < N; q++) {
+            const int s = q * NT + tid;
+            int row = s / L::CPR, c = L::swizzle(row, s % L::CPR);
+            if (KC) row = min(row, left - 1);
+            if (!KC) c = max(min(c, left / V - 1), 0);
+            off[q] = (uint32_t)row * (uint32_t)(o.ld * sizeof(T)) + c * 16;
         }
     }
-    __device__ __forceinline__ void put(int tid, char *lds) const {
-        if constexpr (!DMA) {
-#pragma unroll
-            for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = r[q];
-        }
+    static __device__ __forceinline__ const char *first(const Operand &o, int pass, int s0, int k0) {
+        return (const char *)o.p[pass] + ((KC ? s0 : k0) * (size_t)o.ld + (KC ? k0 : s0)) * sizeof(T);
     }
+    static __device__ __forceinline__ size_t step(const Operand &o) { return KC ? 128 : (size_t)o.ld * sizeof(T) * BK; }
 };
 
 // Which tile a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an L2 of its own: every XCD gets a
@@ -269,91 +273,213 @@ __device__ __forceinline__ void tile_of(int wg, int wgs, int tiles_m, int tiles_
     tm = band * 8 + in % high, tn = in / high;
 }
 
-// BM x BN tile by WM x WN waves. Double-buffered LDS: the next tile is on its way while this one is multiplied.
-template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, bool DMA>
-__global__ __launch_bounds__(64 * WM * WN) void affine_mm(Product P) {
-    constexpr int NT = 64 * WM * WN;
+// What the kernels below share: a BM x BN tile by WM x WN waves, each with FM x FN blocks of 16 x 16 sums.
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
+struct Mm {
+    static constexpr int NT = 64 * WM * WN, BK = Elem<T>::BK, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef Tile<T, AK, BM> TA;
     typedef Tile<T, BKC, BN> TB;
-    constexpr int BK = Elem<T>::BK;
-    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    extern __shared__ __align__(16) char lds[];  // 2 x (TA::BYTES + TB::BYTES)
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave / WN, wn = wave % WN;
-    int split, tm, tn;
-    tile_of(blockIdx.x, gridDim.x, P.tiles_m, P.tiles_n, split, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
-    const int ktiles = (P.k + BK - 1) / BK, all = ktiles * P.passes;
-    const int t0 = (int)((long long)all * split / P.splits), t1 = (int)((long long)all * (split + 1) / P.splits);
-
+    typedef Stage<T, AK, BM, NT> SA;
+    typedef Stage<T, BKC, BN, NT> SB;
+    static constexpr int BYTES = TA::BYTES + TB::BYTES;  // of one of the two buffers
+    typedef typename Elem<T>::frag frag;
+    const Product &P;
+    char *lds;
+    int tid, lane, wm, wn, split, m0, n0;
+    uint32_t at_a, at_b;  // where this lane reads a tile of the first buffer
     v4f acc[FN][FM];
-#pragma unroll
-    for (int i = 0; i < FN; i++)
-#pragma unroll
-        for (int j = 0; j < FM; j++) acc[i][j] = v4f{0, 0, 0, 0};
-    auto rescale = [&]() {
+
+    __device__ __forceinline__ Mm(const Product &P_, char *lds_) : P(P_), lds(lds_) {
+        tid = threadIdx.x, lane = tid & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        wm = wave / WN, wn = wave % WN;
+        int tm, tn;
+        tile_of(blockIdx.x, gridDim.x, P.tiles_m, P.tiles_n, split, tm, tn);
+        m0 = tm * BM, n0 = tn * BN;
+        at_a = lds_address(lds) + TA::origin(wm * FM, lane), at_b = lds_address(lds) + TA::BYTES + TB::origin(wn * FN, lane);
 #pragma unroll
         for (int i = 0; i < FN; i++)
 #pragma unroll
-            for (int j = 0; j < FM; j++) acc[i][j] *= P.rescale;
-    };
-
-    Stage<T, AK, BM, NT, DMA> sa;
-    Stage<T, BKC, BN, NT, DMA> sb;
-    sa.begin(P.a, m0, tid);
-    sb.begin(P.b, n0, tid);
-    auto get = [&](int kt, char *buf) {
-        const int pass = kt / ktiles, k0 = (kt - pass * ktiles) * BK;
-        sa.get(P.a, pass, m0, k0, tid, buf);
-        sb.get(P.b, pass, n0, k0, tid, buf + TA::BYTES);
-    };
-    if (t0 < t1) get(t0, lds);
-    for (int kt = t0; kt < t1; kt++) {
-        char *buf = lds + ((kt - t0) & 1) * (TA::BYTES + TB::BYTES);
-        sa.put(tid, buf);
-        sb.put(tid, buf + TA::BYTES);
-        if constexpr (DMA) wait_loads();
-        __syncthreads();  // this tile is here, and every wave is done with the other buffer
-        if (kt + 1 < t1) get(kt + 1, lds + ((kt + 1 - t0) & 1) * (TA::BYTES + TB::BYTES));
-        if (kt == ktiles && kt > t0 && P.rescale != 1.0f) rescale();
+            for (int j = 0; j < FM; j++) acc[i][j] = v4f{0, 0, 0, 0};
+    }
+    // This workgroup's share of `ktiles` tiles of k a summand: the summands [p0, p1), the tiles [t0, t1) of theirs put one
+    // behind the other, and whether that is the last share of them.
+    __device__ __forceinline__ bool share(int ktiles, int &p0, int &p1, int &t0, int &t1) const {
+        const int subs = P.lift ? P.splits / 2 : P.splits, sub = P.lift ? split % subs : split;
+        p0 = P.lift ? split / subs : 0, p1 = P.lift ? p0 + 1 : P.passes;
+        const long long all = (long long)ktiles * (p1 - p0);
+        t0 = (int)(all * sub / subs), t1 = (int)(all * (sub + 1) / subs);
+        return sub == subs - 1;
+    }
+    __device__ __forceinline__ frag read_a(int buf, int j, int s) const { return TA::read(at_a + buf * BYTES, j, s); }
+    __device__ __forceinline__ frag read_b(int buf, int i, int s) const { return TB::read(at_b + buf * BYTES, i, s); }
+    __device__ __forceinline__ void multiply(int buf) {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            typename Elem<T>::frag fa[FM], fb[FN];
+            frag fa[FM], fb[FN];
 #pragma unroll
-            for (int j = 0; j < FM; j++) fa[j] = TA::read(buf, wm * FM + j, s, lane);
+            for (int j = 0; j < FM; j++) fa[j] = read_a(buf, j, s);
 #pragma unroll
-            for (int i = 0; i < FN; i++) fb[i] = TB::read(buf + TA::BYTES, wn * FN + i, s, lane);
+            for (int i = 0; i < FN; i++) fb[i] = read_b(buf, i, s);
 #pragma unroll
-            for (int i = 0; i < FN; i++)
-#pragma unroll
-                for (int j = 0; j < FM; j++) mma(acc[i][j], fb[i], fa[j]);
+            for (int j = 0; j < FM; j++) mma_col<T, FM, FN>(acc, j, fb, fa[j]);
         }
     }
-    if (t1 <= ktiles && P.passes > 1 && P.rescale != 1.0f) rescale();
+    // one tile, from memory to sums, with nothing overlapped: tiles that end inside a chunk or inside 128 bytes of k
+    __device__ __forceinline__ void plain_tile(int pass, int k0) {
+        __syncthreads();
+        SA::copy(P.a, pass, m0, k0, tid, lds);
+        SB::copy(P.b, pass, n0, k0, tid, lds + TA::BYTES);
+        __syncthreads();
+        multiply(0);
+    }
     // Lane l holds, of each 16 x 16 block, row m = l % 16 and columns n = 4 (l / 16) .. + 3. Every wave turns 16 rows at a
     // time in its own piece of LDS, so that 16 lanes finish (and load and store) one row's 64 consecutive columns.
-    constexpr int COLS = FN * 16, STRIDE = COLS + 4, LANES = FN * 4, ROWS = 64 / LANES;
-    static_assert(WM * WN * 16 * STRIDE * 4 <= 2 * (TA::BYTES + TB::BYTES), "the waves' strips fit the tiles' LDS");
-    __syncthreads();
-    float *strip = (float *)lds + wave * 16 * STRIDE;
-    const int n = n0 + wn * COLS + (lane % LANES) * 4;
+    __device__ __forceinline__ void finish() {
+        constexpr int COLS = FN * 16, STRIDE = COLS + 4, LANES = FN * 4, ROWS = 64 / LANES;
+        static_assert(WM * WN * 16 * STRIDE * 4 <= 2 * BYTES, "the waves' strips fit the tiles' LDS");
+        __syncthreads();
+        float *strip = (float *)lds + (wm * WN + wn) * 16 * STRIDE;
+        const int n = n0 + wn * COLS + (lane % LANES) * 4;
 #pragma unroll
-    for (int j = 0; j < FM; j++) {
+        for (int j = 0; j < FM; j++) {
 #pragma unroll
-        for (int i = 0; i < FN; i++) *(v4f *)(strip + (lane & 15) * STRIDE + i * 16 + (lane >> 4) * 4) = acc[i][j];
-        __builtin_amdgcn_wave_barrier();
+            for (int i = 0; i < FN; i++) *(v4f *)(strip + (lane & 15) * STRIDE + i * 16 + (lane >> 4) * 4) = acc[i][j];
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll 2
-        for (int r = lane / LANES; r < 16; r += ROWS) {
-            const int m = m0 + (wm * FM + j) * 16 + r;
-            const v4f v = *(const v4f *)(strip + r * STRIDE + (lane % LANES) * 4);
-            if (m >= P.m || n >= P.n) continue;
-            if constexpr (OUT == OUT_PART)
-                *(v4f *)(P.part + ((size_t)split * P.m + m) * P.part_ld + n) = v;  // (part_ld: a multiple of 4)
-            else
-                finish4<T, OUT>(P.e, m, n, P.n - n, v);
+            for (int r = lane / LANES; r < 16; r += ROWS) {
+                const int m = m0 + (wm * FM + j) * 16 + r;
+                const v4f v = *(const v4f *)(strip + r * STRIDE + (lane % LANES) * 4);
+                if (m >= P.m || n >= P.n) continue;
+                if constexpr (OUT == OUT_PART)
+                    *(v4f *)(P.part + ((size_t)split * P.m + m) * P.part_ld + n) = v;  // (part_ld: a multiple of 4)
+                else
+                    finish4<T, OUT>(P.e, m, n, P.n - n, v);
+            }
+            __builtin_amdgcn_wave_barrier();
         }
-        __builtin_amdgcn_wave_barrier();
     }
+};
+
+// Operands of any alignment: the next tile is loaded into registers while this one is multiplied.
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
+__global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
+    typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
+    extern __shared__ __align__(1024) char lds[];
+    M mm(P, lds);
+    const int ktiles = (P.k + M::BK - 1) / M::BK;
+    int p0, p1, t0, t1;
+    mm.share(ktiles, p0, p1, t0, t1);
+    v4u ra[M::SA::N], rb[M::SB::N];
+    auto get = [&](int kt) {
+        const int pass = kt / ktiles, k0 = (kt - pass * ktiles) * M::BK;
+        M::SA::get(P.a, p0 + pass, mm.m0, k0, mm.tid, ra);
+        M::SB::get(P.b, p0 + pass, mm.n0, k0, mm.tid, rb);
+    };
+    if (t0 < t1) get(t0);
+    for (int kt = t0; kt < t1; kt++) {
+        char *buf = lds + ((kt - t0) & 1) * M::BYTES;
+        M::SA::put(ra, mm.tid, buf);
+        M::SB::put(rb, mm.tid, buf + M::TA::BYTES);
+        __syncthreads();  // this tile is here, and every wave is done with the other buffer
+        if (kt + 1 < t1) get(kt + 1);
+        mm.multiply((kt - t0) & 1);
+    }
+    mm.finish();
+}
+
+// Operands whose chunks start on 16 bytes: tiles go straight into LDS, and three things are under way at any time. While
+// the first half of a tile's k is multiplied the second half's fragments are read; behind the barrier that says that the
+// next tile has arrived its first fragments are read, and the tile after it is sent for into the buffer just left, while
+// the second half is multiplied. Each fragment's products carry their share of those reads and loads.
+// k that does not fill a tile goes through plain_tile at the end.
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
+    typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
+    typedef typename M::frag frag;
+    constexpr int FM = M::FM, FN = M::FN, NA = M::SA::N, NB = M::SB::N;
+    extern __shared__ __align__(1024) char lds[];
+    M mm(P, lds);
+    const bool inside = M::SA::inside(P.a, mm.m0) && M::SB::inside(P.b, mm.n0);
+    const int full = inside ? P.k / M::BK : 0, rest = full * M::BK;
+    int p0, p1, t0, t1;
+    const bool last = mm.share(full, p0, p1, t0, t1);
+    if (t0 < t1) {
+        uint32_t oa[NA], ob[NB];
+        M::SA::offsets(P.a, mm.m0, mm.tid, oa);
+        M::SB::offsets(P.b, mm.n0, mm.tid, ob);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (mm.tid & ~63) * 16);
+        // the tile to be sent for next: its summand, its number in there, its first elements
+        int pass = p0 + t0 / full, at = t0 % full;
+        const char *pa = M::SA::first(P.a, pass, mm.m0, at * M::BK), *pb = M::SB::first(P.b, pass, mm.n0, at * M::BK);
+        const size_t step_a = M::SA::step(P.a), step_b = M::SB::step(P.b);
+        const auto send = [&](int q, int buf) {  // chunk q of both operands' NA + NB
+            if (q < NA)
+                to_lds(pa, oa[q < NA ? q : 0], to + buf * M::BYTES + q * M::NT * 16);
+            else
+                to_lds(pb, ob[q < NA ? 0 : q - NA], to + buf * M::BYTES + M::TA::BYTES + (q - NA) * M::NT * 16);
+        };
+        const auto advance = [&]() {
+            pa += step_a, pb += step_b;
+            if (++at == full) {
+                at = 0, pass = min(pass + 1, p1 - 1);
+                pa = M::SA::first(P.a, pass, mm.m0, 0), pb = M::SB::first(P.b, pass, mm.n0, 0);
+            }
+        };
+        frag fa[FM], fb[2][FN];
+#pragma unroll
+        for (int q = 0; q < NA + NB; q++) send(q, 0);
+        advance();
+        wait_loads();
+        __syncthreads();
+        if (t0 + 1 < t1) {
+#pragma unroll
+            for (int q = 0; q < NA + NB; q++) send(q, 1);
+            advance();
+        }
+#pragma unroll
+        for (int j = 0; j < FM; j++) fa[j] = mm.read_a(0, j, 0);
+#pragma unroll
+        for (int i = 0; i < FN; i++) fb[0][i] = mm.read_b(0, i, 0);
+        // The products of half 1 - s, and beside them: fragments of half s of the tile in buffer `buf` (of m: into the registers
+        // just used; of n: into a second set), and with SEND the next tile's chunks into buffer `to_buf`.
+        const auto half = [&](auto s_, auto send_, int buf, int to_buf) {
+            constexpr int s = decltype(s_)::value;
+            constexpr bool SEND = decltype(send_)::value;
+#pragma unroll
+            for (int j = 0; j < FM; j++) {
+                if (SEND) {
+#pragma unroll
+                    for (int q = (NA + NB) * j / FM; q < (NA + NB) * (j + 1) / FM; q++) send(q, to_buf);
+                }
+#pragma unroll
+                for (int i = FN * j / FM; i < FN * (j + 1) / FM; i++) fb[s][i] = mm.read_b(buf, i, s);
+                mma_col<T, FM, FN>(mm.acc, j, fb[1 - s], fa[j]);
+                fa[j] = mm.read_a(buf, j, s);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        const std::integral_constant<int, 0> zero;
+        const std::integral_constant<int, 1> one;
+        int kt = t0, cur = 0;
+        for (; kt + 2 < t1; kt++, cur ^= 1) {
+            half(one, std::false_type(), cur, 0);
+            wait_loads();
+            __syncthreads();  // the next tile is here, and every wave has read this one
+            half(zero, std::true_type(), cur ^ 1, cur);
+            advance();
+        }
+        for (; kt < t1; kt++, cur ^= 1) {
+            half(one, std::false_type(), cur, 0);
+            wait_loads();
+            __syncthreads();
+            half(zero, std::false_type(), cur ^ 1, 0);  // (behind the last tile: fragments that nothing uses)
+        }
+    }
+    if (last)
+        for (int pass = p0; pass < p1; pass++)
+            for (int k0 = rest; k0 < P.k; k0 += M::BK) mm.plain_tile(pass, k0);
+    mm.finish();
 }
 
 // the splits' sums added in order, then the epilogue
@@ -363,7 +489,10 @@ __global__ __launch_bounds__(256) void affine_join(Product P) {
     if (q >= cols * P.m) return;
     const int m = (int)(q / cols), n = (int)(q % cols) * 4;
     v4f v = {0, 0, 0, 0};
-    for (int s = 0; s < P.splits; s++) v += *(const v4f *)(P.part + ((size_t)s * P.m + m) * P.part_ld + n);
+    for (int s = 0; s < P.splits; s++) {
+        if (P.lift && s == P.splits / 2) v *= 1.0f / F16_LIFT;
+        v += *(const v4f *)(P.part + ((size_t)s * P.m + m) * P.part_ld + n);
+    }
     finish4<T, OUT>(P.e, m, n, P.n - n, v);
 }
 
@@ -391,7 +520,6 @@ __global__ __launch_bounds__(256) void affine_round_w(const float *__restrict__ 
 // where the product is rounded to bf16 anyway). And the column sums of gz over this workgroup's rows.
 // Thread (c, r) takes column chunk c and every 8th row from r on.
 constexpr int GZ_COLS = 32, GZ_ROWS = 8;
-constexpr float F16_LIFT = 2048.0f;
 template <typename T>
 struct Summands {
     T *p[3];  // largest first
@@ -500,7 +628,7 @@ struct Shape {
 };
 // Tile and split: 128 x 128 tiles where they give every CU one; smaller tiles, then several workgroups on one tile's k,
 // where they do not.
-Shape shape_of(int m, int n, int k, int passes, size_t es) {
+Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false) {
     Shape s;
     const auto count = [&](int b) { return (long long)bt_div_up(m, b) * bt_div_up(n, b); };
     s.bm = s.bn = es == 2 && count(256) >= 200 ? 256 : count(128) >= 256 ? 128 : 64;
@@ -509,28 +637,35 @@ Shape shape_of(int m, int n, int k, int passes, size_t es) {
     long long splits = 512 / tiles;
     if (splits > ktiles / 4) splits = ktiles / 4;
     s.splits = splits < 1 ? 1 : splits > 32 ? 32 : (int)splits;
+    if (lift) s.splits += s.splits & 1;
     return s;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, bool DMA>
-int mm_launch(hipStream_t st, const Product &P) {
+// the tile sizes shape_of chooses from, with or without direct loads
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
+int mm_launch(hipStream_t st, const Product &P, bool direct) {
     const long long blocks = (long long)P.tiles_m * P.tiles_n * P.splits;
     BT_REQUIRE(blocks < (1 << 22), "bt_affine: Mismatched sizes! (%lld tiles)", blocks);
-    const size_t lds = 2 * (Tile<T, AK, BM>::BYTES + Tile<T, BKC, BN>::BYTES);
-    const auto kernel = affine_mm<T, BM, BN, WM, WN, AK, BKC, OUT, DMA>;
-    if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
-    BT_LAUNCH(BTK_AFFINE, st, (affine_mm<T, BM, BN, WM, WN, AK, BKC, OUT, DMA>), dim3((unsigned)blocks), dim3(64 * WM * WN), lds, P);
+    const size_t lds = 2 * Mm<T, BM, BN, WM, WN, AK, BKC, OUT>::BYTES;
+    const dim3 grid((unsigned)blocks), block(64 * WM * WN);
+    if (direct) {
+        const auto kernel = affine_mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT>;
+        if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
+        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT>), grid, block, lds, P);
+    } else if constexpr (BM <= 128) {
+        const auto kernel = affine_mm_any<T, BM, BN, WM, WN, AK, BKC, OUT>;
+        if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
+        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_any<T, BM, BN, WM, WN, AK, BKC, OUT>), grid, block, lds, P);
+    }
     BT_LAUNCH_CHECK();
     return BT_OK;
 }
-// the tile sizes shape_of chooses from, with or without direct loads
 template <typename T, bool AK, bool BKC, int OUT>
-int tile_launch(hipStream_t st, const Product &P, const Shape &s, bool dma) {
+int tile_launch(hipStream_t st, const Product &P, const Shape &s, bool direct) {
     if constexpr (sizeof(T) == 2)
-        if (s.bm == 256) return mm_launch<T, 256, 256, 2, 4, AK, BKC, OUT, true>(st, P);
-    if (s.bm == 128)
-        return dma ? mm_launch<T, 128, 128, 2, 2, AK, BKC, OUT, true>(st, P) : mm_launch<T, 128, 128, 2, 2, AK, BKC, OUT, false>(st, P);
-    return dma ? mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT, true>(st, P) : mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT, false>(st, P);
+        if (s.bm == 256) return mm_launch<T, 256, 256, 2, 4, AK, BKC, OUT>(st, P, direct);
+    if (s.bm == 128) return mm_launch<T, 128, 128, 2, 2, AK, BKC, OUT>(st, P, direct);
+    return mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT>(st, P, direct);
 }
 // direct loads need chunks that start on 16 bytes, and reach rows of one tile through 32-bit offsets
 bool direct(const Operand &o) { return o.aligned && o.ld < (1 << 21); }
@@ -580,7 +715,7 @@ int forward(hipStream_t st, const bt_affine_desc *d, const void *w, const float 
     Product P = {};
     if (int rc = make_w<T>(st, d, w, ws, P.b)) return rc;
     P.a = matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
-    P.m = d->batch, P.n = d->out, P.k = d->in, P.passes = 1, P.rescale = 1.0f;
+    P.m = d->batch, P.n = d->out, P.k = d->in, P.passes = 1;
     P.part = (float *)(ws + round_w_bytes(d));
     P.e = Epilogue{bias, residual, y, saved, d->y_ld, d->act, 1.0f};
     return product_launch<T, true, false, OUT_LAYER>(st, P, s);
@@ -589,7 +724,8 @@ int forward(hipStream_t st, const bt_affine_desc *d, const void *w, const float 
 struct BackwardPlan {
     bool gz;             // gz is kept (else grad_y is gz)
     int np_dw, np_dx;    // summands it is kept as for dW (whose outputs are f32), and how many of them grad_x takes
-    float alpha, rescale;
+    float alpha;
+    int lift;
     int range, ranges;
     Shape dw, dx;
     size_t w_bytes, gz_bytes, sum_bytes, part_bytes, total;
@@ -602,12 +738,12 @@ BackwardPlan backward_plan(const bt_affine_desc *d) {
     p.np_dw = !root || es == 4 ? 1 : d->type == BT_TYPE_BF16 ? 3 : 2;
     p.np_dx = p.np_dw > 2 ? 2 : p.np_dw;
     p.alpha = root ? 2.0f : 1.0f;
-    p.rescale = d->type == BT_TYPE_F16 && root ? 1.0f / F16_LIFT : 1.0f;
+    p.lift = d->type == BT_TYPE_F16 && root;
     p.range = 128;
     while (bt_div_up(d->batch, p.range) > 1024) p.range *= 2;
     p.ranges = bt_div_up(d->batch, p.range);
-    p.dw = shape_of(d->in, d->out, d->batch, p.np_dw, es);
-    p.dx = shape_of(d->batch, d->in, d->out, p.np_dx, es);
+    p.dw = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift);
+    p.dx = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift);
     p.w_bytes = round_w_bytes(d);
     p.gz_bytes = p.gz ? bt_align((size_t)d->batch * padded(d->out, es) * es) : 0;
     p.sum_bytes = bt_align((size_t)p.ranges * d->out * 4);
@@ -658,7 +794,7 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
         Product P = {};
         P.a = matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
         P.b = gz_operand(p.np_dw);
-        P.m = d->in, P.n = d->out, P.k = d->batch, P.passes = p.np_dw, P.rescale = p.rescale;
+        P.m = d->in, P.n = d->out, P.k = d->batch, P.passes = p.np_dw, P.lift = p.lift;
         P.part = (float *)part;
         P.e.out = dw, P.e.ld = d->w_ld, P.e.alpha = p.alpha;
         if (int rc = product_launch<T, false, false, OUT_F32>(st, P, p.dw)) return rc;
@@ -667,7 +803,7 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
         Product P = {};
         if (int rc = make_w<T>(st, d, w, w16, P.b)) return rc;
         P.a = gz_operand(p.np_dx);
-        P.m = d->batch, P.n = d->in, P.k = d->out, P.passes = p.np_dx, P.rescale = p.rescale;
+        P.m = d->batch, P.n = d->in, P.k = d->out, P.passes = p.np_dx, P.lift = p.lift;
         P.part = (float *)part;
         P.e.out = gx, P.e.ld = d->x_ld, P.e.alpha = p.alpha;
         if (int rc = product_launch<T, true, true, OUT_TYPE>(st, P, p.dx)) return rc;
