@@ -238,10 +238,6 @@ struct Stage {
 #pragma unroll
         for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = r[q];
     }
-    static __device__ __forceinline__ void copy(const Operand &o, int pass, int s0, int k0, int tid, char *lds) {
-#pragma unroll 1
-        for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = chunk(o, pass, s0, k0, q * NT + tid);
-    }
     // Direct loads: byte offsets of this thread's chunks from the tile's first element, the same for every tile. Rows (or
     // chunks) of m or n beyond the end are taken from the last one: their sums are not stored.
     static __device__ __forceinline__ bool inside(const Operand &o, int s0) { return KC || o.len - s0 >= SPAN || o.len % V == 0; }
@@ -254,6 +250,21 @@ struct Stage {
             if (KC) row = min(row, left - 1);
             if (!KC) c = max(min(c, left / V - 1), 0);
             off[q] = (uint32_t)row * (uint32_t)(o.ld * sizeof(T)) + c * 16;
+        }
+    }
+    // a tile that the matrix does not fill: its whole chunks directly, the others through registers with zeros for what is
+    // not there
+    static __device__ __forceinline__ void careful(const Operand &o, int pass, int s0, int k0, int tid, char *lds) {
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (tid & ~63) * 16);
+        const char *base = first(o, pass, s0, k0);
+#pragma unroll 1
+        for (int q = 0; q < N; q++) {
+            const int s = q * NT + tid, row = s / L::CPR, c = L::swizzle(row, s % L::CPR);
+            const int r = (KC ? s0 : k0) + row, e = (KC ? k0 : s0) + c * V;
+            if (r < o.rows && o.len - e >= V)
+                to_lds(base, (uint32_t)row * (uint32_t)(o.ld * sizeof(T)) + c * 16, to + q * NT * 16);
+            else
+                *(v4u *)(lds + s * 16) = chunk(o, pass, s0, k0, s);
         }
     }
     static __device__ __forceinline__ const char *first(const Operand &o, int pass, int s0, int k0) {
@@ -325,14 +336,6 @@ struct Mm {
             for (int j = 0; j < FM; j++) mma_col<T, FM, FN>(acc, j, fb, fa[j]);
         }
     }
-    // one tile, from memory to sums, with nothing overlapped: tiles that end inside a chunk or inside 128 bytes of k
-    __device__ __forceinline__ void plain_tile(int pass, int k0) {
-        __syncthreads();
-        SA::copy(P.a, pass, m0, k0, tid, lds);
-        SB::copy(P.b, pass, n0, k0, tid, lds + TA::BYTES);
-        __syncthreads();
-        multiply(0);
-    }
     // Lane l holds, of each 16 x 16 block, row m = l % 16 and columns n = 4 (l / 16) .. + 3. Every wave turns 16 rows at a
     // time in its own piece of LDS, so that 16 lanes finish (and load and store) one row's 64 consecutive columns.
     __device__ __forceinline__ void finish() {
@@ -392,7 +395,8 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 // the first half of a tile's k is multiplied the second half's fragments are read; behind the barrier that says that the
 // next tile has arrived its first fragments are read, and the tile after it is sent for into the buffer just left, while
 // the second half is multiplied. Each fragment's products carry their share of those reads and loads.
-// k that does not fill a tile goes through plain_tile at the end.
+// The tiles that the matrices fill come first; the others (the rest of k, one of each summand; all, where the span ends
+// inside a chunk) take the same way with a check of every chunk.
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
@@ -401,84 +405,96 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     extern __shared__ __align__(1024) char lds[];
     M mm(P, lds);
     const bool inside = M::SA::inside(P.a, mm.m0) && M::SB::inside(P.b, mm.n0);
-    const int full = inside ? P.k / M::BK : 0, rest = full * M::BK;
+    const int ktiles = (P.k + M::BK - 1) / M::BK, full = P.k / M::BK;
     int p0, p1, t0, t1;
-    const bool last = mm.share(full, p0, p1, t0, t1);
-    if (t0 < t1) {
-        uint32_t oa[NA], ob[NB];
-        M::SA::offsets(P.a, mm.m0, mm.tid, oa);
-        M::SB::offsets(P.b, mm.n0, mm.tid, ob);
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (mm.tid & ~63) * 16);
-        // the tile to be sent for next: its summand, its number in there, its first elements
-        int pass = p0 + t0 / full, at = t0 % full;
-        const char *pa = M::SA::first(P.a, pass, mm.m0, at * M::BK), *pb = M::SB::first(P.b, pass, mm.n0, at * M::BK);
-        const size_t step_a = M::SA::step(P.a), step_b = M::SB::step(P.b);
-        const auto send = [&](int q, int buf) {  // chunk q of both operands' NA + NB
-            if (q < NA)
-                to_lds(pa, oa[q < NA ? q : 0], to + buf * M::BYTES + q * M::NT * 16);
-            else
-                to_lds(pb, ob[q < NA ? 0 : q - NA], to + buf * M::BYTES + M::TA::BYTES + (q - NA) * M::NT * 16);
-        };
-        const auto advance = [&]() {
-            pa += step_a, pb += step_b;
-            if (++at == full) {
-                at = 0, pass = min(pass + 1, p1 - 1);
-                pa = M::SA::first(P.a, pass, mm.m0, 0), pb = M::SB::first(P.b, pass, mm.n0, 0);
+    const bool last = mm.share(inside ? full : ktiles, p0, p1, t0, t1);
+    const int quick = inside ? t1 - t0 : 0, tiles = !inside ? t1 - t0 : quick + (last && full < ktiles ? p1 - p0 : 0);
+
+    uint32_t oa[NA], ob[NB];
+    M::SA::offsets(P.a, mm.m0, mm.tid, oa);
+    M::SB::offsets(P.b, mm.n0, mm.tid, ob);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (mm.tid & ~63) * 16);
+    // the filled tile to be sent for next: its summand, its number in there, its first elements
+    int pass = p0, at = 0;
+    if (quick) pass += t0 / full, at = t0 % full;
+    const char *pa = M::SA::first(P.a, pass, mm.m0, at * M::BK), *pb = M::SB::first(P.b, pass, mm.n0, at * M::BK);
+    const size_t step_a = M::SA::step(P.a), step_b = M::SB::step(P.b);
+    const auto send = [&](int q, int buf) {  // chunk q of both operands' NA + NB
+        if (q < NA)
+            to_lds(pa, oa[q < NA ? q : 0], to + buf * M::BYTES + q * M::NT * 16);
+        else
+            to_lds(pb, ob[q < NA ? 0 : q - NA], to + buf * M::BYTES + M::TA::BYTES + (q - NA) * M::NT * 16);
+    };
+    const auto advance = [&]() {
+        pa += step_a, pb += step_b;
+        if (++at == full) {
+            at = 0, pass = min(pass + 1, p1 - 1);
+            pa = M::SA::first(P.a, pass, mm.m0, 0), pb = M::SB::first(P.b, pass, mm.n0, 0);
+        }
+    };
+    const auto careful = [&](int tile, int buf) {
+        const int c = inside ? tile - quick : t0 + tile;
+        const int ps = p0 + (inside ? c : c / ktiles), k0 = (inside ? full : c % ktiles) * M::BK;
+        M::SA::careful(P.a, ps, mm.m0, k0, mm.tid, lds + buf * M::BYTES);
+        M::SB::careful(P.b, ps, mm.n0, k0, mm.tid, lds + buf * M::BYTES + M::TA::BYTES);
+    };
+    frag fa[FM], fb[2][FN];
+    // The products of half 1 - s, and beside them: fragments of half s of the tile in buffer `buf` (of m: into the registers
+    // just used; of n: into a second set), and with SEND the next tile's chunks into buffer `to_buf`.
+    const auto half = [&](auto s_, auto send_, int buf, int to_buf) {
+        constexpr int s = decltype(s_)::value;
+        constexpr bool SEND = decltype(send_)::value;
+#pragma unroll
+        for (int j = 0; j < FM; j++) {
+            if (SEND) {
+#pragma unroll
+                for (int q = (NA + NB) * j / FM; q < (NA + NB) * (j + 1) / FM; q++) send(q, to_buf);
             }
-        };
-        frag fa[FM], fb[2][FN];
 #pragma unroll
-        for (int q = 0; q < NA + NB; q++) send(q, 0);
-        advance();
-        wait_loads();
-        __syncthreads();
-        if (t0 + 1 < t1) {
+            for (int i = FN * j / FM; i < FN * (j + 1) / FM; i++) fb[s][i] = mm.read_b(buf, i, s);
+            mma_col<T, FM, FN>(mm.acc, j, fb[1 - s], fa[j]);
+            fa[j] = mm.read_a(buf, j, s);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const std::integral_constant<int, 0> zero;
+    const std::integral_constant<int, 1> one;
+    if (tiles > 0) {
+#pragma unroll 1
+        for (int t = 0; t < 2 && t < tiles; t++) {
+            if (t < quick) {
 #pragma unroll
-            for (int q = 0; q < NA + NB; q++) send(q, 1);
-            advance();
+                for (int q = 0; q < NA + NB; q++) send(q, t);
+                advance();
+            } else {
+                careful(t, t);
+            }
+            if (t == 0) {
+                wait_loads();
+                __syncthreads();
+            }
         }
 #pragma unroll
         for (int j = 0; j < FM; j++) fa[j] = mm.read_a(0, j, 0);
 #pragma unroll
         for (int i = 0; i < FN; i++) fb[0][i] = mm.read_b(0, i, 0);
-        // The products of half 1 - s, and beside them: fragments of half s of the tile in buffer `buf` (of m: into the registers
-        // just used; of n: into a second set), and with SEND the next tile's chunks into buffer `to_buf`.
-        const auto half = [&](auto s_, auto send_, int buf, int to_buf) {
-            constexpr int s = decltype(s_)::value;
-            constexpr bool SEND = decltype(send_)::value;
-#pragma unroll
-            for (int j = 0; j < FM; j++) {
-                if (SEND) {
-#pragma unroll
-                    for (int q = (NA + NB) * j / FM; q < (NA + NB) * (j + 1) / FM; q++) send(q, to_buf);
-                }
-#pragma unroll
-                for (int i = FN * j / FM; i < FN * (j + 1) / FM; i++) fb[s][i] = mm.read_b(buf, i, s);
-                mma_col<T, FM, FN>(mm.acc, j, fb[1 - s], fa[j]);
-                fa[j] = mm.read_a(buf, j, s);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        const std::integral_constant<int, 0> zero;
-        const std::integral_constant<int, 1> one;
-        int kt = t0, cur = 0;
-        for (; kt + 2 < t1; kt++, cur ^= 1) {
-            half(one, std::false_type(), cur, 0);
-            wait_loads();
-            __syncthreads();  // the next tile is here, and every wave has read this one
-            half(zero, std::true_type(), cur ^ 1, cur);
-            advance();
-        }
-        for (; kt < t1; kt++, cur ^= 1) {
-            half(one, std::false_type(), cur, 0);
-            wait_loads();
-            __syncthreads();
-            half(zero, std::false_type(), cur ^ 1, 0);  // (behind the last tile: fragments that nothing uses)
-        }
     }
-    if (last)
-        for (int pass = p0; pass < p1; pass++)
-            for (int k0 = rest; k0 < P.k; k0 += M::BK) mm.plain_tile(pass, k0);
+    int t = 0, cur = 0;
+    for (; t + 2 < quick; t++, cur ^= 1) {
+        half(one, std::false_type(), cur, 0);
+        wait_loads();
+        __syncthreads();  // the next tile is here, and every wave has read this one
+        half(zero, std::true_type(), cur ^ 1, cur);
+        advance();
+    }
+#pragma unroll 1
+    for (; t < tiles; t++, cur ^= 1) {
+        half(one, std::false_type(), cur, 0);
+        wait_loads();
+        __syncthreads();
+        if (t + 2 < tiles) careful(t + 2, cur);
+        half(zero, std::false_type(), cur ^ 1, 0);  // (behind the last tile: fragments that nothing uses)
+    }
     mm.finish();
 }
 
@@ -496,22 +512,108 @@ __global__ __launch_bounds__(256) void affine_join(Product P) {
     finish4<T, OUT>(P.e, m, n, P.n - n, v);
 }
 
-// f32 weights rounded to the layer's type, rows `to_ld` apart
-template <typename T>
-__global__ __launch_bounds__(256) void affine_round_w(const float *__restrict__ from, long long from_ld, T *__restrict__ to,
-                                                      long long to_ld, int rows, int len) {
-    const long long q = (long long)blockIdx.x * 256 + threadIdx.x, cols = (len + 3) / 4;
+// A matrix with rows on 16 bytes (and f32 weights rounded to the layer's type) for the direct loads: `to_ld` is `len` up to
+// a whole chunk, filled with zeros. One chunk a thread.
+template <typename From, typename T>
+__global__ __launch_bounds__(256) void affine_copy(const From *__restrict__ from, long long from_ld, T *__restrict__ to,
+                                                   long long to_ld, int rows, int len) {
+    constexpr int V = Elem<T>::V;
+    const long long q = (long long)blockIdx.x * 256 + threadIdx.x, cols = to_ld / V;
     if (q >= cols * rows) return;
     const long long row = q / cols;
-    const int c = (int)(q % cols) * 4;
-    v4f v = {0, 0, 0, 0};
-    const float *p = from + row * from_ld + c;
-    if (len - c >= 4) {
-        __builtin_memcpy(&v, p, 16);
+    const int c = (int)(q % cols) * V;
+    const From *p = from + row * from_ld + c;
+    typedef From vec __attribute__((ext_vector_type(V)));
+    vec v = {};
+    if (len - c >= V) {
+        __builtin_memcpy(&v, p, sizeof(v));
     } else {
-        for (int j = 0; j < len - c; j++) v[j] = p[j];
+#pragma unroll
+        for (int j = 0; j < V; j++)
+            if (j < len - c) v[j] = p[j];
     }
-    store4<T>(to + row * to_ld + c, v, len - c);
+    typename Elem<T>::frag r;
+#pragma unroll
+    for (int j = 0; j < V; j++) r[j] = (T)(float)v[j];
+    *(typename Elem<T>::frag *)(to + row * to_ld + c) = r;
+}
+
+// Forward of at most R rows (one position, or a few): the weights are all there is to read, and each is used R times, so
+// there is nothing for the matrix cores. A workgroup of 1024 takes 4 chunks of outputs (64 bytes of every weight column;
+// f32 weights of a 16-bit layer: 128) for all inputs: 256 groups of 4 lanes walk the inputs V at a time with V weight loads
+// in flight each, and their sums meet in DPP, shuffles and LDS, in a fixed order.
+template <typename T, typename TW, int R>
+__global__ __launch_bounds__(1024) void affine_few(const TW *__restrict__ w, long long w_ld, const T *__restrict__ x, long long x_ld,
+                                                   int batch, int in, int out, Epilogue e) {
+    constexpr int V = Elem<T>::V, COLS = 4 * V;
+    typedef TW wvec __attribute__((ext_vector_type(V)));
+    typedef typename Elem<T>::frag xvec;
+    __shared__ __align__(16) float red[16][R][COLS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 2;
+    const int c = blockIdx.x * COLS + (threadIdx.x & 3) * V;
+    float acc[R][V];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < V; j++) acc[r][j] = 0.0f;
+    for (long long k = (long long)group * V; k < in; k += 256 * V) {
+        const int nk = in - k < V ? (int)(in - k) : V;
+        wvec wv[V];
+        xvec xv[R];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            wv[i] = wvec{};
+            if (i < nk) {
+                const TW *p = w + (k + i) * w_ld + c;
+                if (out - c >= V) {
+                    __builtin_memcpy(&wv[i], p, sizeof(wvec));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; j++)
+                        if (j < out - c) wv[i][j] = p[j];
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const T *p = x + (long long)min(r, batch - 1) * x_ld + k;
+            xv[r] = xvec{};
+            if (nk == V) {
+                __builtin_memcpy(&xv[r], p, 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    if (i < nk) xv[r][i] = p[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < nk)
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const float f = (float)(T)wv[i][j];
+#pragma unroll
+                    for (int r = 0; r < R; r++) acc[r][j] = fmaf((float)xv[r][i], f, acc[r][j]);
+                }
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            float v = acc[r][j];  // the 16 lanes of a wave with the same columns
+            v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false));  // 4 lanes on
+            v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));  // 8 lanes on
+            v += __shfl_xor(v, 16, 64);
+            v += __shfl_xor(v, 32, 64);
+            if (lane < 4) red[wave][r][lane * V + j] = v;
+        }
+    __syncthreads();
+    if (threadIdx.x >= R * V) return;  // one thread for 4 outputs of a row
+    const int r = threadIdx.x / V, q = (threadIdx.x % V) * 4, col = blockIdx.x * COLS + q;
+    if (r >= batch || col >= out) return;
+    v4f v = {0, 0, 0, 0};
+    for (int i = 0; i < 16; i++) v += *(const v4f *)&red[i][r][q];
+    finish4<T, OUT_LAYER>(e, r, col, out - col, v);
 }
 
 // gz = grad_y act'(out) (half of it where act' carries a factor 2: the products' alpha gives it back, exactly), as one
@@ -602,9 +704,6 @@ __global__ __launch_bounds__(1024) void affine_dbias(const float *__restrict__ p
 
 // ---- host side
 size_t type_size(int type) { return type == BT_TYPE_F32 ? 4 : 2; }
-bool chunk_aligned(const void *p, long long ld, size_t es) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * es) % 16 == 0;
-}
 bool elem_aligned(const void *p, size_t es) { return (reinterpret_cast<uintptr_t>(p) & (es - 1)) == 0; }
 
 int validate(const bt_affine_desc *d, const char *fn) {
@@ -623,22 +722,38 @@ int validate(const bt_affine_desc *d, const char *fn) {
 }
 
 struct Shape {
-    int bm, bn, tiles_m, tiles_n, splits;
+    int bm, tiles_m, tiles_n, splits;
     size_t part_bytes(int m, int n) const { return splits > 1 ? bt_align((size_t)splits * m * ((n + 3) / 4 * 4) * 4) : 0; }
 };
-// Tile and split: 128 x 128 tiles where they give every CU one; smaller tiles, then several workgroups on one tile's k,
-// where they do not.
+// Tile size and number of workgroups that share a tile's k: the pair whose estimate is lowest. Measured, in us for one
+// tile and 128 bytes of k: alone on its CU, and per workgroup where a CU has several (256 x 256: never more than one).
+//            256        128           64
+//   16-bit   1.75       0.70, 0.48    0.33, 0.18
+//   f32                 2.30, 2.10    0.53, 0.50
+// and for sharing k a launch (4 us) and the partial sums' way through memory (7 TB/s). What this decides, measured both ways
+// (bf16): dW of 16384 x 2048 -> 2048 takes 113 us as 256 / 4, 123 as 128 / 2, 151 as 128 / 1; 4096 x 1024 -> 1024 forward
+// 15.3 us as 64 / 1, 24.8 as 128 / 2, 29.1 as 256 / 1; dW of 8192 x 1024 -> 1880 40.5 us as 128 / 4, 85 as 128 / 1.
 Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false) {
-    Shape s;
-    const auto count = [&](int b) { return (long long)bt_div_up(m, b) * bt_div_up(n, b); };
-    s.bm = s.bn = es == 2 && count(256) >= 200 ? 256 : count(128) >= 256 ? 128 : 64;
-    s.tiles_m = bt_div_up(m, s.bm), s.tiles_n = bt_div_up(n, s.bn);
-    const long long tiles = count(s.bm), ktiles = (long long)bt_div_up(k, (int)(128 / es)) * passes;
-    long long splits = 512 / tiles;
-    if (splits > ktiles / 4) splits = ktiles / 4;
-    s.splits = splits < 1 ? 1 : splits > 32 ? 32 : (int)splits;
-    if (lift) s.splits += s.splits & 1;
-    return s;
+    const struct {
+        int b;
+        double alone, busy;
+    } tiles[] = {{256, 1.75, 1.75}, {128, es == 2 ? 0.70 : 2.30, es == 2 ? 0.48 : 2.10}, {64, es == 2 ? 0.33 : 0.53, es == 2 ? 0.18 : 0.50}};
+    const long long ktiles = (long long)bt_div_up(k, (int)(128 / es)) * passes;
+    Shape best = {};
+    double best_us = 0.0;
+    for (const auto &t : tiles) {
+        if (t.b == 256 && es == 4) continue;
+        const long long count = (long long)bt_div_up(m, t.b) * bt_div_up(n, t.b);
+        for (int splits = lift ? 2 : 1; splits <= 32; splits += lift || splits >= 4 ? 2 : 1) {
+            if (splits > 1 && !lift && ktiles / splits < 2) break;
+            const double each = (double)((ktiles + splits - 1) / splits), per_cu = (double)((count * splits + 255) / 256);
+            double us = each * (per_cu * t.busy > t.alone ? per_cu * t.busy : t.alone);
+            if (splits > 1) us += 4.0 + splits * (double)m * n * 8.0 / 7.0e6;
+            if (best.bm == 0 || us < best_us)
+                best = Shape{t.b, bt_div_up(m, t.b), bt_div_up(n, t.b), splits}, best_us = us;
+        }
+    }
+    return best;
 }
 
 // the tile sizes shape_of chooses from, with or without direct loads
@@ -667,13 +782,10 @@ int tile_launch(hipStream_t st, const Product &P, const Shape &s, bool direct) {
     if (s.bm == 128) return mm_launch<T, 128, 128, 2, 2, AK, BKC, OUT>(st, P, direct);
     return mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT>(st, P, direct);
 }
-// direct loads need chunks that start on 16 bytes, and reach rows of one tile through 32-bit offsets
-bool direct(const Operand &o) { return o.aligned && o.ld < (1 << 21); }
-
 template <typename T, bool AK, bool BKC, int OUT>
 int product_launch(hipStream_t st, Product &P, Shape s) {
-    const bool dma = direct(P.a) && direct(P.b);
-    if (s.bm == 256 && !dma) s.bm = s.bn = 128, s.tiles_m = bt_div_up(P.m, 128), s.tiles_n = bt_div_up(P.n, 128);
+    const bool dma = P.a.aligned && P.b.aligned;
+    if (s.bm == 256 && !dma) s.bm = 128, s.tiles_m = bt_div_up(P.m, 128), s.tiles_n = bt_div_up(P.n, 128);
     P.tiles_m = s.tiles_m, P.tiles_n = s.tiles_n, P.splits = s.splits;
     P.part_ld = (P.n + 3) / 4 * 4;
     if (s.splits == 1) return tile_launch<T, AK, BKC, OUT>(st, P, s, dma);
@@ -684,57 +796,101 @@ int product_launch(hipStream_t st, Product &P, Shape s) {
 }
 
 long long padded(int n, size_t es) { return (n + (16 / es) - 1) / (16 / es) * (16 / es); }
-bool round_w(const bt_affine_desc *d) { return d->w_type != d->type; }
-size_t round_w_bytes(const bt_affine_desc *d) {
-    return round_w(d) ? bt_align((size_t)d->in * padded(d->out, 2) * 2) : 0;
+// direct loads need rows on 16 bytes, and reach those of one tile through 32-bit offsets
+bool direct_ld(long long ld, size_t es) { return ld * es % 16 == 0 && ld < (1 << 21); }
+Operand matrix(const void *p, long long ld, int rows, int len, size_t es) {
+    return Operand{{p, p, p}, ld, rows, len, (reinterpret_cast<uintptr_t>(p) & 15) == 0 && direct_ld(ld, es)};
 }
+// Matrices that are copied into the workspace first: those whose rows do not start on 16 bytes (read through registers
+// instead, 1537 x 1027 -> 1881 f16 takes 34 us, copied 22), and f32 weights of a 16-bit layer. One whose first element alone is
+// off is read through registers.
+size_t copy_bytes(bool copy, int rows, int len, size_t es) { return copy ? bt_align((size_t)rows * padded(len, es) * es) : 0; }
+bool copy_w(const bt_affine_desc *d) { return d->w_type != d->type || !direct_ld(d->w_ld, type_size(d->type)); }
+bool copy_x(const bt_affine_desc *d) { return !direct_ld(d->x_ld, type_size(d->type)); }
 
-template <typename T>
-int make_w(hipStream_t st, const bt_affine_desc *d, const void *w, void *ws, Operand &o) {
-    o.rows = d->in, o.len = d->out;
-    if (round_w(d)) {
-        const long long ld = padded(d->out, 2), quads = (long long)bt_div_up(d->out, 4) * d->in;
-        BT_LAUNCH(BTK_AFFINE, st, affine_round_w<T>, dim3(bt_div_up(quads, 256)), dim3(256), 0, (const float *)w, (long long)d->w_ld,
-                  (T *)ws, ld, d->in, d->out);
-        BT_LAUNCH_CHECK();
-        o.p[0] = o.p[1] = o.p[2] = ws, o.ld = ld;
-    } else {
-        o.p[0] = o.p[1] = o.p[2] = w, o.ld = d->w_ld;
-    }
-    o.aligned = chunk_aligned(o.p[0], o.ld, sizeof(T));
+template <typename From, typename T>
+int copy_launch(hipStream_t st, const void *from, long long ld, void *to, int rows, int len, Operand &o) {
+    const long long to_ld = padded(len, sizeof(T)), chunks = to_ld / Elem<T>::V * rows;
+    BT_LAUNCH(BTK_AFFINE, st, (affine_copy<From, T>), dim3(bt_div_up(chunks, 256)), dim3(256), 0, (const From *)from, ld, (T *)to,
+              to_ld, rows, len);
+    BT_LAUNCH_CHECK();
+    o = matrix(to, to_ld, rows, (int)to_ld, sizeof(T));  // (the zeros behind a row are part of it)
     return BT_OK;
 }
-Operand matrix(const void *p, long long ld, int rows, int len, size_t es) {
-    return Operand{{p, p, p}, ld, rows, len, chunk_aligned(p, ld, es)};
+template <typename T>
+int make_w(hipStream_t st, const bt_affine_desc *d, const void *w, void *ws, Operand &o) {
+    o = matrix(w, d->w_ld, d->in, d->out, sizeof(T));
+    if (!copy_w(d)) return BT_OK;
+    if (d->w_type != d->type) return copy_launch<float, T>(st, w, d->w_ld, ws, d->in, d->out, o);
+    return copy_launch<T, T>(st, w, d->w_ld, ws, d->in, d->out, o);
+}
+template <typename T>
+int make_x(hipStream_t st, const bt_affine_desc *d, const void *x, void *ws, Operand &o) {
+    o = matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
+    return copy_x(d) ? copy_launch<T, T>(st, x, d->x_ld, ws, d->batch, d->in, o) : BT_OK;
 }
 
+constexpr int FEW = 8;  // rows that affine_few takes
+template <typename T, typename TW>
+int few_launch(hipStream_t st, const bt_affine_desc *d, const void *w, const void *x, const Epilogue &e) {
+    const dim3 grid(bt_div_up(d->out, 4 * Elem<T>::V)), block(1024);
+#define FEW_CASE(R)                                                                                                                  BT_LAUNCH(BTK_AFFINE, st, (affine_few<T, TW, R>), grid, block, 0, (const TW *)w, (long long)d->w_ld, (const T *)x,               (long long)d->x_ld, d->batch, d->in, d->out, e)
+    if (d->batch == 1)
+        FEW_CASE(1);
+    else if (d->batch == 2)
+        FEW_CASE(2);
+    else if (d->batch <= 4)
+        FEW_CASE(4);
+    else
+        FEW_CASE(FEW);
+#undef FEW_CASE
+    BT_LAUNCH_CHECK();
+    return BT_OK;
+}
+
+struct ForwardPlan {
+    Shape s;
+    size_t w_bytes, x_bytes, total;
+};
+ForwardPlan forward_plan(const bt_affine_desc *d) {
+    ForwardPlan p = {};
+    if (d->batch <= FEW) return p;
+    const size_t es = type_size(d->type);
+    p.s = shape_of(d->batch, d->out, d->in, 1, es);
+    p.w_bytes = copy_bytes(copy_w(d), d->in, d->out, es), p.x_bytes = copy_bytes(copy_x(d), d->batch, d->in, es);
+    p.total = p.w_bytes + p.x_bytes + p.s.part_bytes(d->batch, d->out);
+    return p;
+}
 template <typename T>
 int forward(hipStream_t st, const bt_affine_desc *d, const void *w, const float *bias, const void *x, const void *residual, void *y,
             void *saved, char *ws) {
-    const Shape s = shape_of(d->batch, d->out, d->in, 1, sizeof(T));
+    const Epilogue e{bias, residual, y, saved, d->y_ld, d->act, 1.0f};
+    if (d->batch <= FEW)
+        return d->w_type == d->type ? few_launch<T, T>(st, d, w, x, e) : few_launch<T, float>(st, d, w, x, e);
+    const ForwardPlan p = forward_plan(d);
     Product P = {};
     if (int rc = make_w<T>(st, d, w, ws, P.b)) return rc;
-    P.a = matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
+    if (int rc = make_x<T>(st, d, x, ws + p.w_bytes, P.a)) return rc;
     P.m = d->batch, P.n = d->out, P.k = d->in, P.passes = 1;
-    P.part = (float *)(ws + round_w_bytes(d));
-    P.e = Epilogue{bias, residual, y, saved, d->y_ld, d->act, 1.0f};
-    return product_launch<T, true, false, OUT_LAYER>(st, P, s);
+    P.part = (float *)(ws + p.w_bytes + p.x_bytes);
+    P.e = e;
+    return product_launch<T, true, false, OUT_LAYER>(st, P, p.s);
 }
 
 struct BackwardPlan {
-    bool gz;             // gz is kept (else grad_y is gz)
+    bool gz;             // gz is kept, with rows on 16 bytes (else grad_y is gz)
     int np_dw, np_dx;    // summands it is kept as for dW (whose outputs are f32), and how many of them grad_x takes
     float alpha;
     int lift;
     int range, ranges;
     Shape dw, dx;
-    size_t w_bytes, gz_bytes, sum_bytes, part_bytes, total;
+    size_t w_bytes, x_bytes, gz_bytes, sum_bytes, part_bytes, total;
 };
 BackwardPlan backward_plan(const bt_affine_desc *d) {
     BackwardPlan p;
     const size_t es = type_size(d->type);
     const bool root = d->act == BT_ACT_SCRELU || d->act == BT_ACT_SQRRELU;
-    p.gz = d->act != BT_ACT_IDENTITY;
+    p.gz = d->act != BT_ACT_IDENTITY || !direct_ld(d->y_ld, es);
     p.np_dw = !root || es == 4 ? 1 : d->type == BT_TYPE_BF16 ? 3 : 2;
     p.np_dx = p.np_dw > 2 ? 2 : p.np_dw;
     p.alpha = root ? 2.0f : 1.0f;
@@ -744,12 +900,12 @@ BackwardPlan backward_plan(const bt_affine_desc *d) {
     p.ranges = bt_div_up(d->batch, p.range);
     p.dw = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift);
     p.dx = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift);
-    p.w_bytes = round_w_bytes(d);
+    p.w_bytes = copy_bytes(copy_w(d), d->in, d->out, es), p.x_bytes = copy_bytes(copy_x(d), d->batch, d->in, es);
     p.gz_bytes = p.gz ? bt_align((size_t)d->batch * padded(d->out, es) * es) : 0;
     p.sum_bytes = bt_align((size_t)p.ranges * d->out * 4);
     const size_t a = p.dw.part_bytes(d->in, d->out), b = p.dx.part_bytes(d->batch, d->in);
     p.part_bytes = a > b ? a : b;
-    p.total = p.w_bytes + p.gz_bytes * p.np_dw + p.sum_bytes + p.part_bytes;
+    p.total = p.w_bytes + p.x_bytes + p.gz_bytes * p.np_dw + p.sum_bytes + p.part_bytes;
     return p;
 }
 
@@ -757,7 +913,7 @@ template <typename T>
 int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void *x, const void *out, const void *gy, float *dw,
              float *dbias, void *gx, char *ws) {
     const BackwardPlan p = backward_plan(d);
-    char *w16 = ws, *kept = w16 + p.w_bytes, *sums = kept + p.gz_bytes * p.np_dw, *part = sums + p.sum_bytes;
+    char *own_w = ws, *own_x = own_w + p.w_bytes, *kept = own_x + p.x_bytes, *sums = kept + p.gz_bytes * p.np_dw, *part = sums + p.sum_bytes;
     const bool keep = p.gz && (dw || gx);
     const int np = !keep ? 1 : dw ? p.np_dw : p.np_dx;
     if (keep || dbias) {
@@ -765,7 +921,7 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
         Summands<T> gz = {{nullptr, nullptr, nullptr}};
         for (int i = 0; i < np && keep; i++) gz.p[i] = (T *)(kept + i * p.gz_bytes);
         float *sum = dbias ? (float *)sums : nullptr;
-        const T *o = p.gz ? (const T *)out : nullptr;
+        const T *o = d->act != BT_ACT_IDENTITY ? (const T *)out : nullptr;
         const long long ld = d->y_ld, gz_ld = padded(d->out, sizeof(T));
 #define GZ_CASE(NP)                                                                                                          BT_LAUNCH(BTK_AFFINE, st, (affine_gz<T, NP>), grid, dim3(256), 0, (const T *)gy, o, ld, gz, gz_ld, sum, d->batch, d->out,               d->act, p.range)
         if (np == 1)
@@ -786,13 +942,14 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
     }
     const auto gz_operand = [&](int n) {  // its n largest summands, the smallest of them first
         if (!p.gz) return matrix(gy, d->y_ld, d->batch, d->out, sizeof(T));
-        Operand o = matrix(kept, padded(d->out, sizeof(T)), d->batch, d->out, sizeof(T));
+        const long long ld = padded(d->out, sizeof(T));  // (the zeros behind a row are part of it)
+        Operand o = matrix(kept, ld, d->batch, (int)ld, sizeof(T));
         for (int i = 0; i < n; i++) o.p[i] = kept + (n - 1 - i) * p.gz_bytes;
         return o;
     };
     if (dw) {
         Product P = {};
-        P.a = matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
+        if (int rc = make_x<T>(st, d, x, own_x, P.a)) return rc;
         P.b = gz_operand(p.np_dw);
         P.m = d->in, P.n = d->out, P.k = d->batch, P.passes = p.np_dw, P.lift = p.lift;
         P.part = (float *)part;
@@ -801,7 +958,7 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
     }
     if (gx) {
         Product P = {};
-        if (int rc = make_w<T>(st, d, w, w16, P.b)) return rc;
+        if (int rc = make_w<T>(st, d, w, own_w, P.b)) return rc;
         P.a = gz_operand(p.np_dx);
         P.m = d->batch, P.n = d->in, P.k = d->out, P.passes = p.np_dx, P.lift = p.lift;
         P.part = (float *)part;
@@ -817,7 +974,7 @@ extern "C" {
 
 size_t bt_affine_forward_workspace_bytes(const bt_affine_desc *d) {
     if (validate(d, "bt_affine_forward_workspace_bytes")) return 0;
-    return round_w_bytes(d) + shape_of(d->batch, d->out, d->in, 1, type_size(d->type)).part_bytes(d->batch, d->out);
+    return forward_plan(d).total;
 }
 
 int bt_affine_forward(void *stream, const bt_affine_desc *d, const void *w, const float *bias, const void *x,

@@ -276,3 +276,21 @@ def test_replayed_from_a_graph_and_on_another_stream():
                 torch.cuda.synchronize()
                 for k, v in out_t.items():
                     assert torch.equal(v, want[k]), (kind, step, how, k)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_on_16_bytes_behind_a_first_element_that_is_not(kind):
+    rng = np.random.default_rng(12)
+    for batch, in_, out in ((5, 40, 72), (140, 200, 264), (300, 72, 136)):
+        run_forward(rng, batch, in_, out, kind, "crelu", residual=True, pad=8, shift=1)
+        run_backward(rng, batch, in_, out, kind, "identity", pad=8, shift=1)
+        run_backward(rng, batch, in_, out, kind, "screlu", pad=8, shift=3)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_few_rows(kind):
+    """one position or a handful: the kernel without matrix cores, every width of its column chunks and tails of k"""
+    rng = np.random.default_rng(13)
+    for batch in (1, 2, 3, 4, 5, 8):
+        for in_, out in ((1, 1), (7, 33), (2048, 64), (2049, 31), (513, 1000)):
+            run_forward(rng, batch, in_, out, kind, "screlu", residual=batch % 2 == 0, w32=batch % 3 == 0, pad=batch % 4, shift=batch % 2)
