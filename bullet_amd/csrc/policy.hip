@@ -20,14 +20,54 @@ struct Row {
     typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint64_t>::type bytes;  // one mask byte per element
 };
 
-// exp(x) for x <= 0 with the rounding of x * log2(e) carried along (x to -100 would lose 7 bits otherwise); below -150 it
-// is 0 in 32 bits, and the select keeps -infinity out of the correction but lets NaN pass
-__device__ __forceinline__ float exp_neg(float x) {
-    const float c = x < -150.0f ? -150.0f : x;
-    const float t = c * 1.44269502f;
-    const float lo = fmaf(c, 1.92596303e-8f, fmaf(c, 1.44269502f, -t));  // c * log2(e) - t
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, lo * 0.693147182f, e);
+// exp(x) for x <= 0 in 32 bits: the rounding of x log2(e) costs 2^-24 |x| of the result, and terms with |x| in the tens have
+// no weight in a sum beside one that is 1. -infinity gives 0, NaN stays.
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+
+// The scalars of a row in 64 bits, each computed by all its lanes, so shorter than the library's functions: their arguments
+// are finite sums and differences of logits, and 1e-13 is plenty.
+// e^x = 2^n e^r, n = round(x log2 e), |r| <= ln 2 / 2, by the Taylor series to r^11 / 11! (remainder below 1e-14).
+__device__ __forceinline__ double exp64(double x) {
+    const double n = rint(x * 1.4426950408889634074);
+    double r = fma(n, -6.93147180369123816490e-1, x);  // ln 2 in two parts, the first with zeros at its end
+    r = fma(n, -1.90821492927058770002e-10, r);
+    double p = 1.0 / 39916800.0;
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    const double m = fmin(fmax(n, -1100.0), 1100.0);
+    const double v = ldexp(p, (int)m);
+    // (beyond the range of r's reduction, and infinities: the limits; NaN goes through)
+    return x > 709.0 ? __builtin_huge_val() : x < -745.0 ? 0.0 : v;
+}
+// log s for a normal s > 0: s = 2^n m, m in [sqrt 1/2, sqrt 2), log m = 2 atanh t, t = (m - 1) / (m + 1), |t| <= 0.172, by its
+// series to t^15 / 15 (remainder below 1e-14)
+__device__ __forceinline__ double log64(double s) {
+    int n;
+    double m = frexp(s, &n);  // [1/2, 1)
+    if (m < 0.70710678118654752440) m *= 2.0, n -= 1;
+    const double d = m + 1.0;
+    double i = __builtin_amdgcn_rcp(d);
+    i = i * fma(-d, i, 2.0);
+    i = i * fma(-d, i, 2.0);
+    const double t = (m - 1.0) * i, u = t * t;
+    double p = 2.0 / 15.0;
+    p = fma(p, u, 2.0 / 13.0);
+    p = fma(p, u, 2.0 / 11.0);
+    p = fma(p, u, 2.0 / 9.0);
+    p = fma(p, u, 2.0 / 7.0);
+    p = fma(p, u, 2.0 / 5.0);
+    p = fma(p, u, 2.0 / 3.0);
+    p = fma(p, u, 2.0);
+    return fma((double)n, 0.69314718055994530942, t * p);
 }
 
 // a launch holds less than 2^32 threads a dimension: many rows fold into the grid's second one
@@ -113,10 +153,13 @@ __device__ __forceinline__ void load_chunk(const T *row, int e0, int width, type
         }
     }
 }
+// (without a mask only a row's last chunk can have anything to leave out; chunks beyond it count as such)
 template <typename T>
-__device__ __forceinline__ void keep_legal(typename Row<T>::bytes b, typename Row<T>::vec &v) {
+__device__ __forceinline__ void keep_legal(const uint8_t *mask, int e0, int width, typename Row<T>::bytes b, typename Row<T>::vec &v) {
+    if (mask || width - e0 < Row<T>::V) {
 #pragma unroll
-    for (int j = 0; j < Row<T>::V; j++) v[j] = legal_at(b, j) ? v[j] : (T)NEG_INF;
+        for (int j = 0; j < Row<T>::V; j++) v[j] = legal_at(b, j) ? v[j] : (T)NEG_INF;
+    }
 }
 template <typename T>
 __device__ __forceinline__ void store_chunk(T *row, int e0, int width, typename Row<T>::vec v) {
@@ -137,17 +180,28 @@ struct RowStats {
     float cross;          // sum of exp(z - top) (z - q)
 };
 
-// What a row's element needs for its gradient: p = exp(z - top) inv;
-//   g = -ca p (+ ca for the action taken), and for the full KL + ck p (z - q - shift)
+// What a row's element needs for its gradient: with e = exp(z - top), g = ce e (+ a share of its own for the action taken),
+// and for the full KL + ck e (z - q - shift). Masked (and vanishing) places, e = 0, get 0 whatever the row's scalars are.
 struct RowGrad {
-    float top, inv, ca, ck, shift;
+    float top, ce, ck, shift;
+    bool plain;  // ce is finite: ce e is 0 by itself where e is
 };
-template <bool FULL>
-__device__ __forceinline__ float row_grad(float e, float z, float q, const RowGrad &r) {
-    const float p = e * r.inv;
-    float g = -r.ca * p;
-    if (FULL) g = fmaf(r.ck * p, (z - q) - r.shift, g);
-    return e == 0.0f ? 0.0f : g;  // masked (and vanishing) places have no share, whatever the row's scalars are
+template <typename T, bool FULL>
+__device__ __forceinline__ typename Row<T>::vec grad_chunk(const float (&e)[Row<T>::V], const typename Row<T>::vec &z,
+                                                           const typename Row<T>::vec &q, const RowGrad &r) {
+    typename Row<T>::vec out;
+    if (FULL || !r.plain) {
+#pragma unroll
+        for (int j = 0; j < Row<T>::V; j++) {
+            float g = r.ce * e[j];
+            if (FULL) g = fmaf(r.ck * e[j], ((float)z[j] - (float)q[j]) - r.shift, g);
+            out[j] = (T)(e[j] == 0.0f ? 0.0f : g);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < Row<T>::V; j++) out[j] = (T)(r.ce * e[j]);
+    }
+    return out;
 }
 
 struct PolicyArgs {
@@ -170,36 +224,38 @@ struct PolicyRow {
 __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, const PolicyRow &pr, const RowStats &st, double sum64,
                                                bool full, RowGrad &g, double &logp, double &kl, float &loss, float &grad_taken) {
     const bt_policy_desc &d = a.d;
-    const double logsum = log(sum64 > 0.0 ? sum64 : (double)st.sum);
+    const double logsum = log64(sum64 > 0.0 ? sum64 : (double)st.sum);
     logp = ((double)pr.za - (double)st.top) - logsum;
     const double adv = a.advantages[row], w = a.weights ? (double)a.weights[row] : 1.0;
-    const double r = exp(logp - (double)a.old_logp[row]);
+    const double r = exp64(logp - (double)a.old_logp[row]);
     const double lo = 1.0 - (double)d.clip_low, hi = 1.0 + (double)d.clip_high;
     // a 32-bit sum of up to 2^24 terms is off by less than 1e-5 of itself
     const bool near = fabs(r - lo) < 1e-5 * lo || fabs(r - hi) < 1e-5 * hi;
     const double free_gain = r * adv, held_gain = fmin(fmax(r, lo), hi) * adv;
     double slope = free_gain <= held_gain || free_gain != free_gain ? -free_gain : 0.0;
     kl = 0.0;
-    g.ck = 0.0f;
+    double ck = 0.0;
     g.shift = 0.0f;
     if (d.kl == BT_KL_TAKEN) {
         const double x = (double)((const float *)a.ref)[row] - logp;
-        const double em1 = expm1(x);
+        const double em1 = exp64(x) - 1.0;  // (off by 1e-15 of 1: d^2 / 2, what is left of small differences, stands 1e9 above)
         kl = em1 - x;
         slope -= (double)d.kl_weight * em1;
     } else if (full) {
-        const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log((double)st.ref_sum));
+        const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log64((double)st.ref_sum));
         kl = (double)st.cross / (double)st.sum - dl;
-        g.ck = (float)(w * (double)d.kl_weight);
+        ck = w * (double)d.kl_weight;
         g.shift = (float)(dl + kl);
     }
     loss = (float)(w * ((double)d.kl_weight * kl - (free_gain != free_gain ? free_gain : fmin(free_gain, held_gain))));
     g.top = st.top;
-    g.inv = (float)(1.0 / (double)st.sum);
-    g.ca = (float)(w * slope);
-    const double pa = exp(logp);
+    const float inv = 1.0f / st.sum;
+    g.ce = -(float)(w * slope) * inv;
+    g.ck = (float)ck * inv;
+    g.plain = fabsf(g.ce) < __builtin_huge_valf();
+    const double pa = exp64(logp);
     grad_taken = (float)(w * slope * (1.0 - pa));
-    if (full && pa > 0.0) grad_taken += (float)((double)g.ck * pa * (((double)pr.za - (double)pr.qa) - (double)g.shift));
+    if (full && pa > 0.0) grad_taken += (float)(ck * pa * (((double)pr.za - (double)pr.qa) - (double)g.shift));
     return near;
 }
 
@@ -260,11 +316,11 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
     float top = NEG_INF, ref_top = NEG_INF;
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        keep_legal<T>(b[k], zc[k]);
+        keep_legal<T>(mask, (lane + k * G) * V, width, b[k], zc[k]);
 #pragma unroll
         for (int j = 0; j < V; j++) top = fmaxf(top, (float)zc[k][j]);
         if (FULL) {
-            keep_legal<T>(b[k], qc[FULL ? k : 0]);
+            keep_legal<T>(mask, (lane + k * G) * V, width, b[k], qc[FULL ? k : 0]);
 #pragma unroll
             for (int j = 0; j < V; j++) ref_top = fmaxf(ref_top, (float)qc[FULL ? k : 0][j]);
         }
@@ -313,11 +369,7 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
     if (!grad) return;
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        vec out;
-#pragma unroll
-        for (int j = 0; j < V; j++)
-            out[j] = (T)row_grad<FULL>(e[k][j], FULL ? (float)zc[k][j] : 0.0f, FULL ? (float)qc[FULL ? k : 0][j] : 0.0f, g);
-        store_chunk<T>(grad, (lane + k * G) * V, width, out);
+        store_chunk<T>(grad, (lane + k * G) * V, width, grad_chunk<T, FULL>(e[k], zc[k], qc[FULL ? k : 0], g));
     }
     // the action taken: written again by the lane that wrote its chunk
     const int act = a.actions[row];
@@ -344,10 +396,10 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
         const bytes b = legal_bytes<T>(mask, (int)e0, width);
         vec zc, qc;
         load_chunk<T>(z, (int)e0, width, b, zc);
-        keep_legal<T>(b, zc);
+        keep_legal<T>(mask, (int)e0, width, b, zc);
         if (FULL) {
             load_chunk<T>(q, (int)e0, width, b, qc);
-            keep_legal<T>(b, qc);
+            keep_legal<T>(mask, (int)e0, width, b, qc);
         }
         float m = top, mq = ref_top;
         for (int j = 0; j < V; j++) {
@@ -392,17 +444,16 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
         vec out = {};
         if (counted) {
             const bytes b = legal_bytes<T>(mask, (int)e0, width);
-            vec zc, qc;
+            vec zc = {}, qc = {};
             load_chunk<T>(z, (int)e0, width, b, zc);
-            keep_legal<T>(b, zc);
+            keep_legal<T>(mask, (int)e0, width, b, zc);
             if (FULL) {
                 load_chunk<T>(q, (int)e0, width, b, qc);
-                keep_legal<T>(b, qc);
+                keep_legal<T>(mask, (int)e0, width, b, qc);
             }
-            for (int j = 0; j < V; j++) {
-                const float zv = (float)zc[j];
-                out[j] = (T)row_grad<FULL>(exp_neg(zv - g.top), zv, FULL ? (float)qc[j] : 0.0f, g);
-            }
+            float e[V];
+            for (int j = 0; j < V; j++) e[j] = exp_neg((float)zc[j] - g.top);
+            out = grad_chunk<T, FULL>(e, zc, qc, g);
         }
         store_chunk<T>(grad, (int)e0, width, out);
     }
@@ -432,19 +483,12 @@ struct PrefArgs {
     const float *ref, *weights;
     void *grad;
     float *pair_loss, *line_logp;
-    double *logp;  // [rows] log-probability of the action taken, 0 where the row is not counted
-    float *top;    // [rows] largest legal logit
-    float *inv;    // [rows] 1 / sum of exp(z - top), 0 where the row is not counted
-    float *slope;  // [pairs] d loss / d s of the preferred line
+    // per row: logit of the action taken, the largest legal one, the sum of exp(z - top) (0: the row is not
+    // counted), and what the pair kernel adds: the gradient's factor on p and the taken action's own gradient
+    float *za, *top, *sum, *ce, *taken;
     bt_preference_desc d;
 };
 __device__ __forceinline__ int pref_offset(const PrefArgs &a, int k) { return min(max(a.offsets[k], 0), a.d.rows); }
-
-__device__ __forceinline__ void pref_row_out(const PrefArgs &a, int row, bool counted, float za, float top, float sum) {
-    a.logp[row] = counted ? ((double)za - (double)top) - log((double)sum) : 0.0;
-    a.top[row] = top;
-    a.inv[row] = counted ? (float)(1.0 / (double)sum) : 0.0f;
-}
 
 template <typename T, int G, int K>
 __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
@@ -461,16 +505,16 @@ __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
     const bool can = act >= 0 && act < width && (!mask || mask[act]);
     const float za = can ? (float)z[act] : 0.0f;
     float top = NEG_INF, s = 0.0f;
-    if (K > 0) {
-        typename Row<T>::bytes b[K ? K : 1];
-        typename Row<T>::vec zc[K ? K : 1];
+    if constexpr (K > 0) {
+        typename Row<T>::bytes b[K];
+        typename Row<T>::vec zc[K];
 #pragma unroll
         for (int k = 0; k < K; k++) b[k] = legal_bytes<T>(mask, (lane + k * G) * V, width);
 #pragma unroll
         for (int k = 0; k < K; k++) load_chunk<T>(z, (lane + k * G) * V, width, b[k], zc[k]);
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            keep_legal<T>(b[k], zc[k]);
+            keep_legal<T>(mask, (lane + k * G) * V, width, b[k], zc[k]);
 #pragma unroll
             for (int j = 0; j < V; j++) top = fmaxf(top, (float)zc[k][j]);
         }
@@ -486,7 +530,7 @@ __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
             const typename Row<T>::bytes b = legal_bytes<T>(mask, (int)e0, width);
             typename Row<T>::vec zc;
             load_chunk<T>(z, (int)e0, width, b, zc);
-            keep_legal<T>(b, zc);
+            keep_legal<T>(mask, (int)e0, width, b, zc);
             float m = top;
             for (int j = 0; j < V; j++) m = fmaxf(m, (float)zc[j]);
             if (m > top) s *= exp_neg(top - m), top = m;
@@ -497,69 +541,100 @@ __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
         s = Group<G>::sum(top == NEG_INF ? s : s * exp_neg(top - all), red);
         top = all;
     }
-    if (lane == 0) pref_row_out(a, row, can && top > NEG_INF, za, top, s);
+    if (lane == 0) {
+        a.za[row] = za;
+        a.top[row] = top;
+        a.sum[row] = can && top > NEG_INF ? s : 0.0f;
+    }
 }
 
-// one wave per pair
+// One wave per pair, one row a lane: the lines' sums and the pair's loss, then what its rows' gradients need.
 __global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
     const long long p64 = row_block() * 4 + (threadIdx.x >> 6);
     const int p = (int)p64, lane = threadIdx.x & 63;
     if (p64 >= a.d.pairs) return;
+    const auto logp = [&](long long r) { return ((double)a.za[r] - (double)a.top[r]) - log64((double)a.sum[r]); };
     double s[2];
     for (int h = 0; h < 2; h++) {
         const int r1 = pref_offset(a, 2 * p + h + 1);
         double v = 0.0;
-        for (long long r = pref_offset(a, 2 * p + h) + lane; r < r1; r += 64) v += a.logp[r];
+        for (long long r = pref_offset(a, 2 * p + h) + lane; r < r1; r += 64)
+            if (a.sum[r] != 0.0f) v += logp(r);
         for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
         s[h] = v;
     }
-    if (lane) return;
     const double beta = a.d.beta, eps = a.d.smoothing, w = a.weights ? (double)a.weights[p] : 1.0;
     const double x = beta * ((s[0] - (double)a.ref[2 * p]) - (s[1] - (double)a.ref[2 * p + 1]));
-    const double soft = log1p(exp(-fabs(x)));  // -log sigmoid(x) = soft - min(x, 0)
-    a.pair_loss[p] = (float)(w * ((1.0 - eps) * (soft - fmin(x, 0.0)) + eps * (soft + fmax(x, 0.0))));
     // sigmoid(x) - (1 - eps), written so that nothing cancels for large x
-    a.slope[p] = (float)(w * beta * (eps - 1.0 / (1.0 + exp(x))));
-    if (a.line_logp) a.line_logp[2 * p] = (float)s[0], a.line_logp[2 * p + 1] = (float)s[1];
+    const double slope = w * beta * (eps - 1.0 / (1.0 + exp64(x)));
+    if (lane == 0) {
+        const double soft = log1p(exp64(-fabs(x)));  // -log sigmoid(x) = soft - min(x, 0)
+        a.pair_loss[p] = (float)(w * ((1.0 - eps) * (soft - fmin(x, 0.0)) + eps * (soft + fmax(x, 0.0))));
+        if (a.line_logp) a.line_logp[2 * p] = (float)s[0], a.line_logp[2 * p + 1] = (float)s[1];
+    }
+    if (!a.grad) return;
+    for (int h = 0; h < 2; h++) {
+        const double c = h ? -slope : slope;
+        const int r1 = pref_offset(a, 2 * p + h + 1);
+        for (long long r = pref_offset(a, 2 * p + h) + lane; r < r1; r += 64) {
+            const float sum = a.sum[r];
+            const bool counted = sum != 0.0f;
+            a.ce[r] = counted ? -(float)c * (1.0f / sum) : 0.0f;
+            a.taken[r] = counted ? (float)(c * (1.0 - exp64(logp(r)))) : 0.0f;
+        }
+    }
 }
 
-template <typename T, int G>
+template <typename T, int G, int K>
 __global__ __launch_bounds__(256) void pref_grad(PrefArgs a) {
     constexpr int V = Row<T>::V;
     const int lane = threadIdx.x % G;
     const long long row64 = row_block() * (256 / G) + threadIdx.x / G;
     if (row64 < pref_offset(a, 0) || row64 >= pref_offset(a, 2 * a.d.pairs)) return;
     const int row = (int)row64;
-    int lo = 0, hi = 2 * a.d.pairs;  // offsets[lo] <= row < offsets[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (pref_offset(a, mid) <= row)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    const float top = a.top[row], inv = a.inv[row];
-    const float ca = (lo & 1) ? -a.slope[lo >> 1] : a.slope[lo >> 1];
-    const bool counted = inv != 0.0f;
-    const int width = a.d.width;
+    const int width = a.d.width, act = a.actions[row];
     const T *z = (const T *)a.z + (size_t)row * a.d.ld;
     const uint8_t *mask = a.mask ? a.mask + (size_t)row * a.d.mask_ld : nullptr;
     T *grad = (T *)a.grad + (size_t)row * a.d.ld;
-    const RowGrad g{top, inv, ca, 0.0f, 0.0f};
-    for (long long e0 = (long long)lane * V; e0 < width; e0 += G * V) {
-        typename Row<T>::vec out = {};
-        if (counted) {
-            const typename Row<T>::bytes b = legal_bytes<T>(mask, (int)e0, width);
-            typename Row<T>::vec zc;
-            load_chunk<T>(z, (int)e0, width, b, zc);
-            keep_legal<T>(b, zc);
+    RowGrad g{a.top[row], a.ce[row], 0.0f, 0.0f, false};
+    g.plain = fabsf(g.ce) < __builtin_huge_valf();
+    const bool counted = a.sum[row] != 0.0f;
+    const float taken = a.taken[row];
+    const auto gradient = [&](int e0, typename Row<T>::bytes b, typename Row<T>::vec &zc) {
+        keep_legal<T>(mask, e0, width, b, zc);
+        float e[V];
 #pragma unroll
-            for (int j = 0; j < V; j++) out[j] = (T)row_grad<false>(exp_neg((float)zc[j] - top), 0.0f, 0.0f, g);
+        for (int j = 0; j < V; j++) e[j] = exp_neg((float)zc[j] - g.top);
+        store_chunk<T>(grad, e0, width, grad_chunk<T, false>(e, zc, zc, g));
+    };
+    const typename Row<T>::vec none = {};
+    if constexpr (K > 0) {
+        typename Row<T>::bytes b[K];
+        typename Row<T>::vec zc[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) b[k] = legal_bytes<T>(mask, (lane + k * G) * V, width);
+#pragma unroll
+        for (int k = 0; k < K; k++) load_chunk<T>(z, (lane + k * G) * V, width, b[k], zc[k]);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (counted)
+                gradient((lane + k * G) * V, b[k], zc[k]);
+            else
+                store_chunk<T>(grad, (lane + k * G) * V, width, none);
         }
-        store_chunk<T>(grad, (int)e0, width, out);
+    } else {
+        for (long long e0 = (long long)lane * V; e0 < width; e0 += G * V) {
+            if (counted) {
+                const typename Row<T>::bytes b = legal_bytes<T>(mask, (int)e0, width);
+                typename Row<T>::vec zc;
+                load_chunk<T>(z, (int)e0, width, b, zc);
+                gradient((int)e0, b, zc);
+            } else {
+                store_chunk<T>(grad, (int)e0, width, none);
+            }
+        }
     }
-    const int act = a.actions[row];
-    if (counted && lane == (act / V) % G) grad[act] = (T)((double)ca * (1.0 - exp(a.logp[row])));
+    if (counted && lane == (act / V) % G) grad[act] = (T)taken;
 }
 
 // ---- host side
@@ -614,12 +689,10 @@ int pref_launch(hipStream_t s, const PrefArgs &a) {
     BT_LAUNCH(BTK_POLICY, s, pref_pairs, row_grid(bt_div_up(a.d.pairs, 4)), dim3(256), 0, a);
     BT_LAUNCH_CHECK();
     if (a.grad && a.d.rows > 0) {
-        if (chunks <= 8)
-            BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 8>), row_grid(bt_div_up(a.d.rows, 32)), dim3(256), 0, a);
-        else if (chunks <= 512)
-            BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 64>), row_grid(bt_div_up(a.d.rows, 4)), dim3(256), 0, a);
-        else
-            BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 256>), row_grid(a.d.rows), dim3(256), 0, a);
+#define GRAD_CASE(G, K) BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, G, K>), row_grid(bt_div_up(a.d.rows, 256 / G)), dim3(256), 0, a);
+        ROW_SHAPES(GRAD_CASE)
+        else BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 256, 0>), row_grid(a.d.rows), dim3(256), 0, a);
+#undef GRAD_CASE
         BT_LAUNCH_CHECK();
     }
     return BT_OK;
@@ -669,7 +742,7 @@ int bt_policy_loss(void *stream, const bt_policy_desc *d, const void *logits, co
 
 size_t bt_preference_loss_workspace_bytes(const bt_preference_desc *d) {
     if (pref_validate(d, "bt_preference_loss_workspace_bytes", false)) return 0;
-    return bt_align((size_t)d->rows * 8) + 2 * bt_align((size_t)d->rows * 4) + bt_align((size_t)d->pairs * 4);
+    return 5 * bt_align((size_t)d->rows * 4) + 256;
 }
 
 int bt_preference_loss(void *stream, const bt_preference_desc *d, const void *logits, const uint8_t *mask,
@@ -680,16 +753,13 @@ int bt_preference_loss(void *stream, const bt_preference_desc *d, const void *lo
     BT_REQUIRE(offsets && ref_logp && loss_sum && pair_loss && workspace, "bt_preference_loss: null pointer");
     BT_REQUIRE(d->rows == 0 || (logits && actions), "bt_preference_loss: null pointer");
     BT_REQUIRE(workspace_bytes >= bt_preference_loss_workspace_bytes(d), "bt_preference_loss: workspace too small");
-    BT_REQUIRE(aligned(workspace, 8), "bt_preference_loss: workspace is not aligned to 8 bytes");
+    BT_REQUIRE(aligned(workspace, 4), "bt_preference_loss: workspace is not aligned to 4 bytes");
     const size_t es = type_size(d->type);
     BT_REQUIRE(aligned(logits, es) && aligned(grad, es), "bt_preference_loss: a buffer is not aligned to its element type");
-    char *ws = static_cast<char *>(workspace);
-    PrefArgs a{logits, mask, actions, offsets, ref_logp, pair_weights, grad, pair_loss, line_logp, nullptr, nullptr, nullptr,
-               nullptr, *d};
-    a.logp = reinterpret_cast<double *>(ws), ws += bt_align((size_t)d->rows * 8);
-    a.top = reinterpret_cast<float *>(ws), ws += bt_align((size_t)d->rows * 4);
-    a.inv = reinterpret_cast<float *>(ws), ws += bt_align((size_t)d->rows * 4);
-    a.slope = reinterpret_cast<float *>(ws);
+    const size_t per_row = bt_align((size_t)d->rows * 4) / sizeof(float);
+    float *ws = static_cast<float *>(workspace);
+    PrefArgs a{logits, mask, actions, offsets, ref_logp, pair_weights, grad, pair_loss, line_logp, ws, ws + per_row,
+               ws + 2 * per_row, ws + 3 * per_row, ws + 4 * per_row, *d};
     hipStream_t s = bt_stream(stream);
     if (int rc = d->type == BT_TYPE_F32    ? pref_launch<float>(s, a)
                  : d->type == BT_TYPE_BF16 ? pref_launch<__bf16>(s, a)

@@ -55,7 +55,7 @@ def preference(d, z=P, mask=P, actions=P, offsets=P, ref=P, w=P, loss=P, grad=P,
     (dict(smoothing=-0.1), {}, b"smoothing"), ({}, dict(z=None), b"null pointer"), ({}, dict(actions=None), b"null pointer"),
     ({}, dict(offsets=None), b"null pointer"), ({}, dict(ref=None), b"null pointer"), ({}, dict(loss=None), b"null pointer"),
     ({}, dict(pair_loss=None), b"null pointer"), ({}, dict(ws=None), b"null pointer"), ({}, dict(wsb=100), b"workspace too small"),
-    ({}, dict(ws=68), b"not aligned to 8 bytes"), ({}, dict(z=65), b"not aligned"), ({}, dict(grad=66), b"not aligned"),
+    ({}, dict(ws=66), b"not aligned to 4 bytes"), ({}, dict(z=65), b"not aligned"), ({}, dict(grad=66), b"not aligned"),
 ])
 def test_preference_loss_refuses(change, args, message):
     d = pr.preference_desc(4, 30, 10, "f32")
@@ -67,7 +67,7 @@ def test_preference_loss_refuses(change, args, message):
 
 def test_preference_workspace():
     d = pr.preference_desc(4, 30, 10, "f32")
-    assert L.bt_preference_loss_workspace_bytes(C.byref(d)) == 4 * 256
+    assert L.bt_preference_loss_workspace_bytes(C.byref(d)) == 6 * 256
     d.ld = 3
     assert L.bt_preference_loss_workspace_bytes(C.byref(d)) == 0 and b"leading dimension 3" in L.bt_last_error()
 
