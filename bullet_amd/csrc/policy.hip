@@ -139,11 +139,12 @@ template <typename B>
 __device__ __forceinline__ bool legal_at(B b, int j) {
     return (b >> (8 * j)) & 0xff;
 }
-// the chunk's elements that the mask leaves (a chunk it leaves empty is not read), -infinity elsewhere
+// the chunk that starts at element e0. (Not under the mask's control, although few moves are legal: waiting for the mask's
+// bytes costs more than the skipped chunks save, 112 us instead of 83 for 16384 x 1880 f32 with 35 legal moves a row.)
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T *row, int e0, int width, typename Row<T>::bytes b, typename Row<T>::vec &v) {
+__device__ __forceinline__ void load_chunk(const T *row, int e0, int width, typename Row<T>::vec &v) {
     constexpr int V = Row<T>::V;
-    if (b) {
+    if (e0 < width) {
         if (width - e0 >= V) {
             __builtin_memcpy(&v, row + e0, 16);
         } else {
@@ -310,8 +311,8 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
     for (int k = 0; k < K; k++) b[k] = legal_bytes<T>(mask, (lane + k * G) * V, width);
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        load_chunk<T>(z, (lane + k * G) * V, width, b[k], zc[k]);
-        if (FULL) load_chunk<T>(q, (lane + k * G) * V, width, b[k], qc[FULL ? k : 0]);
+        load_chunk<T>(z, (lane + k * G) * V, width, zc[k]);
+        if (FULL) load_chunk<T>(q, (lane + k * G) * V, width, qc[FULL ? k : 0]);
     }
     float top = NEG_INF, ref_top = NEG_INF;
 #pragma unroll
@@ -395,10 +396,10 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
     for (long long e0 = (long long)lane * V; e0 < width; e0 += 256 * V) {
         const bytes b = legal_bytes<T>(mask, (int)e0, width);
         vec zc, qc;
-        load_chunk<T>(z, (int)e0, width, b, zc);
+        load_chunk<T>(z, (int)e0, width, zc);
         keep_legal<T>(mask, (int)e0, width, b, zc);
         if (FULL) {
-            load_chunk<T>(q, (int)e0, width, b, qc);
+            load_chunk<T>(q, (int)e0, width, qc);
             keep_legal<T>(mask, (int)e0, width, b, qc);
         }
         float m = top, mq = ref_top;
@@ -445,10 +446,10 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
         if (counted) {
             const bytes b = legal_bytes<T>(mask, (int)e0, width);
             vec zc = {}, qc = {};
-            load_chunk<T>(z, (int)e0, width, b, zc);
+            load_chunk<T>(z, (int)e0, width, zc);
             keep_legal<T>(mask, (int)e0, width, b, zc);
             if (FULL) {
-                load_chunk<T>(q, (int)e0, width, b, qc);
+                load_chunk<T>(q, (int)e0, width, qc);
                 keep_legal<T>(mask, (int)e0, width, b, qc);
             }
             float e[V];
@@ -461,18 +462,31 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
     if (counted && lane == (act / V) % 256) grad[act] = (T)grad_taken;
 }
 
-// loss_sum = sum of the rows' losses, in 64 bits and a fixed order
-__global__ __launch_bounds__(1024) void loss_sum_kernel(const float *__restrict__ rows, int n, float *__restrict__ out) {
-    __shared__ double red[16];
+// loss_sum = sum of n losses, in 64 bits and a fixed order, by THREADS threads
+template <int THREADS>
+__device__ __forceinline__ void loss_sum(const float *rows, int n, float *out) {
+    __shared__ double red[THREADS / 64];
     double s = 0.0;
-    for (long long i = threadIdx.x; i < n; i += 1024) s += (double)rows[i];
+    const int tid = threadIdx.x;
+    long long i = tid;
+    for (; i + 7 * THREADS < n; i += 8 * THREADS) {  // eight loads in flight
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = rows[i + j * THREADS];
+#pragma unroll
+        for (int j = 0; j < 8; j++) s += (double)v[j];
+    }
+    for (; i < n; i += THREADS) s += (double)rows[i];
     for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if ((tid & 63) == 0) red[tid >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 16; i++) s += red[i];
+    if (tid == 0) {
+        for (int j = 1; j < THREADS / 64; j++) s += red[j];
         out[0] = (float)s;
     }
+}
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float *__restrict__ rows, int n, float *__restrict__ out) {
+    loss_sum<1024>(rows, n, out);
 }
 
 // ---- preference loss: row statistics -> pairs -> gradient rows
@@ -482,7 +496,7 @@ struct PrefArgs {
     const int32_t *actions, *offsets;
     const float *ref, *weights;
     void *grad;
-    float *pair_loss, *line_logp;
+    float *pair_loss, *line_logp, *loss_sum;
     // per row: logit of the action taken, the largest legal one, the sum of exp(z - top) (0: the row is not
     // counted), and what the pair kernel adds: the gradient's factor on p and the taken action's own gradient
     float *za, *top, *sum, *ce, *taken;
@@ -511,7 +525,7 @@ __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
 #pragma unroll
         for (int k = 0; k < K; k++) b[k] = legal_bytes<T>(mask, (lane + k * G) * V, width);
 #pragma unroll
-        for (int k = 0; k < K; k++) load_chunk<T>(z, (lane + k * G) * V, width, b[k], zc[k]);
+        for (int k = 0; k < K; k++) load_chunk<T>(z, (lane + k * G) * V, width, zc[k]);
 #pragma unroll
         for (int k = 0; k < K; k++) {
             keep_legal<T>(mask, (lane + k * G) * V, width, b[k], zc[k]);
@@ -529,7 +543,7 @@ __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
         for (long long e0 = (long long)lane * V; e0 < width; e0 += G * V) {
             const typename Row<T>::bytes b = legal_bytes<T>(mask, (int)e0, width);
             typename Row<T>::vec zc;
-            load_chunk<T>(z, (int)e0, width, b, zc);
+            load_chunk<T>(z, (int)e0, width, zc);
             keep_legal<T>(mask, (int)e0, width, b, zc);
             float m = top;
             for (int j = 0; j < V; j++) m = fmaxf(m, (float)zc[j]);
@@ -585,11 +599,17 @@ __global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
     }
 }
 
+// (the first workgroup adds the pairs' losses up, the others follow with the rows)
 template <typename T, int G, int K>
 __global__ __launch_bounds__(256) void pref_grad(PrefArgs a) {
     constexpr int V = Row<T>::V;
+    const long long block = row_block();
+    if (block == 0) {
+        loss_sum<256>(a.pair_loss, a.d.pairs, a.loss_sum);
+        return;
+    }
     const int lane = threadIdx.x % G;
-    const long long row64 = row_block() * (256 / G) + threadIdx.x / G;
+    const long long row64 = (block - 1) * (256 / G) + threadIdx.x / G;
     if (row64 < pref_offset(a, 0) || row64 >= pref_offset(a, 2 * a.d.pairs)) return;
     const int row = (int)row64;
     const int width = a.d.width, act = a.actions[row];
@@ -614,7 +634,7 @@ __global__ __launch_bounds__(256) void pref_grad(PrefArgs a) {
 #pragma unroll
         for (int k = 0; k < K; k++) b[k] = legal_bytes<T>(mask, (lane + k * G) * V, width);
 #pragma unroll
-        for (int k = 0; k < K; k++) load_chunk<T>(z, (lane + k * G) * V, width, b[k], zc[k]);
+        for (int k = 0; k < K; k++) load_chunk<T>(z, (lane + k * G) * V, width, zc[k]);
 #pragma unroll
         for (int k = 0; k < K; k++) {
             if (counted)
@@ -627,7 +647,7 @@ __global__ __launch_bounds__(256) void pref_grad(PrefArgs a) {
             if (counted) {
                 const typename Row<T>::bytes b = legal_bytes<T>(mask, (int)e0, width);
                 typename Row<T>::vec zc;
-                load_chunk<T>(z, (int)e0, width, b, zc);
+                load_chunk<T>(z, (int)e0, width, zc);
                 gradient((int)e0, b, zc);
             } else {
                 store_chunk<T>(grad, (int)e0, width, none);
@@ -689,12 +709,14 @@ int pref_launch(hipStream_t s, const PrefArgs &a) {
     BT_LAUNCH(BTK_POLICY, s, pref_pairs, row_grid(bt_div_up(a.d.pairs, 4)), dim3(256), 0, a);
     BT_LAUNCH_CHECK();
     if (a.grad && a.d.rows > 0) {
-#define GRAD_CASE(G, K) BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, G, K>), row_grid(bt_div_up(a.d.rows, 256 / G)), dim3(256), 0, a);
+#define GRAD_CASE(G, K) BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, G, K>), row_grid(1 + (long long)bt_div_up(a.d.rows, 256 / G)), dim3(256), 0, a);
         ROW_SHAPES(GRAD_CASE)
-        else BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 256, 0>), row_grid(a.d.rows), dim3(256), 0, a);
+        else BT_LAUNCH(BTK_POLICY, s, (pref_grad<T, 256, 0>), row_grid(1 + (long long)a.d.rows), dim3(256), 0, a);
 #undef GRAD_CASE
-        BT_LAUNCH_CHECK();
+    } else {
+        BT_LAUNCH(BTK_POLICY, s, loss_sum_kernel, dim3(1), dim3(1024), 0, a.pair_loss, a.d.pairs, a.loss_sum);
     }
+    BT_LAUNCH_CHECK();
     return BT_OK;
 }
 
@@ -758,15 +780,13 @@ int bt_preference_loss(void *stream, const bt_preference_desc *d, const void *lo
     BT_REQUIRE(aligned(logits, es) && aligned(grad, es), "bt_preference_loss: a buffer is not aligned to its element type");
     const size_t per_row = bt_align((size_t)d->rows * 4) / sizeof(float);
     float *ws = static_cast<float *>(workspace);
-    PrefArgs a{logits, mask, actions, offsets, ref_logp, pair_weights, grad, pair_loss, line_logp, ws, ws + per_row,
+    PrefArgs a{logits, mask, actions, offsets, ref_logp, pair_weights, grad, pair_loss, line_logp, loss_sum, ws, ws + per_row,
                ws + 2 * per_row, ws + 3 * per_row, ws + 4 * per_row, *d};
     hipStream_t s = bt_stream(stream);
     if (int rc = d->type == BT_TYPE_F32    ? pref_launch<float>(s, a)
                  : d->type == BT_TYPE_BF16 ? pref_launch<__bf16>(s, a)
                                            : pref_launch<_Float16>(s, a))
         return rc;
-    BT_LAUNCH(BTK_POLICY, s, loss_sum_kernel, dim3(1), dim3(1024), 0, pair_loss, d->pairs, loss_sum);
-    BT_LAUNCH_CHECK();
     return BT_OK;
 }
 
