@@ -303,8 +303,6 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
     const T *z = (const T *)a.z + (size_t)row * a.d.ld;
     const T *q = FULL ? (const T *)a.ref + (size_t)row * a.d.ld : nullptr;
     const uint8_t *mask = a.mask ? a.mask + (size_t)row * a.d.mask_ld : nullptr;
-    const PolicyRow pr = policy_row_begin(a, z, q, mask, row, FULL);
-
     bytes b[K];
     vec zc[K], qc[FULL ? K : 1];
 #pragma unroll
@@ -314,6 +312,7 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
         load_chunk<T>(z, (lane + k * G) * V, width, zc[k]);
         if (FULL) load_chunk<T>(q, (lane + k * G) * V, width, qc[FULL ? k : 0]);
     }
+    const PolicyRow pr = policy_row_begin(a, z, q, mask, row, FULL);  // (its three loads in turn: behind those of the row)
     float top = NEG_INF, ref_top = NEG_INF;
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -567,13 +566,28 @@ __global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
     const long long p64 = row_block() * 4 + (threadIdx.x >> 6);
     const int p = (int)p64, lane = threadIdx.x & 63;
     if (p64 >= a.d.pairs) return;
-    const auto logp = [&](long long r) { return ((double)a.za[r] - (double)a.top[r]) - log64((double)a.sum[r]); };
+    // a lane's first row of each line stays in registers (lines are seldom longer than a wave)
+    struct Entry {
+        float sum;
+        double logp;
+    };
+    const auto entry = [&](long long r) {
+        Entry e{a.sum[r], 0.0};
+        const double rel = (double)a.za[r] - (double)a.top[r];
+        if (e.sum != 0.0f) e.logp = rel - log64((double)e.sum);
+        return e;
+    };
+    int r0[2], r1[2];
+    Entry first[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) r0[h] = pref_offset(a, 2 * p + h) + lane, r1[h] = pref_offset(a, 2 * p + h + 1);
+#pragma unroll
+    for (int h = 0; h < 2; h++) first[h] = r0[h] < r1[h] ? entry(r0[h]) : Entry{0.0f, 0.0};
     double s[2];
+#pragma unroll
     for (int h = 0; h < 2; h++) {
-        const int r1 = pref_offset(a, 2 * p + h + 1);
-        double v = 0.0;
-        for (long long r = pref_offset(a, 2 * p + h) + lane; r < r1; r += 64)
-            if (a.sum[r] != 0.0f) v += logp(r);
+        double v = first[h].logp;
+        for (long long r = r0[h] + 64ll; r < r1[h]; r += 64) v += entry(r).logp;
         for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
         s[h] = v;
     }
@@ -587,15 +601,16 @@ __global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
         if (a.line_logp) a.line_logp[2 * p] = (float)s[0], a.line_logp[2 * p + 1] = (float)s[1];
     }
     if (!a.grad) return;
+#pragma unroll
     for (int h = 0; h < 2; h++) {
         const double c = h ? -slope : slope;
-        const int r1 = pref_offset(a, 2 * p + h + 1);
-        for (long long r = pref_offset(a, 2 * p + h) + lane; r < r1; r += 64) {
-            const float sum = a.sum[r];
-            const bool counted = sum != 0.0f;
-            a.ce[r] = counted ? -(float)c * (1.0f / sum) : 0.0f;
-            a.taken[r] = counted ? (float)(c * (1.0 - exp64(logp(r)))) : 0.0f;
-        }
+        const auto put = [&](long long r, const Entry &e) {
+            const bool counted = e.sum != 0.0f;
+            a.ce[r] = counted ? -(float)c * (1.0f / e.sum) : 0.0f;
+            a.taken[r] = counted ? (float)(c * (1.0 - exp64(e.logp))) : 0.0f;
+        };
+        if (r0[h] < r1[h]) put(r0[h], first[h]);
+        for (long long r = r0[h] + 64ll; r < r1[h]; r += 64) put(r, entry(r));
     }
 }
 
