@@ -99,29 +99,37 @@ struct Tile {
 
 // An operand in memory: `rows` rows of `len` contiguous elements, `ld` apart.
 struct Operand {
-    const void *p[3];  // the summands that a 16-bit gradient may be kept as, or the same matrix three times
+    const void *p0, *p1, *p2;  // the summands that a 16-bit gradient may be kept as, or the same matrix three times
     long long ld;
     int rows, len;
     int aligned;  // every chunk of every row starts on 16 bytes
+    // the pointers in registers of their own: a choice between them must not become a choice of where to load one from
+    // (that puts the kernel's arguments into scratch memory)
+    __device__ __forceinline__ Operand pinned() const {
+        Operand o = *this;
+        asm("" : "+s"(o.p0), "+s"(o.p1), "+s"(o.p2));
+        return o;
+    }
+    __device__ __forceinline__ const void *summand(int i) const { return i == 0 ? p0 : i == 1 ? p1 : p2; }
 };
 
 // chunk (row, element e) of the matrix, zeros outside it
 template <typename T>
 __device__ __forceinline__ v4u load_chunk(const T *base, const Operand &o, int row, long long e) {
     constexpr int V = Elem<T>::V;
-    v4u r = {0, 0, 0, 0};
-    if (row >= o.rows || e >= o.len) return r;
-    const T *p = base + (size_t)row * o.ld + e;
-    if (o.len - e >= V) {
-        __builtin_memcpy(&r, p, 16);
-    } else {
-        typename Elem<T>::frag t = {};
+    typedef typename Elem<T>::frag frag __attribute__((aligned(sizeof(T))));
+    typename Elem<T>::frag r = {};
+    if (row < o.rows && e < o.len) {
+        const auto *p = (const __attribute__((address_space(1))) T *)base + ((size_t)row * o.ld + e);
+        if (o.len - e >= V) {
+            r = *(const __attribute__((address_space(1))) frag *)p;
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; j++)
-            if (j < o.len - e) t[j] = p[j];
-        r = __builtin_bit_cast(v4u, t);
+            for (int j = 0; j < V; j++)
+                if (j < o.len - e) r[j] = p[j];
+        }
     }
-    return r;
+    return __builtin_bit_cast(v4u, r);
 }
 
 enum { OUT_LAYER = 0, OUT_TYPE = 1, OUT_F32 = 2, OUT_PART = 3 };
@@ -148,9 +156,25 @@ __device__ __forceinline__ void store4(T *p, v4f v, int n) {  // the first n of 
             if (j < n) p[j] = q[j];
     }
 }
-// what becomes of 4 sums of one row, columns c .. c + 3 (n of them inside the matrix)
+// the residual under 4 sums of one row, columns c .. c + 3 (n of them inside the matrix); zeros without one
 template <typename T, int OUT>
-__device__ __forceinline__ void finish4(const Epilogue &e, int row, int c, int n, v4f v) {
+__device__ __forceinline__ typename Elem<T>::quad residual4(const Epilogue &e, int row, int c, int n) {
+    typename Elem<T>::quad q = {};
+    if (OUT == OUT_LAYER && e.residual) {
+        const T *r = (const T *)e.residual + ((size_t)row * e.ld + c);
+        if (n >= 4) {
+            __builtin_memcpy(&q, r, sizeof(q));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (j < n) q[j] = r[j];
+        }
+    }
+    return q;
+}
+// what becomes of those sums
+template <typename T, int OUT>
+__device__ __forceinline__ void finish4(const Epilogue &e, int row, int c, int n, v4f v, typename Elem<T>::quad residual) {
     const size_t at = (size_t)row * e.ld + c;
     if constexpr (OUT == OUT_F32) {
         store4<float>((float *)e.out + at, v * e.alpha, n);
@@ -178,23 +202,39 @@ __device__ __forceinline__ void finish4(const Epilogue &e, int row, int c, int n
         }
         if (e.saved) store4<T>((T *)e.saved + at, v, n);
         if (e.residual) {
-            const T *r = (const T *)e.residual + at;
-            if (n >= 4) {
-                typename Elem<T>::quad q;
-                __builtin_memcpy(&q, r, sizeof(q));
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[j] += (float)q[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (j < n) v[j] += (float)r[j];
-            }
+            for (int j = 0; j < 4; j++) v[j] += (float)residual[j];
         }
         store4<T>((T *)e.out + at, v, n);
     }
 }
 
 constexpr float F16_LIFT = 2048.0f;  // between the two summands of an f16 gradient (affine_gz)
+
+// dbias from the row ranges' sums that affine_prepare leaves, by workgroups of their own behind a product's
+struct BiasSum {
+    const float *part;  // [parts][n]
+    float *out;
+    int parts, n, blocks;
+    float alpha;
+};
+constexpr int BIAS_COLS = 32;
+template <int NT>
+__device__ __forceinline__ void bias_sum(const BiasSum b, int block, float *lds) {  // lds: NT floats
+    const int c = threadIdx.x % BIAS_COLS, r = threadIdx.x / BIAS_COLS, col = block * BIAS_COLS + c;
+    float s = 0.0f;
+    if (col < b.n)
+        for (int p = r; p < b.parts; p += NT / BIAS_COLS) s += b.part[(size_t)p * b.n + col];
+    lds[threadIdx.x] = s;
+    __syncthreads();
+    if (r || col >= b.n) return;
+    for (int q = 1; q < NT / BIAS_COLS; q++) s += lds[q * BIAS_COLS + c];
+    b.out[col] = s * b.alpha;
+}
+__global__ __launch_bounds__(256) void affine_dbias(BiasSum b) {
+    __shared__ float lds[256];
+    bias_sum<256>(b, blockIdx.x, lds);
+}
 
 struct Product {
     Operand a, b;
@@ -207,6 +247,7 @@ struct Product {
     float *part;         // [splits][m][part_ld]
     long long part_ld;
     Epilogue e;
+    BiasSum bias;
 };
 
 // A chunk straight from memory into LDS, 16 bytes a lane: lane l's lands 16 l bytes behind `lds` (the same in all lanes).
@@ -228,7 +269,7 @@ struct Stage {
     // chunk of slot s of the tile at (s0, k0), zeros where the matrix has nothing
     static __device__ __forceinline__ v4u chunk(const Operand &o, int pass, int s0, int k0, int s) {
         const int row = s / L::CPR, c = L::swizzle(row, s % L::CPR);
-        return load_chunk<T>((const T *)o.p[pass], o, (KC ? s0 : k0) + row, (long long)(KC ? k0 : s0) + c * V);
+        return load_chunk<T>((const T *)o.summand(pass), o, (KC ? s0 : k0) + row, (long long)(KC ? k0 : s0) + c * V);
     }
     static __device__ __forceinline__ void get(const Operand &o, int pass, int s0, int k0, int tid, v4u (&r)[N]) {
 #pragma unroll
@@ -268,7 +309,7 @@ struct Stage {
         }
     }
     static __device__ __forceinline__ const char *first(const Operand &o, int pass, int s0, int k0) {
-        return (const char *)o.p[pass] + ((KC ? s0 : k0) * (size_t)o.ld + (KC ? k0 : s0)) * sizeof(T);
+        return (const char *)o.summand(pass) + ((KC ? s0 : k0) * (size_t)o.ld + (KC ? k0 : s0)) * sizeof(T);
     }
     static __device__ __forceinline__ size_t step(const Operand &o) { return KC ? 128 : (size_t)o.ld * sizeof(T) * BK; }
 };
@@ -295,17 +336,18 @@ struct Mm {
     static constexpr int BYTES = TA::BYTES + TB::BYTES;  // of one of the two buffers
     typedef typename Elem<T>::frag frag;
     const Product &P;
+    const Operand a, b;
     char *lds;
     int tid, lane, wm, wn, split, m0, n0;
     uint32_t at_a, at_b;  // where this lane reads a tile of the first buffer
     v4f acc[FN][FM];
 
-    __device__ __forceinline__ Mm(const Product &P_, char *lds_) : P(P_), lds(lds_) {
+    __device__ __forceinline__ Mm(const Product &P_, char *lds_) : P(P_), a(P_.a.pinned()), b(P_.b.pinned()), lds(lds_) {
         tid = threadIdx.x, lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         wm = wave / WN, wn = wave % WN;
         int tm, tn;
-        tile_of(blockIdx.x, gridDim.x, P.tiles_m, P.tiles_n, split, tm, tn);
+        tile_of(blockIdx.x, gridDim.x - P.bias.blocks, P.tiles_m, P.tiles_n, split, tm, tn);
         m0 = tm * BM, n0 = tn * BN;
         at_a = lds_address(lds) + TA::origin(wm * FM, lane), at_b = lds_address(lds) + TA::BYTES + TB::origin(wn * FN, lane);
 #pragma unroll
@@ -344,20 +386,35 @@ struct Mm {
         __syncthreads();
         float *strip = (float *)lds + (wm * WN + wn) * 16 * STRIDE;
         const int n = n0 + wn * COLS + (lane % LANES) * 4;
+        // the residual's loads go ahead of everything, as far as registers allow: in turn with the stores (which may go to
+        // the same buffer) each would wait for memory
+        constexpr int PASSES = 16 / ROWS, AHEAD = FM <= 4 ? FM : 1;
+        typename Elem<T>::quad res[AHEAD][PASSES];
+        const auto ahead = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) {
+                const int m = m0 + (wm * FM + j) * 16 + i * ROWS + lane / LANES;
+                if (m < P.m && n < P.n) res[j % AHEAD][i] = residual4<T, OUT>(P.e, m, n, P.n - n);
+            }
+        };
+        if (AHEAD > 1)
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) ahead(j);
 #pragma unroll
         for (int j = 0; j < FM; j++) {
+            if (AHEAD == 1) ahead(j);
 #pragma unroll
             for (int i = 0; i < FN; i++) *(v4f *)(strip + (lane & 15) * STRIDE + i * 16 + (lane >> 4) * 4) = acc[i][j];
             __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-            for (int r = lane / LANES; r < 16; r += ROWS) {
-                const int m = m0 + (wm * FM + j) * 16 + r;
+#pragma unroll
+            for (int i = 0; i < PASSES; i++) {
+                const int r = i * ROWS + lane / LANES, m = m0 + (wm * FM + j) * 16 + r;
                 const v4f v = *(const v4f *)(strip + r * STRIDE + (lane % LANES) * 4);
                 if (m >= P.m || n >= P.n) continue;
                 if constexpr (OUT == OUT_PART)
                     *(v4f *)(P.part + ((size_t)split * P.m + m) * P.part_ld + n) = v;  // (part_ld: a multiple of 4)
                 else
-                    finish4<T, OUT>(P.e, m, n, P.n - n, v);
+                    finish4<T, OUT>(P.e, m, n, P.n - n, v, res[j % AHEAD][i]);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -369,6 +426,8 @@ template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT
 __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
     typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
     extern __shared__ __align__(1024) char lds[];
+    if (blockIdx.x >= gridDim.x - P.bias.blocks)
+        return bias_sum<M::NT>(P.bias, blockIdx.x - (gridDim.x - P.bias.blocks), (float *)lds);
     M mm(P, lds);
     const int ktiles = (P.k + M::BK - 1) / M::BK;
     int p0, p1, t0, t1;
@@ -376,8 +435,8 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
     v4u ra[M::SA::N], rb[M::SB::N];
     auto get = [&](int kt) {
         const int pass = kt / ktiles, k0 = (kt - pass * ktiles) * M::BK;
-        M::SA::get(P.a, p0 + pass, mm.m0, k0, mm.tid, ra);
-        M::SB::get(P.b, p0 + pass, mm.n0, k0, mm.tid, rb);
+        M::SA::get(mm.a, p0 + pass, mm.m0, k0, mm.tid, ra);
+        M::SB::get(mm.b, p0 + pass, mm.n0, k0, mm.tid, rb);
     };
     if (t0 < t1) get(t0);
     for (int kt = t0; kt < t1; kt++) {
@@ -403,21 +462,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     typedef typename M::frag frag;
     constexpr int FM = M::FM, FN = M::FN, NA = M::SA::N, NB = M::SB::N;
     extern __shared__ __align__(1024) char lds[];
+    if (blockIdx.x >= gridDim.x - P.bias.blocks)
+        return bias_sum<M::NT>(P.bias, blockIdx.x - (gridDim.x - P.bias.blocks), (float *)lds);
     M mm(P, lds);
-    const bool inside = M::SA::inside(P.a, mm.m0) && M::SB::inside(P.b, mm.n0);
+    const bool inside = M::SA::inside(mm.a, mm.m0) && M::SB::inside(mm.b, mm.n0);
     const int ktiles = (P.k + M::BK - 1) / M::BK, full = P.k / M::BK;
     int p0, p1, t0, t1;
     const bool last = mm.share(inside ? full : ktiles, p0, p1, t0, t1);
     const int quick = inside ? t1 - t0 : 0, tiles = !inside ? t1 - t0 : quick + (last && full < ktiles ? p1 - p0 : 0);
 
     uint32_t oa[NA], ob[NB];
-    M::SA::offsets(P.a, mm.m0, mm.tid, oa);
-    M::SB::offsets(P.b, mm.n0, mm.tid, ob);
+    M::SA::offsets(mm.a, mm.m0, mm.tid, oa);
+    M::SB::offsets(mm.b, mm.n0, mm.tid, ob);
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (mm.tid & ~63) * 16);
     // the filled tile to be sent for next: its summand, its number in there, its first elements
     int pass = p0, at = 0;
     if (quick) pass += t0 / full, at = t0 % full;
-    const char *pa = M::SA::first(P.a, pass, mm.m0, at * M::BK), *pb = M::SB::first(P.b, pass, mm.n0, at * M::BK);
+    const char *pa = M::SA::first(mm.a, pass, mm.m0, at * M::BK), *pb = M::SB::first(mm.b, pass, mm.n0, at * M::BK);
     const size_t step_a = M::SA::step(P.a), step_b = M::SB::step(P.b);
     const auto send = [&](int q, int buf) {  // chunk q of both operands' NA + NB
         if (q < NA)
@@ -429,14 +490,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
         pa += step_a, pb += step_b;
         if (++at == full) {
             at = 0, pass = min(pass + 1, p1 - 1);
-            pa = M::SA::first(P.a, pass, mm.m0, 0), pb = M::SB::first(P.b, pass, mm.n0, 0);
+            pa = M::SA::first(mm.a, pass, mm.m0, 0), pb = M::SB::first(mm.b, pass, mm.n0, 0);
         }
     };
     const auto careful = [&](int tile, int buf) {
         const int c = inside ? tile - quick : t0 + tile;
         const int ps = p0 + (inside ? c : c / ktiles), k0 = (inside ? full : c % ktiles) * M::BK;
-        M::SA::careful(P.a, ps, mm.m0, k0, mm.tid, lds + buf * M::BYTES);
-        M::SB::careful(P.b, ps, mm.n0, k0, mm.tid, lds + buf * M::BYTES + M::TA::BYTES);
+        M::SA::careful(mm.a, ps, mm.m0, k0, mm.tid, lds + buf * M::BYTES);
+        M::SB::careful(mm.b, ps, mm.n0, k0, mm.tid, lds + buf * M::BYTES + M::TA::BYTES);
     };
     frag fa[FM], fb[2][FN];
     // The products of half 1 - s, and beside them: fragments of half s of the tile in buffer `buf` (of m: into the registers
@@ -509,33 +570,144 @@ __global__ __launch_bounds__(256) void affine_join(Product P) {
         if (P.lift && s == P.splits / 2) v *= 1.0f / F16_LIFT;
         v += *(const v4f *)(P.part + ((size_t)s * P.m + m) * P.part_ld + n);
     }
-    finish4<T, OUT>(P.e, m, n, P.n - n, v);
+    finish4<T, OUT>(P.e, m, n, P.n - n, v, residual4<T, OUT>(P.e, m, n, P.n - n));
 }
 
-// A matrix with rows on 16 bytes (and f32 weights rounded to the layer's type) for the direct loads: `to_ld` is `len` up to
-// a whole chunk, filled with zeros. One chunk a thread.
+// What a product needs made before it, in one launch: copies of matrices, and gz.
+//
+// A copy has rows on 128 bytes (so that a tile's row of k is one line of memory), of the layer's type (f32 weights are
+// rounded), with zeros up to a whole chunk. One chunk a thread.
+template <typename T>
+struct Copy {
+    const void *from;
+    T *to;
+    long long from_ld, to_ld;
+    int rows, len, f32, blocks;
+};
 template <typename From, typename T>
-__global__ __launch_bounds__(256) void affine_copy(const From *__restrict__ from, long long from_ld, T *__restrict__ to,
-                                                   long long to_ld, int rows, int len) {
+__device__ __forceinline__ void copy_chunk(const From *p, int left, T *to) {
     constexpr int V = Elem<T>::V;
-    const long long q = (long long)blockIdx.x * 256 + threadIdx.x, cols = to_ld / V;
-    if (q >= cols * rows) return;
-    const long long row = q / cols;
-    const int c = (int)(q % cols) * V;
-    const From *p = from + row * from_ld + c;
     typedef From vec __attribute__((ext_vector_type(V)));
     vec v = {};
-    if (len - c >= V) {
+    if (left >= V) {
         __builtin_memcpy(&v, p, sizeof(v));
     } else {
 #pragma unroll
         for (int j = 0; j < V; j++)
-            if (j < len - c) v[j] = p[j];
+            if (j < left) v[j] = p[j];
     }
     typename Elem<T>::frag r;
 #pragma unroll
     for (int j = 0; j < V; j++) r[j] = (T)(float)v[j];
-    *(typename Elem<T>::frag *)(to + row * to_ld + c) = r;
+    *(typename Elem<T>::frag *)to = r;
+}
+template <typename T>
+__device__ __forceinline__ void copy_block(const Copy<T> &c, long long block) {
+    constexpr int V = Elem<T>::V;
+    const long long q = block * 256 + threadIdx.x, cols = (c.len + V - 1) / V;
+    if (q >= cols * c.rows) return;
+    const long long row = q / cols;
+    const int e = (int)(q % cols) * V;
+    T *to = c.to + row * c.to_ld + e;
+    if (c.f32)
+        copy_chunk<float, T>((const float *)c.from + row * c.from_ld + e, c.len - e, to);
+    else
+        copy_chunk<T, T>((const T *)c.from + row * c.from_ld + e, c.len - e, to);
+}
+
+// gz = grad_y act'(out) (half of it where act' carries a factor 2: the products' alpha gives it back, exactly), as one
+// number of the layer's type or, NP > 1, as a sum: each further summand takes what the rounding of those before left over
+// (two of f16: 22 bits, the second one times 2^11 so that it stays clear of the subnormals; three of bf16: 24 bits, two
+// where the product is rounded to bf16 anyway). And the column sums of gz over this workgroup's rows.
+// Thread (c, r) takes column chunk c and every 8th row from r on.
+constexpr int GZ_COLS = 32, GZ_ROWS = 8;
+template <typename T>
+struct Gz {
+    const T *gy, *out;  // out: null = no derivative
+    T *p[3];            // summands, largest first; null = sums only
+    float *sums;        // [ranges][n], or null
+    long long ld, gz_ld;
+    int batch, n, act, range, col_blocks, blocks;
+};
+template <typename T, int NP>
+__device__ __forceinline__ void gz_block(const Gz<T> &G, int block) {
+    constexpr int V = Elem<T>::V;
+    constexpr float LIFT = std::is_same<T, _Float16>::value ? F16_LIFT : 1.0f;
+    typedef typename Elem<T>::frag frag;
+    __shared__ float red[GZ_ROWS][GZ_COLS * V];
+    const int bx = block % G.col_blocks, by = block / G.col_blocks;
+    const int c = threadIdx.x % GZ_COLS, r = threadIdx.x / GZ_COLS;
+    const long long e = ((long long)bx * GZ_COLS + c) * V;
+    const long long b0 = (long long)by * G.range, b1 = b0 + G.range < G.batch ? b0 + G.range : G.batch;
+    const int left = e < G.n ? (int)(G.n - e < V ? G.n - e : V) : 0;
+    const bool root = G.act == BT_ACT_SCRELU || G.act == BT_ACT_SQRRELU;
+    const float top = G.act == BT_ACT_CRELU || G.act == BT_ACT_SCRELU ? 1.0f : __builtin_huge_valf();
+    float sum[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) sum[j] = 0.0f;
+    if (left)
+        for (long long b = b0 + r; b < b1; b += GZ_ROWS) {
+            frag g = {}, o = {}, part[NP];
+            const T *pg = G.gy + b * G.ld + e, *po = G.out ? G.out + b * G.ld + e : nullptr;
+            if (left == V) {
+                __builtin_memcpy(&g, pg, 16);
+                if (po) __builtin_memcpy(&o, po, 16);
+            } else {
+                for (int j = 0; j < V; j++)
+                    if (j < left) {
+                        g[j] = pg[j];
+                        if (po) o[j] = po[j];
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                // bt_act_deriv, halved where it has a factor 2, without its branches (for every output an activation has)
+                const float a = (float)o[j];
+                float slope = a > 0.0f && a < top ? 1.0f : 0.0f;
+                if (root) slope *= __builtin_amdgcn_sqrtf(a);
+                const float v = po ? (float)g[j] * slope : (float)g[j];
+                sum[j] += v;
+                float rest = v;
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    part[p][j] = (T)rest;
+                    rest = (rest - (float)part[p][j]) * LIFT;
+                    if (rest != rest) rest = 0.0f;  // (an infinite gradient stays one)
+                }
+            }
+            if (G.p[0]) {
+#pragma unroll
+                for (int p = 0; p < NP; p++)  // (gz_ld is a multiple of V: a last chunk is whole)
+                    __builtin_memcpy(G.p[p] + b * G.gz_ld + e, &part[p], 16);
+            }
+        }
+    if (!G.sums) return;
+#pragma unroll
+    for (int j = 0; j < V; j++) red[r][c * V + j] = sum[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < GZ_COLS * V; i += 256) {
+        const long long col = (long long)bx * GZ_COLS * V + i;
+        if (col >= G.n) continue;
+        float s = 0.0f;
+        for (int q = 0; q < GZ_ROWS; q++) s += red[q][i];
+        G.sums[(size_t)by * G.n + col] = s;
+    }
+}
+
+template <typename T>
+struct Prepare {
+    Copy<T> w, x;
+    Gz<T> gz;
+};
+template <typename T, int NP>  // NP = 0: copies only
+__global__ __launch_bounds__(256) void affine_prepare(Prepare<T> p) {
+    long long block = blockIdx.x;
+    if constexpr (NP > 0) {
+        if (block < p.gz.blocks) return gz_block<T, NP>(p.gz, (int)block);
+        block -= p.gz.blocks;
+    }
+    if (block < p.w.blocks) return copy_block<T>(p.w, block);
+    copy_block<T>(p.x, block - p.w.blocks);
 }
 
 // Forward of at most R rows (one position, or a few): the weights are all there is to read, and each is used R times, so
@@ -613,93 +785,7 @@ __global__ __launch_bounds__(1024) void affine_few(const TW *__restrict__ w, lon
     if (r >= batch || col >= out) return;
     v4f v = {0, 0, 0, 0};
     for (int i = 0; i < 16; i++) v += *(const v4f *)&red[i][r][q];
-    finish4<T, OUT_LAYER>(e, r, col, out - col, v);
-}
-
-// gz = grad_y act'(out) (half of it where act' carries a factor 2: the products' alpha gives it back, exactly), as one
-// number of the layer's type or, NP > 1, as a sum: each further summand takes what the rounding of those before left over
-// (two of f16: 22 bits, the second one times 2^11 so that it stays clear of the subnormals; three of bf16: 24 bits, two
-// where the product is rounded to bf16 anyway). And the column sums of gz over this workgroup's rows.
-// Thread (c, r) takes column chunk c and every 8th row from r on.
-constexpr int GZ_COLS = 32, GZ_ROWS = 8;
-template <typename T>
-struct Summands {
-    T *p[3];  // largest first
-};
-template <typename T, int NP>
-__global__ __launch_bounds__(256) void affine_gz(const T *__restrict__ gy, const T *__restrict__ out, long long ld, Summands<T> gz,
-                                                 long long gz_ld, float *__restrict__ part, int batch, int n, int act, int range) {
-    constexpr int V = Elem<T>::V;
-    constexpr float LIFT = std::is_same<T, _Float16>::value ? F16_LIFT : 1.0f;
-    typedef typename Elem<T>::frag frag;
-    __shared__ float red[GZ_ROWS][GZ_COLS * V];
-    const int c = threadIdx.x % GZ_COLS, r = threadIdx.x / GZ_COLS;
-    const long long e = ((long long)blockIdx.x * GZ_COLS + c) * V;
-    const long long b0 = (long long)blockIdx.y * range, b1 = b0 + range < batch ? b0 + range : batch;
-    const int left = e < n ? (int)(n - e < V ? n - e : V) : 0;
-    const float half = act == BT_ACT_SCRELU || act == BT_ACT_SQRRELU ? 0.5f : 1.0f;
-    float sum[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) sum[j] = 0.0f;
-    if (left)
-        for (long long b = b0 + r; b < b1; b += GZ_ROWS) {
-            frag g = {}, o = {}, part_of[NP];
-            const T *pg = gy + b * ld + e, *po = out ? out + b * ld + e : nullptr;
-            if (left == V) {
-                __builtin_memcpy(&g, pg, 16);
-                if (out) __builtin_memcpy(&o, po, 16);
-            } else {
-                for (int j = 0; j < V; j++)
-                    if (j < left) {
-                        g[j] = pg[j];
-                        if (out) o[j] = po[j];
-                    }
-            }
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float v = out ? (float)g[j] * (bt_act_deriv(act, (float)o[j]) * half) : (float)g[j];
-                sum[j] += v;
-                float rest = v;
-#pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    part_of[p][j] = (T)rest;
-                    rest = (rest - (float)part_of[p][j]) * LIFT;
-                    if (rest != rest) rest = 0.0f;  // (an infinite gradient stays one)
-                }
-            }
-            if (gz.p[0]) {
-#pragma unroll
-                for (int p = 0; p < NP; p++)  // (gz_ld is a multiple of V: a last chunk is whole)
-                    __builtin_memcpy(gz.p[p] + b * gz_ld + e, &part_of[p], 16);
-            }
-        }
-    if (!part) return;
-#pragma unroll
-    for (int j = 0; j < V; j++) red[r][c * V + j] = sum[j];
-    __syncthreads();
-    for (int i = threadIdx.x; i < GZ_COLS * V; i += 256) {
-        const long long col = (long long)blockIdx.x * GZ_COLS * V + i;
-        if (col >= n) continue;
-        float s = 0.0f;
-        for (int q = 0; q < GZ_ROWS; q++) s += red[q][i];
-        part[(size_t)blockIdx.y * n + col] = s;
-    }
-}
-
-// dbias: the row ranges' sums, 16 threads a column, in a fixed order
-__global__ __launch_bounds__(1024) void affine_dbias(const float *__restrict__ part, int parts, int n, float alpha,
-                                                     float *__restrict__ dbias) {
-    __shared__ float red[16][64];
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-    const long long col = (long long)blockIdx.x * 64 + c;
-    float s = 0.0f;
-    if (col < n)
-        for (int p = r; p < parts; p += 16) s += part[(size_t)p * n + col];
-    red[r][c] = s;
-    __syncthreads();
-    if (r || col >= n) return;
-    for (int q = 1; q < 16; q++) s += red[q][c];
-    dbias[col] = s * alpha;
+    finish4<T, OUT_LAYER>(e, r, col, out - col, v, residual4<T, OUT_LAYER>(e, r, col, out - col));
 }
 
 // ---- host side
@@ -762,7 +848,7 @@ int mm_launch(hipStream_t st, const Product &P, bool direct) {
     const long long blocks = (long long)P.tiles_m * P.tiles_n * P.splits;
     BT_REQUIRE(blocks < (1 << 22), "bt_affine: Mismatched sizes! (%lld tiles)", blocks);
     const size_t lds = 2 * Mm<T, BM, BN, WM, WN, AK, BKC, OUT>::BYTES;
-    const dim3 grid((unsigned)blocks), block(64 * WM * WN);
+    const dim3 grid((unsigned)(blocks + P.bias.blocks)), block(64 * WM * WN);
     if (direct) {
         const auto kernel = affine_mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT>;
         if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
@@ -795,12 +881,16 @@ int product_launch(hipStream_t st, Product &P, Shape s) {
     return BT_OK;
 }
 
-long long padded(int n, size_t es) { return (n + (16 / es) - 1) / (16 / es) * (16 / es); }
+long long padded(int n, size_t es) { return (n + (128 / es) - 1) / (128 / es) * (128 / es); }  // rows on 128 bytes
+int whole_chunks(int n, size_t es) { return (int)((n + (16 / es) - 1) / (16 / es) * (16 / es)); }
 // direct loads need rows on 16 bytes, and reach those of one tile through 32-bit offsets
 bool direct_ld(long long ld, size_t es) { return ld * es % 16 == 0 && ld < (1 << 21); }
 Operand matrix(const void *p, long long ld, int rows, int len, size_t es) {
-    return Operand{{p, p, p}, ld, rows, len, (reinterpret_cast<uintptr_t>(p) & 15) == 0 && direct_ld(ld, es)};
+    return Operand{p, p, p, ld, rows, len, (reinterpret_cast<uintptr_t>(p) & 15) == 0 && direct_ld(ld, es)};
 }
+// one of the workspace's: the zeros behind a row are part of it
+Operand own_matrix(const void *p, int rows, int len, size_t es) { return matrix(p, padded(len, es), rows, whole_chunks(len, es), es); }
+
 // Matrices that are copied into the workspace first: those whose rows do not start on 16 bytes (read through registers
 // instead, 1537 x 1027 -> 1881 f16 takes 34 us, copied 22), and f32 weights of a 16-bit layer. One whose first element alone is
 // off is read through registers.
@@ -808,26 +898,43 @@ size_t copy_bytes(bool copy, int rows, int len, size_t es) { return copy ? bt_al
 bool copy_w(const bt_affine_desc *d) { return d->w_type != d->type || !direct_ld(d->w_ld, type_size(d->type)); }
 bool copy_x(const bt_affine_desc *d) { return !direct_ld(d->x_ld, type_size(d->type)); }
 
-template <typename From, typename T>
-int copy_launch(hipStream_t st, const void *from, long long ld, void *to, int rows, int len, Operand &o) {
-    const long long to_ld = padded(len, sizeof(T)), chunks = to_ld / Elem<T>::V * rows;
-    BT_LAUNCH(BTK_AFFINE, st, (affine_copy<From, T>), dim3(bt_div_up(chunks, 256)), dim3(256), 0, (const From *)from, ld, (T *)to,
-              to_ld, rows, len);
+template <typename T>
+Copy<T> copy_of(const void *from, long long ld, bool f32, void *to, int rows, int len) {
+    Copy<T> c{from, (T *)to, ld, padded(len, sizeof(T)), rows, len, f32, 0};
+    c.blocks = bt_div_up((long long)whole_chunks(len, sizeof(T)) / Elem<T>::V * rows, 256);
+    return c;
+}
+// w / x as the products take them; adds the copy, if there is one, to `p`
+template <typename T>
+Operand weights(const bt_affine_desc *d, const void *w, void *ws, Prepare<T> &p) {
+    if (!copy_w(d)) return matrix(w, d->w_ld, d->in, d->out, sizeof(T));
+    p.w = copy_of<T>(w, d->w_ld, d->w_type != d->type, ws, d->in, d->out);
+    return own_matrix(ws, d->in, d->out, sizeof(T));
+}
+template <typename T>
+Operand inputs(const bt_affine_desc *d, const void *x, void *ws, Prepare<T> &p) {
+    if (!copy_x(d)) return matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
+    p.x = copy_of<T>(x, d->x_ld, false, ws, d->batch, d->in);
+    return own_matrix(ws, d->batch, d->in, sizeof(T));
+}
+template <typename T>
+int prepare_launch(hipStream_t st, const Prepare<T> &p, int np) {
+    const long long blocks = (long long)p.w.blocks + p.x.blocks + p.gz.blocks;
+    if (blocks == 0) return BT_OK;
+    BT_REQUIRE(blocks < (1 << 24), "bt_affine: Mismatched sizes! (too large to be copied: %lld blocks)", blocks);
+    const dim3 grid((unsigned)blocks), block(256);
+    if (p.gz.blocks == 0)
+        BT_LAUNCH(BTK_AFFINE, st, (affine_prepare<T, 0>), grid, block, 0, p);
+    else if (np == 1)
+        BT_LAUNCH(BTK_AFFINE, st, (affine_prepare<T, 1>), grid, block, 0, p);
+    else if constexpr (sizeof(T) == 2) {
+        if (np == 2)
+            BT_LAUNCH(BTK_AFFINE, st, (affine_prepare<T, 2>), grid, block, 0, p);
+        else if constexpr (std::is_same<T, __bf16>::value)
+            BT_LAUNCH(BTK_AFFINE, st, (affine_prepare<T, 3>), grid, block, 0, p);
+    }
     BT_LAUNCH_CHECK();
-    o = matrix(to, to_ld, rows, (int)to_ld, sizeof(T));  // (the zeros behind a row are part of it)
     return BT_OK;
-}
-template <typename T>
-int make_w(hipStream_t st, const bt_affine_desc *d, const void *w, void *ws, Operand &o) {
-    o = matrix(w, d->w_ld, d->in, d->out, sizeof(T));
-    if (!copy_w(d)) return BT_OK;
-    if (d->w_type != d->type) return copy_launch<float, T>(st, w, d->w_ld, ws, d->in, d->out, o);
-    return copy_launch<T, T>(st, w, d->w_ld, ws, d->in, d->out, o);
-}
-template <typename T>
-int make_x(hipStream_t st, const bt_affine_desc *d, const void *x, void *ws, Operand &o) {
-    o = matrix(x, d->x_ld, d->batch, d->in, sizeof(T));
-    return copy_x(d) ? copy_launch<T, T>(st, x, d->x_ld, ws, d->batch, d->in, o) : BT_OK;
 }
 
 constexpr int FEW = 8;  // rows that affine_few takes
@@ -869,8 +976,10 @@ int forward(hipStream_t st, const bt_affine_desc *d, const void *w, const float 
         return d->w_type == d->type ? few_launch<T, T>(st, d, w, x, e) : few_launch<T, float>(st, d, w, x, e);
     const ForwardPlan p = forward_plan(d);
     Product P = {};
-    if (int rc = make_w<T>(st, d, w, ws, P.b)) return rc;
-    if (int rc = make_x<T>(st, d, x, ws + p.w_bytes, P.a)) return rc;
+    Prepare<T> prep = {};
+    P.b = weights<T>(d, w, ws, prep);
+    P.a = inputs<T>(d, x, ws + p.w_bytes, prep);
+    if (int rc = prepare_launch<T>(st, prep, 0)) return rc;
     P.m = d->batch, P.n = d->out, P.k = d->in, P.passes = 1;
     P.part = (float *)(ws + p.w_bytes + p.x_bytes);
     P.e = e;
@@ -882,7 +991,7 @@ struct BackwardPlan {
     int np_dw, np_dx;    // summands it is kept as for dW (whose outputs are f32), and how many of them grad_x takes
     float alpha;
     int lift;
-    int range, ranges;
+    int range, ranges, col_blocks;
     Shape dw, dx;
     size_t w_bytes, x_bytes, gz_bytes, sum_bytes, part_bytes, total;
 };
@@ -895,8 +1004,9 @@ BackwardPlan backward_plan(const bt_affine_desc *d) {
     p.np_dx = p.np_dw > 2 ? 2 : p.np_dw;
     p.alpha = root ? 2.0f : 1.0f;
     p.lift = d->type == BT_TYPE_F16 && root;
-    p.range = 128;
-    while (bt_div_up(d->batch, p.range) > 1024) p.range *= 2;
+    // row ranges of affine_prepare: as many workgroups as fill the chip, at least the rows that one takes at once
+    p.col_blocks = bt_div_up(d->out, GZ_COLS * (int)(16 / es));
+    p.range = GZ_ROWS * bt_div_up((long long)d->batch * p.col_blocks, 1024 * GZ_ROWS);
     p.ranges = bt_div_up(d->batch, p.range);
     p.dw = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift);
     p.dx = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift);
@@ -915,54 +1025,47 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
     const BackwardPlan p = backward_plan(d);
     char *own_w = ws, *own_x = own_w + p.w_bytes, *kept = own_x + p.x_bytes, *sums = kept + p.gz_bytes * p.np_dw, *part = sums + p.sum_bytes;
     const bool keep = p.gz && (dw || gx);
-    const int np = !keep ? 1 : dw ? p.np_dw : p.np_dx;
+    const int np = dw ? p.np_dw : p.np_dx;
+    Prepare<T> prep = {};
+    const Operand ow = gx ? weights<T>(d, w, own_w, prep) : Operand{}, ox = dw ? inputs<T>(d, x, own_x, prep) : Operand{};
     if (keep || dbias) {
-        const dim3 grid(bt_div_up(d->out, GZ_COLS * Elem<T>::V), p.ranges);
-        Summands<T> gz = {{nullptr, nullptr, nullptr}};
-        for (int i = 0; i < np && keep; i++) gz.p[i] = (T *)(kept + i * p.gz_bytes);
-        float *sum = dbias ? (float *)sums : nullptr;
-        const T *o = d->act != BT_ACT_IDENTITY ? (const T *)out : nullptr;
-        const long long ld = d->y_ld, gz_ld = padded(d->out, sizeof(T));
-#define GZ_CASE(NP)                                                                                                          BT_LAUNCH(BTK_AFFINE, st, (affine_gz<T, NP>), grid, dim3(256), 0, (const T *)gy, o, ld, gz, gz_ld, sum, d->batch, d->out,               d->act, p.range)
-        if (np == 1)
-            GZ_CASE(1);
-        else if constexpr (sizeof(T) == 2) {
-            if (np == 2)
-                GZ_CASE(2);
-            else
-                GZ_CASE(3);
-        }
-#undef GZ_CASE
-        BT_LAUNCH_CHECK();
+        Gz<T> &g = prep.gz;
+        g.gy = (const T *)gy, g.out = d->act != BT_ACT_IDENTITY ? (const T *)out : nullptr;
+        for (int i = 0; i < np && keep; i++) g.p[i] = (T *)(kept + i * p.gz_bytes);
+        g.sums = dbias ? (float *)sums : nullptr;
+        g.ld = d->y_ld, g.gz_ld = padded(d->out, sizeof(T));
+        g.batch = d->batch, g.n = d->out, g.act = d->act, g.range = p.range, g.col_blocks = p.col_blocks;
+        g.blocks = p.col_blocks * p.ranges;
     }
-    if (dbias) {
-        BT_LAUNCH(BTK_AFFINE, st, affine_dbias, dim3(bt_div_up(d->out, 64)), dim3(1024), 0, (const float *)sums, p.ranges, d->out,
-                  p.alpha, dbias);
+    if (int rc = prepare_launch<T>(st, prep, keep ? np : 1)) return rc;
+    BiasSum bias = {};
+    if (dbias) bias = BiasSum{(const float *)sums, dbias, p.ranges, d->out, bt_div_up(d->out, BIAS_COLS), p.alpha};
+    if (dbias && !dw && !gx) {
+        BT_LAUNCH(BTK_AFFINE, st, affine_dbias, dim3(bias.blocks), dim3(256), 0, bias);
         BT_LAUNCH_CHECK();
     }
     const auto gz_operand = [&](int n) {  // its n largest summands, the smallest of them first
         if (!p.gz) return matrix(gy, d->y_ld, d->batch, d->out, sizeof(T));
-        const long long ld = padded(d->out, sizeof(T));  // (the zeros behind a row are part of it)
-        Operand o = matrix(kept, ld, d->batch, (int)ld, sizeof(T));
-        for (int i = 0; i < n; i++) o.p[i] = kept + (n - 1 - i) * p.gz_bytes;
+        Operand o = own_matrix(kept, d->batch, d->out, sizeof(T));
+        o.p0 = kept + (n - 1) * p.gz_bytes, o.p1 = n > 1 ? kept + (n - 2) * p.gz_bytes : kept, o.p2 = kept;
         return o;
     };
     if (dw) {
         Product P = {};
-        if (int rc = make_x<T>(st, d, x, own_x, P.a)) return rc;
-        P.b = gz_operand(p.np_dw);
+        P.a = ox, P.b = gz_operand(p.np_dw);
         P.m = d->in, P.n = d->out, P.k = d->batch, P.passes = p.np_dw, P.lift = p.lift;
         P.part = (float *)part;
         P.e.out = dw, P.e.ld = d->w_ld, P.e.alpha = p.alpha;
+        P.bias = bias;
         if (int rc = product_launch<T, false, false, OUT_F32>(st, P, p.dw)) return rc;
     }
     if (gx) {
         Product P = {};
-        if (int rc = make_w<T>(st, d, w, own_w, P.b)) return rc;
-        P.a = gz_operand(p.np_dx);
+        P.a = gz_operand(p.np_dx), P.b = ow;
         P.m = d->batch, P.n = d->in, P.k = d->out, P.passes = p.np_dx, P.lift = p.lift;
         P.part = (float *)part;
         P.e.out = gx, P.e.ld = d->x_ld, P.e.alpha = p.alpha;
+        if (!dw) P.bias = bias;
         if (int rc = product_launch<T, true, true, OUT_TYPE>(st, P, p.dx)) return rc;
     }
     return BT_OK;
