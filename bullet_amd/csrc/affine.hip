@@ -314,11 +314,15 @@ struct Stage {
     static __device__ __forceinline__ size_t step(const Operand &o) { return KC ? 128 : (size_t)o.ld * sizeof(T) * BK; }
 };
 
-// Which tile a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an L2 of its own: every XCD gets a
-// contiguous share of the tiles, and walks it in bands of 8 tiles of m so that what it holds of both operands is reused.
-__device__ __forceinline__ void tile_of(int wg, int wgs, int tiles_m, int tiles_n, int &split, int &tm, int &tn) {
+// Workgroups go to the 8 XCDs in turn, each with an L2 of its own: what number makes every XCD's share contiguous
+__device__ __forceinline__ int xcd_share(int wg, int wgs) {
     const int per = wgs / 8, rest = wgs % 8, xcd = wg % 8;
-    wg = xcd * per + min(xcd, rest) + wg / 8;
+    return xcd * per + min(xcd, rest) + wg / 8;
+}
+// Which tile a workgroup takes: an XCD walks its share in bands of 8 tiles of m, so that what it holds of both operands is
+// reused.
+__device__ __forceinline__ void tile_of(int wg, int wgs, int tiles_m, int tiles_n, int &split, int &tm, int &tn) {
+    wg = xcd_share(wg, wgs);
     const int tiles = tiles_m * tiles_n;
     split = wg / tiles;
     const int t = wg % tiles, band = t / (8 * tiles_n), in = t % (8 * tiles_n), high = min(8, tiles_m - band * 8);
@@ -722,7 +726,8 @@ __global__ __launch_bounds__(1024) void affine_few(const TW *__restrict__ w, lon
     typedef typename Elem<T>::frag xvec;
     __shared__ __align__(16) float red[16][R][COLS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 2;
-    const int c = blockIdx.x * COLS + (threadIdx.x & 3) * V;
+    const int chunk = xcd_share(blockIdx.x, gridDim.x);  // (neighbours read halves of the same lines)
+    const int c = chunk * COLS + (threadIdx.x & 3) * V;
     float acc[R][V];
 #pragma unroll
     for (int r = 0; r < R; r++)
@@ -781,7 +786,7 @@ __global__ __launch_bounds__(1024) void affine_few(const TW *__restrict__ w, lon
         }
     __syncthreads();
     if (threadIdx.x >= R * V) return;  // one thread for 4 outputs of a row
-    const int r = threadIdx.x / V, q = (threadIdx.x % V) * 4, col = blockIdx.x * COLS + q;
+    const int r = threadIdx.x / V, q = (threadIdx.x % V) * 4, col = chunk * COLS + q;
     if (r >= batch || col >= out) return;
     v4f v = {0, 0, 0, 0};
     for (int i = 0; i < 16; i++) v += *(const v4f *)&red[i][r][q];
