@@ -224,6 +224,7 @@ __device__ __forceinline__ void bias_sum(const BiasSum b, int block, float *lds)
     const int c = threadIdx.x % BIAS_COLS, r = threadIdx.x / BIAS_COLS, col = block * BIAS_COLS + c;
     float s = 0.0f;
     if (col < b.n)
+#pragma unroll 8
         for (int p = r; p < b.parts; p += NT / BIAS_COLS) s += b.part[(size_t)p * b.n + col];
     lds[threadIdx.x] = s;
     __syncthreads();
@@ -280,8 +281,9 @@ struct Stage {
         for (int q = 0; q < N; q++) *(v4u *)(lds + (q * NT + tid) * 16) = r[q];
     }
     // Direct loads: byte offsets of this thread's chunks from the tile's first element, the same for every tile. Rows (or
-    // chunks) of m or n beyond the end are taken from the last one: their sums are not stored.
-    static __device__ __forceinline__ bool inside(const Operand &o, int s0) { return KC || o.len - s0 >= SPAN || o.len % V == 0; }
+    // chunks) of m or n beyond the end are taken from the last one: their sums are not stored. Where that chunk is ragged,
+    // the elements behind it are whatever lies there up to the next row; there is no next row behind the last one.
+    static __device__ __forceinline__ bool ragged(const Operand &o, int s0) { return !KC && o.len - s0 < SPAN && o.len % V; }
     static __device__ __forceinline__ void offsets(const Operand &o, int s0, int tid, uint32_t (&off)[N]) {
         const int left = (KC ? o.rows : o.len) - s0;  // > 0
 #pragma unroll
@@ -289,7 +291,7 @@ struct Stage {
             const int s = q * NT + tid;
             int row = s / L::CPR, c = L::swizzle(row, s % L::CPR);
             if (KC) row = min(row, left - 1);
-            if (!KC) c = max(min(c, left / V - 1), 0);
+            if (!KC) c = min(c, (left - 1) / V);
             off[q] = (uint32_t)row * (uint32_t)(o.ld * sizeof(T)) + c * 16;
         }
     }
@@ -458,8 +460,8 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 // the first half of a tile's k is multiplied the second half's fragments are read; behind the barrier that says that the
 // next tile has arrived its first fragments are read, and the tile after it is sent for into the buffer just left, while
 // the second half is multiplied. Each fragment's products carry their share of those reads and loads.
-// The tiles that the matrices fill come first; the others (the rest of k, one of each summand; all, where the span ends
-// inside a chunk) take the same way with a check of every chunk.
+// The tiles that k fills come first; the others, one of each summand (the rest of k; the last full one, where its last row
+// must not be read to the end of a chunk), take the same way with a check of every chunk.
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
@@ -469,11 +471,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     if (blockIdx.x >= gridDim.x - P.bias.blocks)
         return bias_sum<M::NT>(P.bias, blockIdx.x - (gridDim.x - P.bias.blocks), (float *)lds);
     M mm(P, lds);
-    const bool inside = M::SA::inside(mm.a, mm.m0) && M::SB::inside(mm.b, mm.n0);
-    const int ktiles = (P.k + M::BK - 1) / M::BK, full = P.k / M::BK;
+    const bool ragged = M::SA::ragged(mm.a, mm.m0) || M::SB::ragged(mm.b, mm.n0);
+    const int full = (P.k - ragged) / M::BK;
     int p0, p1, t0, t1;
-    const bool last = mm.share(inside ? full : ktiles, p0, p1, t0, t1);
-    const int quick = inside ? t1 - t0 : 0, tiles = !inside ? t1 - t0 : quick + (last && full < ktiles ? p1 - p0 : 0);
+    const bool last = mm.share(full, p0, p1, t0, t1);
+    const int quick = t1 - t0, tiles = quick + (last && full * M::BK < P.k ? p1 - p0 : 0);
 
     uint32_t oa[NA], ob[NB];
     M::SA::offsets(mm.a, mm.m0, mm.tid, oa);
@@ -498,10 +500,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
         }
     };
     const auto careful = [&](int tile, int buf) {
-        const int c = inside ? tile - quick : t0 + tile;
-        const int ps = p0 + (inside ? c : c / ktiles), k0 = (inside ? full : c % ktiles) * M::BK;
-        M::SA::careful(mm.a, ps, mm.m0, k0, mm.tid, lds + buf * M::BYTES);
-        M::SB::careful(mm.b, ps, mm.n0, k0, mm.tid, lds + buf * M::BYTES + M::TA::BYTES);
+        M::SA::careful(mm.a, p0 + tile - quick, mm.m0, full * M::BK, mm.tid, lds + buf * M::BYTES);
+        M::SB::careful(mm.b, p0 + tile - quick, mm.n0, full * M::BK, mm.tid, lds + buf * M::BYTES + M::TA::BYTES);
     };
     frag fa[FM], fb[2][FN];
     // The products of half 1 - s, and beside them: fragments of half s of the tile in buffer `buf` (of m: into the registers
@@ -570,10 +570,16 @@ __global__ __launch_bounds__(256) void affine_join(Product P) {
     if (q >= cols * P.m) return;
     const int m = (int)(q / cols), n = (int)(q % cols) * 4;
     v4f v = {0, 0, 0, 0};
-    for (int s = 0; s < P.splits; s++) {
-        if (P.lift && s == P.splits / 2) v *= 1.0f / F16_LIFT;
-        v += *(const v4f *)(P.part + ((size_t)s * P.m + m) * P.part_ld + n);
-    }
+    const float *part = P.part + (size_t)m * P.part_ld + n;
+    const size_t step = (size_t)P.m * P.part_ld;
+    const auto add = [&](int s0, int s1) {
+#pragma unroll 8
+        for (int s = s0; s < s1; s++) v += *(const v4f *)(part + s * step);
+    };
+    const int lifted = P.lift ? P.splits / 2 : 0;
+    add(0, lifted);
+    if (P.lift) v *= 1.0f / F16_LIFT;
+    add(lifted, P.splits);
     finish4<T, OUT>(P.e, m, n, P.n - n, v, residual4<T, OUT>(P.e, m, n, P.n - n));
 }
 
@@ -1009,9 +1015,11 @@ BackwardPlan backward_plan(const bt_affine_desc *d) {
     p.np_dx = p.np_dw > 2 ? 2 : p.np_dw;
     p.alpha = root ? 2.0f : 1.0f;
     p.lift = d->type == BT_TYPE_F16 && root;
-    // row ranges of affine_prepare: as many workgroups as fill the chip, at least the rows that one takes at once
+    // row ranges of affine_prepare: as many workgroups as fill the chip, at least the rows that one takes at once, and no
+    // more ranges than bias_sum adds up in a few us (8192 x 288 -> 6 f16: 1024 ranges 66 us in all, 256 @@ us)
     p.col_blocks = bt_div_up(d->out, GZ_COLS * (int)(16 / es));
-    p.range = GZ_ROWS * bt_div_up((long long)d->batch * p.col_blocks, 1024 * GZ_ROWS);
+    const int fill = bt_div_up((long long)d->batch * p.col_blocks, 1024 * GZ_ROWS), few = bt_div_up(d->batch, 256 * GZ_ROWS);
+    p.range = GZ_ROWS * (fill > few ? fill : few);
     p.ranges = bt_div_up(d->batch, p.range);
     p.dw = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift);
     p.dx = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift);
