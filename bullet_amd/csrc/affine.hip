@@ -721,16 +721,18 @@ __global__ __launch_bounds__(256) void affine_prepare(Prepare<T> p) {
 }
 
 // Forward of at most R rows (one position, or a few): the weights are all there is to read, and each is used R times, so
-// there is nothing for the matrix cores. A workgroup of 1024 takes 4 chunks of outputs (64 bytes of every weight column;
-// f32 weights of a 16-bit layer: 128) for all inputs: 256 groups of 4 lanes walk the inputs V at a time with V weight loads
-// in flight each, and their sums meet in DPP, shuffles and LDS, in a fixed order.
+// there is nothing for the matrix cores. A workgroup takes 4 chunks of outputs (64 bytes of every weight column; f32
+// weights of a 16-bit layer: 128) for all inputs: its groups of 4 lanes walk the inputs V at a time with V weight loads in
+// flight each, and their sums meet in DPP, shuffles and LDS, in a fixed order. 1024 threads, or 512 where the sums and
+// loads of more than 2 rows need the registers.
+constexpr int few_threads(int rows) { return rows > 2 ? 512 : 1024; }
 template <typename T, typename TW, int R>
-__global__ __launch_bounds__(1024) void affine_few(const TW *__restrict__ w, long long w_ld, const T *__restrict__ x, long long x_ld,
+__global__ __launch_bounds__(few_threads(R)) void affine_few(const TW *__restrict__ w, long long w_ld, const T *__restrict__ x, long long x_ld,
                                                    int batch, int in, int out, Epilogue e) {
-    constexpr int V = Elem<T>::V, COLS = 4 * V;
+    constexpr int V = Elem<T>::V, COLS = 4 * V, NT = few_threads(R);
     typedef TW wvec __attribute__((ext_vector_type(V)));
     typedef typename Elem<T>::frag xvec;
-    __shared__ __align__(16) float red[16][R][COLS];
+    __shared__ __align__(16) float red[NT / 64][R][COLS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 2;
     const int chunk = xcd_share(blockIdx.x, gridDim.x);  // (neighbours read halves of the same lines)
     const int c = chunk * COLS + (threadIdx.x & 3) * V;
@@ -739,7 +741,7 @@ __global__ __launch_bounds__(1024) void affine_few(const TW *__restrict__ w, lon
     for (int r = 0; r < R; r++)
 #pragma unroll
         for (int j = 0; j < V; j++) acc[r][j] = 0.0f;
-    for (long long k = (long long)group * V; k < in; k += 256 * V) {
+    for (long long k = (long long)group * V; k < in; k += NT / 4 * V) {
         const int nk = in - k < V ? (int)(in - k) : V;
         wvec wv[V];
         xvec xv[R];
@@ -795,7 +797,7 @@ __global__ __launch_bounds__(1024) void affine_few(const TW *__restrict__ w, lon
     const int r = threadIdx.x / V, q = (threadIdx.x % V) * 4, col = chunk * COLS + q;
     if (r >= batch || col >= out) return;
     v4f v = {0, 0, 0, 0};
-    for (int i = 0; i < 16; i++) v += *(const v4f *)&red[i][r][q];
+    for (int i = 0; i < NT / 64; i++) v += *(const v4f *)&red[i][r][q];
     finish4<T, OUT_LAYER>(e, r, col, out - col, v, residual4<T, OUT_LAYER>(e, r, col, out - col));
 }
 
@@ -948,19 +950,22 @@ int prepare_launch(hipStream_t st, const Prepare<T> &p, int np) {
     return BT_OK;
 }
 
-constexpr int FEW = 8;  // rows that affine_few takes
+// Rows that affine_few takes: 8, but 4 where both weights and rows have 16 bits (2048 -> 4096 bf16: 4 rows 8.9 us against 9.9 on
+// the matrix cores, 8 rows 13.3 against 9.9; f32: 8 rows 11.2 against 16; f32 weights that would have to be rounded into a
+// copy first: 8 rows 16 against 20)
+int few_rows(const bt_affine_desc *d) { return d->w_type == BT_TYPE_F32 ? 8 : 4; }
 template <typename T, typename TW>
 int few_launch(hipStream_t st, const bt_affine_desc *d, const void *w, const void *x, const Epilogue &e) {
-    const dim3 grid(bt_div_up(d->out, 4 * Elem<T>::V)), block(1024);
-#define FEW_CASE(R)                                                                                                                  BT_LAUNCH(BTK_AFFINE, st, (affine_few<T, TW, R>), grid, block, 0, (const TW *)w, (long long)d->w_ld, (const T *)x,               (long long)d->x_ld, d->batch, d->in, d->out, e)
+    const dim3 grid(bt_div_up(d->out, 4 * Elem<T>::V));
+#define FEW_CASE(R)                                                                                                                  BT_LAUNCH(BTK_AFFINE, st, (affine_few<T, TW, R>), grid, dim3(few_threads(R)), 0, (const TW *)w, (long long)d->w_ld, (const T *)x,               (long long)d->x_ld, d->batch, d->in, d->out, e)
     if (d->batch == 1)
         FEW_CASE(1);
     else if (d->batch == 2)
         FEW_CASE(2);
     else if (d->batch <= 4)
         FEW_CASE(4);
-    else
-        FEW_CASE(FEW);
+    else if constexpr (sizeof(TW) == 4)
+        FEW_CASE(8);
 #undef FEW_CASE
     BT_LAUNCH_CHECK();
     return BT_OK;
@@ -972,7 +977,7 @@ struct ForwardPlan {
 };
 ForwardPlan forward_plan(const bt_affine_desc *d) {
     ForwardPlan p = {};
-    if (d->batch <= FEW) return p;
+    if (d->batch <= few_rows(d)) return p;
     const size_t es = type_size(d->type);
     p.s = shape_of(d->batch, d->out, d->in, 1, es);
     p.w_bytes = copy_bytes(copy_w(d), d->in, d->out, es), p.x_bytes = copy_bytes(copy_x(d), d->batch, d->in, es);
@@ -983,7 +988,7 @@ template <typename T>
 int forward(hipStream_t st, const bt_affine_desc *d, const void *w, const float *bias, const void *x, const void *residual, void *y,
             void *saved, char *ws) {
     const Epilogue e{bias, residual, y, saved, d->y_ld, d->act, 1.0f};
-    if (d->batch <= FEW)
+    if (d->batch <= few_rows(d))
         return d->w_type == d->type ? few_launch<T, T>(st, d, w, x, e) : few_launch<T, float>(st, d, w, x, e);
     const ForwardPlan p = forward_plan(d);
     Product P = {};
