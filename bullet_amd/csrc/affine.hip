@@ -711,13 +711,13 @@ struct Prepare {
 };
 template <typename T, int NP>  // NP = 0: copies only
 __global__ __launch_bounds__(256) void affine_prepare(Prepare<T> p) {
-    long long block = blockIdx.x;
+    long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
     if constexpr (NP > 0) {
         if (block < p.gz.blocks) return gz_block<T, NP>(p.gz, (int)block);
         block -= p.gz.blocks;
     }
     if (block < p.w.blocks) return copy_block<T>(p.w, block);
-    copy_block<T>(p.x, block - p.w.blocks);
+    if (block - p.w.blocks < p.x.blocks) copy_block<T>(p.x, block - p.w.blocks);
 }
 
 // Forward of at most R rows (one position, or a few): the weights are all there is to read, and each is used R times, so
@@ -859,7 +859,7 @@ Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false) {
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
 int mm_launch(hipStream_t st, const Product &P, bool direct) {
     const long long blocks = (long long)P.tiles_m * P.tiles_n * P.splits;
-    BT_REQUIRE(blocks < (1 << 22), "bt_affine: Mismatched sizes! (%lld tiles)", blocks);
+    BT_REQUIRE((blocks + P.bias.blocks) * 64 * WM * WN < (1ll << 32), "bt_affine: Mismatched sizes! (%lld tiles)", blocks);
     const size_t lds = 2 * Mm<T, BM, BN, WM, WN, AK, BKC, OUT>::BYTES;
     const dim3 grid((unsigned)(blocks + P.bias.blocks)), block(64 * WM * WN);
     if (direct) {
@@ -905,8 +905,8 @@ Operand matrix(const void *p, long long ld, int rows, int len, size_t es) {
 Operand own_matrix(const void *p, int rows, int len, size_t es) { return matrix(p, padded(len, es), rows, whole_chunks(len, es), es); }
 
 // Matrices that are copied into the workspace first: those whose rows do not start on 16 bytes (read through registers
-// instead, 1537 x 1027 -> 1881 f16 takes 34 us, copied 22), and f32 weights of a 16-bit layer. One whose first element alone is
-// off is read through registers.
+// instead, both operands of 4096 x 1024 -> 1024 make the forward product 38 us of bf16 and 102 of f32; the copies take 8 and
+// 13 us and leave 18 and 73), and f32 weights of a 16-bit layer. One whose first element alone is off is read through registers.
 size_t copy_bytes(bool copy, int rows, int len, size_t es) { return copy ? bt_align((size_t)rows * padded(len, es) * es) : 0; }
 bool copy_w(const bt_affine_desc *d) { return d->w_type != d->type || !direct_ld(d->w_ld, type_size(d->type)); }
 bool copy_x(const bt_affine_desc *d) { return !direct_ld(d->x_ld, type_size(d->type)); }
@@ -934,8 +934,9 @@ template <typename T>
 int prepare_launch(hipStream_t st, const Prepare<T> &p, int np) {
     const long long blocks = (long long)p.w.blocks + p.x.blocks + p.gz.blocks;
     if (blocks == 0) return BT_OK;
-    BT_REQUIRE(blocks < (1 << 24), "bt_affine: Mismatched sizes! (too large to be copied: %lld blocks)", blocks);
-    const dim3 grid((unsigned)blocks), block(256);
+    // (a launch holds less than 2^32 threads a dimension)
+    constexpr long long W = 1 << 22;
+    const dim3 grid((unsigned)(blocks < W ? blocks : W), (unsigned)((blocks + W - 1) / W)), block(256);
     if (p.gz.blocks == 0)
         BT_LAUNCH(BTK_AFFINE, st, (affine_prepare<T, 0>), grid, block, 0, p);
     else if (np == 1)
@@ -1021,7 +1022,7 @@ BackwardPlan backward_plan(const bt_affine_desc *d) {
     p.alpha = root ? 2.0f : 1.0f;
     p.lift = d->type == BT_TYPE_F16 && root;
     // row ranges of affine_prepare: as many workgroups as fill the chip, at least the rows that one takes at once, and no
-    // more ranges than bias_sum adds up in a few us (8192 x 288 -> 6 f16: 1024 ranges 66 us in all, 256 @@ us)
+    // more ranges than bias_sum adds up in a few us (8192 x 288 -> 6 f16: 1024 ranges 66 us in all, 256 50 us)
     p.col_blocks = bt_div_up(d->out, GZ_COLS * (int)(16 / es));
     const int fill = bt_div_up((long long)d->batch * p.col_blocks, 1024 * GZ_ROWS), few = bt_div_up(d->batch, 256 * GZ_ROWS);
     p.range = GZ_ROWS * (fill > few ? fill : few);

@@ -8,7 +8,16 @@ import pytest
 import affine_ref as ar
 from bullet_amd import lib
 
-L = lib.load()
+
+class Library:
+    """the library, loaded by the first call and not while tests are collected: torch's own HIP runtime has to be the
+    process's first one where there is a GPU"""
+
+    def __getattr__(self, name):
+        return getattr(lib.load(), name)
+
+
+L = Library()
 A = [256 * (i + 1) for i in range(12)]  # stand for buffers: distinct, aligned, and never used by a call that is refused
 
 

@@ -331,6 +331,24 @@ def test_preference_offsets_out_of_range_are_clamped():
     assert out[0][0] == out[1][0] and np.array_equal(out[0][1], out[1][1])
 
 
+def test_preference_without_rows_or_gradient():
+    """no rows at all: every line is empty; and the losses alone"""
+    for rows in (0, 5):
+        d = pr.preference_desc(3, rows, 20, "f32")
+        ws = torch.zeros(lib.load().bt_preference_loss_workspace_bytes(C.byref(d)), dtype=torch.uint8, device="cuda")
+        z, actions = np.random.default_rng(28).standard_normal((max(rows, 1), 20)), np.zeros(max(rows, 1), np.int32)
+        offsets = np.minimum(np.arange(7), rows).astype(np.int32)
+        ref = np.linspace(-1, 1, 6).astype(np.float32)
+        loss, pl, ll = torch.zeros(1, device="cuda"), torch.zeros(3, device="cuda"), torch.zeros(6, device="cuda")
+        zt = dev(z, np.float32)
+        pr.call_preference(stream(), d, zt, None, dev(actions), dev(offsets), dev(ref), None, loss, zt if rows == 0 else None,
+                           pl, ll, ws)
+        want, tol = pr.preference(zt.double().cpu().numpy(), None, actions, offsets, ref, None, 0.1, 0.05)
+        for name, t in (("loss", loss), ("pair_loss", pl), ("line_logp", ll)):
+            pr.check(t.cpu().numpy(), want[name], tol[name], "f32", name)
+        assert np.array_equal(zt.cpu().numpy(), z.astype(np.float32))
+
+
 # ---------------------------------------------------------------- streams and graphs
 def test_losses_replayed_from_a_graph_and_on_another_stream():
     rng = np.random.default_rng(31)

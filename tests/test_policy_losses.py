@@ -8,7 +8,16 @@ import pytest
 import policy_ref as pr
 from bullet_amd import lib
 
-L = lib.load()
+
+class Library:
+    """the library, loaded by the first call and not while tests are collected: torch's own HIP runtime has to be the
+    process's first one where there is a GPU"""
+
+    def __getattr__(self, name):
+        return getattr(lib.load(), name)
+
+
+L = Library()
 P = 64  # stands for a buffer: aligned, never followed by a call that is refused
 
 
