@@ -9,24 +9,21 @@ import affine_ref as ar
 from bullet_amd import lib
 
 
-class Library:
+def L():
     """the library, loaded by the first call and not while tests are collected: torch's own HIP runtime has to be the
     process's first one where there is a GPU"""
-
-    def __getattr__(self, name):
-        return getattr(lib.load(), name)
+    return lib.load()
 
 
-L = Library()
 A = [256 * (i + 1) for i in range(12)]  # stand for buffers: distinct, aligned, and never used by a call that is refused
 
 
 def fwd(d, w=A[0], bias=A[1], x=A[2], res=A[3], y=A[4], saved=A[5], ws=A[6], wsb=1 << 40):
-    return L.bt_affine_forward(None, C.byref(d) if d is not None else None, w, bias, x, res, y, saved, ws, wsb)
+    return L().bt_affine_forward(None, C.byref(d) if d is not None else None, w, bias, x, res, y, saved, ws, wsb)
 
 
 def bwd(d, w=A[0], x=A[1], out=A[2], gy=A[3], dw=A[4], db=A[5], gx=A[6], ws=A[7], wsb=1 << 40):
-    return L.bt_affine_backward(None, C.byref(d) if d is not None else None, w, x, out, gy, dw, db, gx, ws, wsb)
+    return L().bt_affine_backward(None, C.byref(d) if d is not None else None, w, x, out, gy, dw, db, gx, ws, wsb)
 
 
 SHAPES = [(dict(batch=0), b"0 x 8 -> 6"), (dict(in_=-1), b"4 x -1"), (dict(out=0), b"Mismatched sizes"),
@@ -41,9 +38,9 @@ def test_shapes_are_refused(change, message):
     for k, v in change.items():
         setattr(d, k, v)
     for call in (fwd, bwd):
-        assert call(d) == 1 and message in L.bt_last_error(), L.bt_last_error()
-    assert L.bt_affine_forward_workspace_bytes(C.byref(d)) == 0 and message in L.bt_last_error()
-    assert L.bt_affine_backward_workspace_bytes(C.byref(d)) == 0 and message in L.bt_last_error()
+        assert call(d) == 1 and message in L().bt_last_error(), L().bt_last_error()
+    assert L().bt_affine_forward_workspace_bytes(C.byref(d)) == 0 and message in L().bt_last_error()
+    assert L().bt_affine_backward_workspace_bytes(C.byref(d)) == 0 and message in L().bt_last_error()
 
 
 @pytest.mark.parametrize("args,message", [
@@ -53,7 +50,7 @@ def test_shapes_are_refused(change, message):
     (dict(saved=A[3]), b"overlap"), (dict(y=A[2]), b"overlap"),
 ])
 def test_forward_refuses(args, message):
-    assert fwd(ar.desc(4, 8, 6, "f32"), **args) == 1 and message in L.bt_last_error(), L.bt_last_error()
+    assert fwd(ar.desc(4, 8, 6, "f32"), **args) == 1 and message in L().bt_last_error(), L().bt_last_error()
 
 
 @pytest.mark.parametrize("args,message", [
@@ -63,18 +60,18 @@ def test_forward_refuses(args, message):
     (dict(dw=1282), b"not aligned"), (dict(gx=A[3]), b"overlaps"), (dict(gx=A[1]), b"overlaps"), (dict(dw=A[0]), b"overlaps"),
 ])
 def test_backward_refuses(args, message):
-    assert bwd(ar.desc(4, 8, 6, "f32", "relu"), **args) == 1 and message in L.bt_last_error(), L.bt_last_error()
+    assert bwd(ar.desc(4, 8, 6, "f32", "relu"), **args) == 1 and message in L().bt_last_error(), L().bt_last_error()
 
 
 def test_other_refusals():
-    assert fwd(None) == 1 and bwd(None) == 1 and b"null pointer" in L.bt_last_error()
-    assert bwd(ar.desc(4, 8, 6, "f16", "sqrrelu")) == 1 and b"range of f16" in L.bt_last_error()
+    assert fwd(None) == 1 and bwd(None) == 1 and b"null pointer" in L().bt_last_error()
+    assert bwd(ar.desc(4, 8, 6, "f16", "sqrrelu")) == 1 and b"range of f16" in L().bt_last_error()
     d = ar.desc(64, 256, 96, "bf16", "relu", w32=True)
-    need = L.bt_affine_forward_workspace_bytes(C.byref(d))
+    need = L().bt_affine_forward_workspace_bytes(C.byref(d))
     assert need >= 256 * 96 * 2
-    assert fwd(d, wsb=need - 1) == 1 and b"workspace too small" in L.bt_last_error()
-    assert fwd(d, ws=None) == 1 and b"workspace too small" in L.bt_last_error()
-    assert fwd(d, ws=A[6] + 4) == 1 and b"workspace is not aligned" in L.bt_last_error()
+    assert fwd(d, wsb=need - 1) == 1 and b"workspace too small" in L().bt_last_error()
+    assert fwd(d, ws=None) == 1 and b"workspace too small" in L().bt_last_error()
+    assert fwd(d, ws=A[6] + 4) == 1 and b"workspace is not aligned" in L().bt_last_error()
 
 
 @pytest.mark.parametrize("kind", ["identity", "relu", "crelu", "screlu", "sqrrelu"])

@@ -9,20 +9,17 @@ import policy_ref as pr
 from bullet_amd import lib
 
 
-class Library:
+def L():
     """the library, loaded by the first call and not while tests are collected: torch's own HIP runtime has to be the
     process's first one where there is a GPU"""
-
-    def __getattr__(self, name):
-        return getattr(lib.load(), name)
+    return lib.load()
 
 
-L = Library()
 P = 64  # stands for a buffer: aligned, never followed by a call that is refused
 
 
 def policy(d, z=P, mask=P, actions=P, old=P, adv=P, ref=P, w=P, loss=P, grad=P * 2, row_loss=P, logp=P, kl=P):
-    return L.bt_policy_loss(None, C.byref(d) if d is not None else None, z, mask, actions, old, adv, ref, w, loss, grad,
+    return L().bt_policy_loss(None, C.byref(d) if d is not None else None, z, mask, actions, old, adv, ref, w, loss, grad,
                             row_loss, logp, kl)
 
 
@@ -44,15 +41,15 @@ def test_policy_loss_refuses(change, args, message):
     for k, v in change.items():
         setattr(d, k, v)
     assert policy(d, **args) == 1
-    assert message in L.bt_last_error(), L.bt_last_error()
+    assert message in L().bt_last_error(), L().bt_last_error()
 
 
 def test_policy_loss_refuses_a_null_descriptor():
-    assert policy(None) == 1 and b"null pointer" in L.bt_last_error()
+    assert policy(None) == 1 and b"null pointer" in L().bt_last_error()
 
 
 def preference(d, z=P, mask=P, actions=P, offsets=P, ref=P, w=P, loss=P, grad=P, pair_loss=P, line=P, ws=P, wsb=1 << 30):
-    return L.bt_preference_loss(None, C.byref(d) if d is not None else None, z, mask, actions, offsets, ref, w, loss, grad,
+    return L().bt_preference_loss(None, C.byref(d) if d is not None else None, z, mask, actions, offsets, ref, w, loss, grad,
                                 pair_loss, line, ws, wsb)
 
 
@@ -71,14 +68,14 @@ def test_preference_loss_refuses(change, args, message):
     for k, v in change.items():
         setattr(d, k, v)
     assert preference(d, **args) == 1
-    assert message in L.bt_last_error(), L.bt_last_error()
+    assert message in L().bt_last_error(), L().bt_last_error()
 
 
 def test_preference_workspace():
     d = pr.preference_desc(4, 30, 10, "f32")
-    assert L.bt_preference_loss_workspace_bytes(C.byref(d)) == 6 * 256
+    assert L().bt_preference_loss_workspace_bytes(C.byref(d)) == 6 * 256
     d.ld = 3
-    assert L.bt_preference_loss_workspace_bytes(C.byref(d)) == 0 and b"leading dimension 3" in L.bt_last_error()
+    assert L().bt_preference_loss_workspace_bytes(C.byref(d)) == 0 and b"leading dimension 3" in L().bt_last_error()
 
 
 @pytest.mark.parametrize("kl", ["none", "taken", "full"])
