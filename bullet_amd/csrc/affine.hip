@@ -21,7 +21,6 @@ struct Elem {
     static constexpr int V = 16 / sizeof(T);          // elements of a 16-byte chunk
     static constexpr int BK = 128 / sizeof(T);        // k per tile: 128 bytes
     typedef T frag __attribute__((ext_vector_type(16 / sizeof(T))));
-    typedef T quad __attribute__((ext_vector_type(4)));
 };
 
 // acc += a b^T over the k of one fragment: lane l holds row l % 16 and, of 16-bit types, k = 8 (l / 16) .. + 7 of 32 (one
@@ -142,70 +141,70 @@ struct Epilogue {
     float alpha;
 };
 
-template <typename T>
-__device__ __forceinline__ void store4(T *p, v4f v, int n) {  // the first n of 4
-    typedef T quad __attribute__((ext_vector_type(4)));
-    quad q;
-#pragma unroll
-    for (int j = 0; j < 4; j++) q[j] = (T)v[j];
-    if (n >= 4) {
-        __builtin_memcpy(p, &q, sizeof(q));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (j < n) p[j] = q[j];
-    }
-}
-// the residual under 4 sums of one row, columns c .. c + 3 (n of them inside the matrix); zeros without one
-template <typename T, int OUT>
-__device__ __forceinline__ typename Elem<T>::quad residual4(const Epilogue &e, int row, int c, int n) {
-    typename Elem<T>::quad q = {};
-    if (OUT == OUT_LAYER && e.residual) {
-        const T *r = (const T *)e.residual + ((size_t)row * e.ld + c);
-        if (n >= 4) {
-            __builtin_memcpy(&q, r, sizeof(q));
+// W neighbouring columns of one row, n of them inside the matrix
+template <typename T, int W>
+struct Cols {
+    typedef float sums __attribute__((ext_vector_type(W)));
+    typedef T vec __attribute__((ext_vector_type(W)));
+    static __device__ __forceinline__ vec load(const T *p, int n) {
+        vec v = {};
+        if (n >= W) {
+            __builtin_memcpy(&v, p, sizeof(v));
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j < n) q[j] = r[j];
+            for (int j = 0; j < W; j++)
+                if (j < n) v[j] = p[j];
+        }
+        return v;
+    }
+    static __device__ __forceinline__ void store(T *p, sums v, int n) {
+        vec q;
+#pragma unroll
+        for (int j = 0; j < W; j++) q[j] = (T)v[j];
+        if (n >= W) {
+            __builtin_memcpy(p, &q, sizeof(q));
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; j++)
+                if (j < n) p[j] = q[j];
         }
     }
-    return q;
+};
+template <typename T, int OUT, int W>
+__device__ __forceinline__ typename Cols<T, W>::vec residual_at(const Epilogue &e, int row, int c, int n) {
+    if (OUT != OUT_LAYER || !e.residual) return typename Cols<T, W>::vec{};
+    return Cols<T, W>::load((const T *)e.residual + ((size_t)row * e.ld + c), n);
 }
-// what becomes of those sums
-template <typename T, int OUT>
-__device__ __forceinline__ void finish4(const Epilogue &e, int row, int c, int n, v4f v, typename Elem<T>::quad residual) {
+template <int OUT, int W>
+__device__ __forceinline__ typename Cols<float, W>::sums bias_at(const Epilogue &e, int c, int n) {
+    if (OUT != OUT_LAYER || !e.bias || n <= 0) return typename Cols<float, W>::sums{};
+    return Cols<float, W>::load(e.bias + c, n);
+}
+// what becomes of W sums of one row, columns from c on
+template <typename T, int OUT, int W>
+__device__ __forceinline__ void finish_at(const Epilogue &e, int row, int c, int n, typename Cols<T, W>::sums v,
+                                          typename Cols<T, W>::sums bias, typename Cols<T, W>::vec residual) {
     const size_t at = (size_t)row * e.ld + c;
     if constexpr (OUT == OUT_F32) {
-        store4<float>((float *)e.out + at, v * e.alpha, n);
+        Cols<float, W>::store((float *)e.out + at, v * e.alpha, n);
     } else if constexpr (OUT == OUT_TYPE) {
-        store4<T>((T *)e.out + at, v * e.alpha, n);
+        Cols<T, W>::store((T *)e.out + at, v * e.alpha, n);
     } else {
-        if (e.bias) {
-            v4f b = {0, 0, 0, 0};
-            if (n >= 4) {
-                __builtin_memcpy(&b, e.bias + c, 16);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (j < n) b[j] = e.bias[c + j];
-            }
-            v += b;
-        }
+        v += bias;
         // bt_act_fwd without its branches: this is unrolled over a whole tile
         const float top = e.act == BT_ACT_CRELU || e.act == BT_ACT_SCRELU ? 1.0f : __builtin_huge_valf();
         const bool clamp = e.act != BT_ACT_IDENTITY, square = e.act == BT_ACT_SCRELU || e.act == BT_ACT_SQRRELU;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < W; j++) {
             const float a = fminf(fmaxf(v[j], 0.0f), top), b = square ? a * a : a;
             v[j] = clamp ? b : v[j];
         }
-        if (e.saved) store4<T>((T *)e.saved + at, v, n);
+        if (e.saved) Cols<T, W>::store((T *)e.saved + at, v, n);
         if (e.residual) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] += (float)residual[j];
+            for (int j = 0; j < W; j++) v[j] += (float)residual[j];
         }
-        store4<T>((T *)e.out + at, v, n);
+        Cols<T, W>::store((T *)e.out + at, v, n);
     }
 }
 
@@ -325,10 +324,13 @@ __device__ __forceinline__ int xcd_share(int wg, int wgs) {
 // reused.
 __device__ __forceinline__ void tile_of(int wg, int wgs, int tiles_m, int tiles_n, int &split, int &tm, int &tn) {
     wg = xcd_share(wg, wgs);
-    const int tiles = tiles_m * tiles_n;
-    split = wg / tiles;
-    const int t = wg % tiles, band = t / (8 * tiles_n), in = t % (8 * tiles_n), high = min(8, tiles_m - band * 8);
-    tm = band * 8 + in % high, tn = in / high;
+    // (a division costs more than a tile's worth of products of a short sum: none where the answer is known)
+    const unsigned tiles = tiles_m * tiles_n;
+    split = wgs == (int)tiles ? 0 : (unsigned)wg / tiles;
+    const unsigned t = wg - split * tiles, per_band = 8 * tiles_n, band = t / per_band, in = t - band * per_band;
+    const unsigned high = min(8, tiles_m - (int)band * 8);
+    tn = high == 8 ? in / 8 : in / high;
+    tm = band * 8 + (in - tn * high);
 }
 
 // What the kernels below share: a BM x BN tile by WM x WN waves, each with FM x FN blocks of 16 x 16 sums.
@@ -366,10 +368,17 @@ struct Mm {
     // This workgroup's share of `ktiles` tiles of k a summand: the summands [p0, p1), the tiles [t0, t1) of theirs put one
     // behind the other, and whether that is the last share of them.
     __device__ __forceinline__ bool share(int ktiles, int &p0, int &p1, int &t0, int &t1) const {
-        const int subs = P.lift ? P.splits / 2 : P.splits, sub = P.lift ? split % subs : split;
-        p0 = P.lift ? split / subs : 0, p1 = P.lift ? p0 + 1 : P.passes;
-        const long long all = (long long)ktiles * (p1 - p0);
-        t0 = (int)(all * sub / subs), t1 = (int)(all * (sub + 1) / subs);
+        const int half = P.lift ? P.splits / 2 : 0;  // splits of the first summand, where each takes one of the two
+        const bool second = P.lift && split >= half;
+        const int subs = P.lift ? half : P.splits, sub = second ? split - half : split;
+        p0 = second, p1 = P.lift ? p0 + 1 : P.passes;
+        const unsigned all = (unsigned)ktiles * (p1 - p0);
+        if (subs == 1) {
+            t0 = 0, t1 = all;
+        } else {  // the first all % subs shares are one longer
+            const unsigned each = all / subs, rest = all - each * subs;
+            t0 = sub * each + min((unsigned)sub, rest), t1 = t0 + each + ((unsigned)sub < rest);
+        }
         return sub == subs - 1;
     }
     __device__ __forceinline__ frag read_a(int buf, int j, int s) const { return TA::read(at_a + buf * BYTES, j, s); }
@@ -387,27 +396,31 @@ struct Mm {
         }
     }
     // Lane l holds, of each 16 x 16 block, row m = l % 16 and columns n = 4 (l / 16) .. + 3. Every wave turns 16 rows at a
-    // time in its own piece of LDS, so that 16 lanes finish (and load and store) one row's 64 consecutive columns.
+    // time in its own piece of LDS, so that neighbouring lanes finish (and load and store) 16 bytes each of one row's
+    // consecutive columns. (8 bytes each take twice as long: 67 MB of bf16 in 21 us, as long as 134 MB of f32.)
     __device__ __forceinline__ void finish() {
-        constexpr int COLS = FN * 16, STRIDE = COLS + 4, LANES = FN * 4, ROWS = 64 / LANES;
+        constexpr int W = OUT <= OUT_TYPE ? Elem<T>::V : 4;
+        constexpr int COLS = FN * 16, STRIDE = COLS + 4, LANES = COLS / W, ROWS = 64 / LANES;
         static_assert(WM * WN * 16 * STRIDE * 4 <= 2 * BYTES, "the waves' strips fit the tiles' LDS");
-        __syncthreads();
+        typedef Cols<T, W> Row;
         float *strip = (float *)lds + (wm * WN + wn) * 16 * STRIDE;
-        const int n = n0 + wn * COLS + (lane % LANES) * 4;
+        const int n = n0 + wn * COLS + (lane % LANES) * W;
         // the residual's loads go ahead of everything, as far as registers allow: in turn with the stores (which may go to
         // the same buffer) each would wait for memory
         constexpr int PASSES = 16 / ROWS, AHEAD = FM <= 4 ? FM : 1;
-        typename Elem<T>::quad res[AHEAD][PASSES];
+        typename Row::vec res[AHEAD][PASSES];
         const auto ahead = [&](int j) {
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
                 const int m = m0 + (wm * FM + j) * 16 + i * ROWS + lane / LANES;
-                if (m < P.m && n < P.n) res[j % AHEAD][i] = residual4<T, OUT>(P.e, m, n, P.n - n);
+                if (m < P.m && n < P.n) res[j % AHEAD][i] = residual_at<T, OUT, W>(P.e, m, n, P.n - n);
             }
         };
         if (AHEAD > 1)
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) ahead(j);
+        const typename Row::sums bias = bias_at<OUT, W>(P.e, n, P.n - n);
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < FM; j++) {
             if (AHEAD == 1) ahead(j);
@@ -417,12 +430,18 @@ struct Mm {
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
                 const int r = i * ROWS + lane / LANES, m = m0 + (wm * FM + j) * 16 + r;
-                const v4f v = *(const v4f *)(strip + r * STRIDE + (lane % LANES) * 4);
+                typename Row::sums v;
+#pragma unroll
+                for (int q = 0; q < W; q += 4) {
+                    const v4f x = *(const v4f *)(strip + r * STRIDE + (lane % LANES) * W + q);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) v[q + c] = x[c];
+                }
                 if (m >= P.m || n >= P.n) continue;
                 if constexpr (OUT == OUT_PART)
                     *(v4f *)(P.part + ((size_t)split * P.m + m) * P.part_ld + n) = v;  // (part_ld: a multiple of 4)
                 else
-                    finish4<T, OUT>(P.e, m, n, P.n - n, v, res[j % AHEAD][i]);
+                    finish_at<T, OUT, W>(P.e, m, n, P.n - n, v, bias, res[j % AHEAD][i]);
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -484,7 +503,7 @@ __device__ __forceinline__ void mm_direct(const Product &P, int wg, int wgs, cha
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + (mm.tid & ~63) * 16);
     // the filled tile to be sent for next: its summand, its number in there, its first elements
     int pass = p0, at = 0;
-    if (quick) pass += t0 / full, at = t0 % full;
+    if (t0) pass += t0 / full, at = t0 % full;  // (t0 > 0: so is full)
     const char *pa = M::SA::first(mm.a, pass, mm.m0, at * M::BK), *pb = M::SB::first(mm.b, pass, mm.n0, at * M::BK);
     const size_t step_a = M::SA::step(P.a), step_b = M::SB::step(P.b);
     const auto send = [&](int q, int buf) {  // chunk q of both operands' NA + NB
@@ -596,7 +615,7 @@ __global__ __launch_bounds__(256) void affine_join(Product P) {
     add(0, lifted);
     if (P.lift) v *= 1.0f / F16_LIFT;
     add(lifted, P.splits);
-    finish4<T, OUT>(P.e, m, n, P.n - n, v, residual4<T, OUT>(P.e, m, n, P.n - n));
+    finish_at<T, OUT, 4>(P.e, m, n, P.n - n, v, bias_at<OUT, 4>(P.e, n, P.n - n), residual_at<T, OUT, 4>(P.e, m, n, P.n - n));
 }
 
 // What a product needs made before it, in one launch: copies of matrices, and gz.
@@ -814,7 +833,8 @@ __global__ __launch_bounds__(few_threads(R)) void affine_few(const TW *__restric
     if (r >= batch || col >= out) return;
     v4f v = {0, 0, 0, 0};
     for (int i = 0; i < NT / 64; i++) v += *(const v4f *)&red[i][r][q];
-    finish4<T, OUT_LAYER>(e, r, col, out - col, v, residual4<T, OUT_LAYER>(e, r, col, out - col));
+    finish_at<T, OUT_LAYER, 4>(e, r, col, out - col, v, bias_at<OUT_LAYER, 4>(e, col, out - col),
+                               residual_at<T, OUT_LAYER, 4>(e, r, col, out - col));
 }
 
 // ---- host side
