@@ -271,7 +271,8 @@ int bt_faux_quantise(void *stream, const float *x, float *y, size_t n, float val
  * more. Matrices are row-major with a leading dimension in elements (rows `ld` apart, ld >= width); elements between two
  * rows are neither used nor written. Buffers need the alignment of their element type only; 16-byte aligned buffers with
  * leading dimensions that are multiples of 16 bytes are faster. All calls are enqueue-only on `stream`, allocate nothing
- * and may be captured into a graph. Results are the same from run to run.
+ * and may be captured into a graph. Results are the same from run to run. A workspace need not be cleared, and holds nothing
+ * between calls; calls that may run at the same time (on two streams, or replayed from two graphs) need one each.
  * ------------------------------------------------------------------------------------------ */
 enum { BT_TYPE_F32 = 0, BT_TYPE_BF16 = 1, BT_TYPE_F16 = 2 };
 
