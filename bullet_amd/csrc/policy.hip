@@ -249,7 +249,7 @@ __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, con
         g.shift = (float)(dl + kl);
     }
     loss = (float)(w * ((double)d.kl_weight * kl - (free_gain != free_gain ? free_gain : fmin(free_gain, held_gain))));
-    g.top = st.top;
+    g.top = st.top == NEG_INF ? 0.0f : st.top;  // (nothing but NaN)
     const float inv = 1.0f / st.sum;
     g.ce = -(float)(w * slope) * inv;
     g.ck = (float)ck * inv;
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
     st.sum = Group<G>::sum(s, red);
     st.ref_sum = FULL ? Group<G>::sum(sq, red) : 1.0f;
     st.cross = FULL ? Group<G>::sum(cross, red) : 0.0f;
-    const bool counted = pr.counted && st.top > NEG_INF;
+    const bool counted = pr.counted && st.sum != 0.0f;  // (0: nothing above -infinity; NaN counts)
 
     T *grad = a.grad ? (T *)a.grad + (size_t)row * a.d.ld : nullptr;
     if (!counted) {
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
     st.ref_top = FULL ? Group<256>::max(ref_top, red) : 0.0f;
     st.ref_sum = FULL ? Group<256>::sum(ref_top == NEG_INF ? sq : sq * exp_neg(ref_top - st.ref_top), red) : 1.0f;
     st.cross = FULL ? Group<256>::sum(top == NEG_INF ? cross : cross * f, red) : 0.0f;
-    const bool counted = pr.counted && st.top > NEG_INF;
+    const bool counted = pr.counted && st.sum != 0.0f;  // (0: nothing above -infinity; NaN counts)
     T *grad = a.grad ? (T *)a.grad + (size_t)row * a.d.ld : nullptr;
     RowGrad g;
     double logp = 0.0, kl = 0.0;
@@ -563,8 +563,8 @@ __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
     }
     if (lane == 0) {
         a.za[row] = za;
-        a.top[row] = top;
-        a.sum[row] = can && top > NEG_INF ? s : 0.0f;
+        a.top[row] = top == NEG_INF ? 0.0f : top;  // (nothing, or nothing but NaN)
+        a.sum[row] = can ? s : 0.0f;
     }
 }
 

@@ -316,7 +316,7 @@ int bt_affine_backward(void *stream, const bt_affine_desc *desc, const void *w, 
  *                and mask as `logits` (lref: their log-softmax over the legal moves); no gradient goes into it
  * mask: U8[batch*mask_ld], non-zero = legal, or NULL = every move is legal. What stands in masked places (infinities, NaN)
  * has no effect. actions: I32[batch]. A row is not counted (loss, gradient, row outputs all exactly 0) if its action is
- * outside [0, width) (-1 marks padding), is masked, or if no legal logit is above -infinity. grad of masked places is 0.
+ * outside [0, width) (-1 marks padding), is masked, or if every legal logit is -infinity. grad of masked places is 0.
  * The gradient passes where r A is not above its clipped value. NaN or +infinity in a legal place makes its row's loss NaN,
  * and so do reference logits that leave a counted row nothing above -infinity.
  * row_weights F32[batch] or NULL = 1. Outputs: loss_sum F32[1] (overwritten, un-normalised, as bt_loss); grad (type and

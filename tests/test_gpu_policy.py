@@ -187,6 +187,29 @@ def test_policy_nan_stays_in_its_row():
     assert np.isnan(loss.item()) and np.isfinite(grad.cpu().numpy()[~bad]).all()
 
 
+@pytest.mark.parametrize("width", [5, 50, 4100, 9000])
+@pytest.mark.parametrize("kl", ["none", "taken", "full"])
+def test_policy_rows_of_nothing_but_nan(kl, width):
+    """a head that has diverged: its rows' losses are NaN, not the 0 of a row without moves; masked places keep gradient 0"""
+    z = np.full((3, width), np.nan, np.float32)
+    mask = np.zeros((3, width), np.uint8)
+    mask[:, 1::2] = 1
+    z[1] = 0.0
+    z[2] = -np.inf
+    for m in (None, mask):
+        rows = [torch.zeros(3, device="cuda") for _ in range(3)]
+        loss, grad = torch.zeros(1, device="cuda"), torch.full((3, width), 9.0, device="cuda")
+        ref = None if kl == "none" else dev(np.full(3, -1.0), np.float32) if kl == "taken" else torch.zeros(3, width, device="cuda")
+        pr.call_policy(stream(), pr.policy_desc(3, width, "f32", kl=kl), dev(z), dev(m), dev(np.full(3, 3), np.int32),
+                       dev(np.full(3, -1.0), np.float32), dev(np.ones(3), np.float32), ref, None, loss, grad, *rows)
+        g = grad.cpu().numpy()
+        for t in rows[:2]:
+            assert np.isnan(t[0].item()) and np.isfinite(t[1].item()) and t[2].item() == 0
+        assert np.isnan(loss.item()) and np.isfinite(g[1]).all() and (g[2] == 0).all()
+        legal = np.ones(width, bool) if m is None else m[0] != 0
+        assert np.isnan(g[0, legal]).all() and (g[0, ~legal] == 0).all()
+
+
 def test_policy_ratio_next_to_the_clipping_border():
     """ratios within a few 2^-24 of the border: which side they are on decides the whole gradient of the row"""
     rng = np.random.default_rng(17)
@@ -313,6 +336,28 @@ def test_preference_extreme_margins():
     want, tol = pr.preference(zt.double().cpu().numpy(), None, actions, offsets, ref, None, 0.1, 0.05)
     for name, t in (("loss", loss), ("pair_loss", pl), ("grad", grad)):
         pr.check(t.cpu().numpy(), want[name], tol[name], "f32", name)
+
+
+@pytest.mark.parametrize("width", [5, 50, 4100, 20001])
+def test_preference_rows_of_nothing_but_nan(width):
+    """such a row makes its pair's loss and gradients NaN, and no other's"""
+    n, offsets = 5, np.array([0, 1, 2, 3, 5], np.int32)
+    z = np.zeros((n, width), np.float32)
+    z[1] = np.nan
+    z[4] = -np.inf  # a row without a move in the other pair
+    mask = np.zeros((n, width), np.uint8)
+    mask[:, 1::2] = 1
+    d = pr.preference_desc(2, n, width, "f32")
+    ws = torch.empty(lib.load().bt_preference_loss_workspace_bytes(C.byref(d)), dtype=torch.uint8, device="cuda")
+    pair, line = torch.zeros(2, device="cuda"), torch.zeros(4, device="cuda")
+    loss, grad = torch.zeros(1, device="cuda"), torch.full((n, width), 9.0, device="cuda")
+    pr.call_preference(stream(), d, dev(z), dev(mask), dev(np.full(n, 3), np.int32), dev(offsets), torch.zeros(4, device="cuda"),
+                       None, loss, grad, pair, line, ws)
+    g, legal = grad.cpu().numpy(), mask[0] != 0
+    assert np.isnan(pair.cpu().numpy()).tolist() == [True, False] and np.isnan(loss.item())
+    assert np.isnan(line.cpu().numpy()).tolist() == [False, True, False, False]
+    assert np.isnan(g[:2][:, legal]).all() and (g[:, ~legal] == 0).all()
+    assert np.isfinite(g[2:]).all() and (g[4] == 0).all()
 
 
 def test_preference_offsets_out_of_range_are_clamped():
