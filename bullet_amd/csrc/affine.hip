@@ -261,6 +261,12 @@ __device__ __forceinline__ uint32_t lds_address(const char *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
 }
 
+// between a wave's writes to LDS and its own lanes' reads of them, which the hardware takes in order
+__device__ __forceinline__ void lds_turn() {
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // One operand's tiles on their way into LDS, for a workgroup of NT threads.
 template <typename T, bool KC, int SPAN, int NT>
 struct Stage {
@@ -426,7 +432,7 @@ struct Mm {
             if (AHEAD == 1) ahead(j);
 #pragma unroll
             for (int i = 0; i < FN; i++) *(v4f *)(strip + (lane & 15) * STRIDE + i * 16 + (lane >> 4) * 4) = acc[i][j];
-            __builtin_amdgcn_wave_barrier();
+            lds_turn();
 #pragma unroll
             for (int i = 0; i < PASSES; i++) {
                 const int r = i * ROWS + lane / LANES, m = m0 + (wm * FM + j) * 16 + r;
@@ -443,7 +449,7 @@ struct Mm {
                 else
                     finish_at<T, OUT, W>(P.e, m, n, P.n - n, v, bias, res[j % AHEAD][i]);
             }
-            __builtin_amdgcn_wave_barrier();
+            lds_turn();
         }
     }
 };
@@ -609,7 +615,7 @@ __global__ __launch_bounds__(256, 2) void affine_mm_both(Product W, Product X, i
 // 5.8 TB/s.
 template <typename T, int OUT>
 __global__ __launch_bounds__(256) void affine_join(Product P) {
-    const long long q = (long long)blockIdx.x * 256 + threadIdx.x, cols = P.part_ld / 4;
+    const long long q = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x, cols = P.part_ld / 4;
     if (q >= cols * P.m) return;
     const int m = (int)(q / cols), n = (int)(q % cols) * 4;
     v4f v = {0, 0, 0, 0};
@@ -726,7 +732,7 @@ __device__ __forceinline__ void gz_block(const Gz<T> &G, int block) {
                 for (int p = 0; p < NP; p++) {
                     part[p][j] = (T)rest;
                     rest = (rest - (float)part[p][j]) * LIFT;
-                    if (rest != rest) rest = 0.0f;  // (an infinite gradient stays one)
+                    if (!(fabsf(rest) < __builtin_huge_valf())) rest = 0.0f;  // (an infinite gradient stays one)
                 }
             }
             if (G.p[0]) {
@@ -862,7 +868,10 @@ int validate(const bt_affine_desc *d, const char *fn) {
     BT_REQUIRE(d->w_ld >= d->out && d->x_ld >= d->in && d->y_ld >= d->out,
                "%s: Mismatched sizes! (a leading dimension is less than its row: w %d / %d, x %d / %d, y %d / %d)", fn, d->w_ld,
                d->out, d->x_ld, d->in, d->y_ld, d->out);
-    BT_REQUIRE(d->batch <= (1 << 30) && d->in <= (1 << 30) && d->out <= (1 << 30), "%s: Mismatched sizes! (too large)", fn);
+    // (each matrix is less than 2^36 elements, so that numbers of tiles, chunks and rows of partial sums fit 32 bits)
+    const long long b = d->batch, i = d->in, o = d->out, most = 1ll << 36;
+    BT_REQUIRE(b <= (1 << 30) && i <= (1 << 30) && o <= (1 << 30) && b * i <= most && b * o <= most && i * o <= most,
+               "%s: Mismatched sizes! (too large)", fn);
     return BT_OK;
 }
 
@@ -901,6 +910,12 @@ Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false) {
     return best;
 }
 
+// a launch holds less than 2^32 threads a dimension: many workgroups fold into the grid's second one
+dim3 folded(long long blocks) {
+    constexpr long long W = 1 << 22;
+    return dim3((unsigned)(blocks < W ? blocks : W), (unsigned)((blocks + W - 1) / W));
+}
+
 // the tile sizes shape_of chooses from, with or without direct loads
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
 int mm_launch(hipStream_t st, const Product &P, bool direct) {
@@ -933,7 +948,7 @@ void set_shape(Product &P, const Shape &s) {
 }
 template <typename T, int OUT>
 int join_launch(hipStream_t st, const Product &P) {
-    BT_LAUNCH(BTK_AFFINE, st, (affine_join<T, OUT>), dim3(bt_div_up(P.part_ld / 4 * P.m, 256)), dim3(256), 0, P);
+    BT_LAUNCH(BTK_AFFINE, st, (affine_join<T, OUT>), folded(bt_div_up(P.part_ld / 4 * P.m, 256)), dim3(256), 0, P);
     BT_LAUNCH_CHECK();
     return BT_OK;
 }
@@ -1009,9 +1024,7 @@ template <typename T>
 int prepare_launch(hipStream_t st, const Prepare<T> &p, int np) {
     const long long blocks = (long long)p.w.blocks + p.x.blocks + p.gz.blocks;
     if (blocks == 0) return BT_OK;
-    // (a launch holds less than 2^32 threads a dimension)
-    constexpr long long W = 1 << 22;
-    const dim3 grid((unsigned)(blocks < W ? blocks : W), (unsigned)((blocks + W - 1) / W)), block(256);
+    const dim3 grid = folded(blocks), block(256);
     if (p.gz.blocks == 0)
         BT_LAUNCH(BTK_AFFINE, st, (affine_prepare<T, 0>), grid, block, 0, p);
     else if (np == 1)

@@ -43,6 +43,23 @@ def test_shapes_are_refused(change, message):
     assert L().bt_affine_backward_workspace_bytes(C.byref(d)) == 0 and message in L().bt_last_error()
 
 
+@pytest.mark.parametrize("batch,in_,out", [(1 << 30, 1, 1 << 20), (1 << 30, 1 << 30, 1), (1, 1 << 30, 1 << 30), (1 << 30,) * 3])
+def test_matrices_beyond_any_memory_are_refused(batch, in_, out):
+    d = ar.desc(batch, in_, out, "bf16", "relu")
+    for size in (L().bt_affine_forward_workspace_bytes, L().bt_affine_backward_workspace_bytes):
+        assert size(C.byref(d)) == 0 and b"too large" in L().bt_last_error()
+    assert fwd(d) == 1 and bwd(d) == 1 and b"too large" in L().bt_last_error()
+
+
+@pytest.mark.parametrize("batch,in_,out", [(1 << 30, 64, 64), (64, 1 << 30, 64), (64, 64, 1 << 30), (1 << 18,) * 3])
+def test_workspaces_of_the_largest_matrices(batch, in_, out):
+    """what is taken has a workspace, of at most the matrices' own bytes and 32 of f32 partial sums of either product"""
+    d = ar.desc(batch, in_, out, "f16", "screlu", w32=True)
+    mats = batch * in_ + batch * out + in_ * out
+    for size in (L().bt_affine_forward_workspace_bytes, L().bt_affine_backward_workspace_bytes):
+        assert 0 < size(C.byref(d)) <= 33 * 4 * mats * 2
+
+
 @pytest.mark.parametrize("args,message", [
     (dict(w=None), b"null pointer"), (dict(x=None), b"null pointer"), (dict(y=None), b"null pointer"),
     (dict(w=258), b"not aligned"), (dict(x=770), b"not aligned"), (dict(y=1281), b"not aligned"), (dict(res=1025), b"not aligned"),
