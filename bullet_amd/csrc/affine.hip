@@ -601,14 +601,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT>(P, blockIdx.x, gridDim.x, lds);
 }
 // dW and grad_x of a small layer in one launch: neither has tiles enough to fill the chip, or to hide its own latency
-// (200 x 512 -> 333 f32: 11 us, 91 workgroups that each walk their whole k)
-template <typename T, int OUT_W, int OUT_X>
+// (200 x 512 -> 333 f32: 8 us, 288 workgroups of 32 x 32 that each walk their whole k; 76 of 64 x 64: 11)
+template <typename T, int B, int OUT_W, int OUT_X>
 __global__ __launch_bounds__(256, 2) void affine_mm_both(Product W, Product X, int wgs) {  // wgs: W's
     extern __shared__ __align__(1024) char lds[];
     if ((int)blockIdx.x < wgs)
-        mm_direct<T, 64, 64, 2, 2, false, false, OUT_W>(W, blockIdx.x, wgs, lds);
+        mm_direct<T, B, B, 2, 2, false, false, OUT_W>(W, blockIdx.x, wgs, lds);
     else
-        mm_direct<T, 64, 64, 2, 2, true, true, OUT_X>(X, blockIdx.x - wgs, gridDim.x - wgs, lds);
+        mm_direct<T, B, B, 2, 2, true, true, OUT_X>(X, blockIdx.x - wgs, gridDim.x - wgs, lds);
 }
 
 // The splits' sums added in order, then the epilogue. Memory bound: 4 splits of 2048 x 2048 (67 MB of sums, 8 MB out) 13 us,
@@ -877,34 +877,38 @@ int validate(const bt_affine_desc *d, const char *fn) {
 
 struct Shape {
     int bm, tiles_m, tiles_n, splits;
+    double us;  // the estimate
     size_t part_bytes(int m, int n) const { return splits > 1 ? bt_align((size_t)splits * m * ((n + 3) / 4 * 4) * 4) : 0; }
 };
 // Tile size and number of workgroups that share a tile's k: the pair whose estimate is lowest. Measured, in us for one
 // tile and 128 bytes of k: alone on its CU, and per workgroup where a CU has several (256 x 256: never more than one).
-//            256        128           64
-//   16-bit   1.75       0.70, 0.48    0.33, 0.18
-//   f32                 2.30, 2.10    0.53, 0.50
+//            256        128           64            32
+//   16-bit   1.75       0.70, 0.48    0.33, 0.18    (waits for memory, not for the matrix cores: nothing to gain)
+//   f32                 2.30, 2.10    0.53, 0.50    0.26, 0.17    (128: never better than four of 64, so not built)
 // and for sharing k a launch (4 us) and the partial sums' way through memory (7 TB/s). What this decides, measured both ways
 // (bf16): dW of 16384 x 2048 -> 2048 takes 113 us as 256 / 4, 123 as 128 / 2, 151 as 128 / 1; 4096 x 1024 -> 1024 forward
-// 15.3 us as 64 / 1, 24.8 as 128 / 2, 29.1 as 256 / 1; dW of 8192 x 1024 -> 1880 40.5 us as 128 / 4, 85 as 128 / 1.
-Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false) {
-    const struct {
+// 15.3 us as 64 / 1, 24.8 as 128 / 2, 29.1 as 256 / 1; dW of 8192 x 1024 -> 1880 40.5 us as 128 / 4, 85 as 128 / 1. And of f32,
+// forward: 512 x 512 -> 512 7.3 us as 32 / 1, 10.9 as 64 / 2; 4096 x 1024 -> 1024 66 us as 64 / 1, 78 as 32 / 1.
+Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false, int only = 0) {
+    struct Cost {
         int b;
         double alone, busy;
-    } tiles[] = {{256, 1.75, 1.75}, {128, es == 2 ? 0.70 : 2.30, es == 2 ? 0.48 : 2.10}, {64, es == 2 ? 0.33 : 0.53, es == 2 ? 0.18 : 0.50}};
+    };
+    static const Cost of_2[] = {{256, 1.75, 1.75}, {128, 0.70, 0.48}, {64, 0.33, 0.18}};
+    static const Cost of_4[] = {{64, 0.53, 0.50}, {32, 0.26, 0.17}};
     const long long ktiles = (long long)bt_div_up(k, (int)(128 / es)) * passes;
     Shape best = {};
-    double best_us = 0.0;
-    for (const auto &t : tiles) {
-        if (t.b == 256 && es == 4) continue;
+    for (int i = 0; i < (es == 2 ? 3 : 2); i++) {
+        const Cost &t = es == 2 ? of_2[i] : of_4[i];
+        if (only && t.b != only) continue;
         const long long count = (long long)bt_div_up(m, t.b) * bt_div_up(n, t.b);
         for (int splits = lift ? 2 : 1; splits <= 32; splits += lift || splits >= 4 ? 2 : 1) {
             if (splits > 1 && !lift && ktiles / splits < 2) break;
             const double each = (double)((ktiles + splits - 1) / splits), per_cu = (double)((count * splits + 255) / 256);
             double us = each * (per_cu * t.busy > t.alone ? per_cu * t.busy : t.alone);
             if (splits > 1) us += 4.0 + splits * (double)m * n * 8.0 / 7.0e6;
-            if (best.bm == 0 || us < best_us)
-                best = Shape{t.b, bt_div_up(m, t.b), bt_div_up(n, t.b), splits}, best_us = us;
+            if (best.bm == 0 || us < best.us)
+                best = Shape{t.b, bt_div_up(m, t.b), bt_div_up(n, t.b), splits, us};
         }
     }
     return best;
@@ -937,9 +941,12 @@ int mm_launch(hipStream_t st, const Product &P, bool direct) {
 }
 template <typename T, bool AK, bool BKC, int OUT>
 int tile_launch(hipStream_t st, const Product &P, const Shape &s, bool direct) {
-    if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2) {
         if (s.bm == 256) return mm_launch<T, 256, 256, 2, 4, AK, BKC, OUT>(st, P, direct);
-    if (s.bm == 128) return mm_launch<T, 128, 128, 2, 2, AK, BKC, OUT>(st, P, direct);
+        if (s.bm == 128) return mm_launch<T, 128, 128, 2, 2, AK, BKC, OUT>(st, P, direct);
+    } else {
+        if (s.bm == 32) return mm_launch<T, 32, 32, 2, 2, AK, BKC, OUT>(st, P, direct);
+    }
     return mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT>(st, P, direct);
 }
 void set_shape(Product &P, const Shape &s) {
@@ -962,26 +969,32 @@ int product_launch(hipStream_t st, Product &P, Shape s) {
     return join_launch<T, OUT>(st, P);
 }
 // both products of a backward pass, each with its sums in a place of its own
-template <typename T, int OUT_W, int OUT_X>
+template <typename T, int B, int OUT_W, int OUT_X>
 int both_launch(hipStream_t st, const Product &W, const Product &X) {
     const long long w = (long long)W.tiles_m * W.tiles_n * W.splits + W.bias.blocks, x = (long long)X.tiles_m * X.tiles_n * X.splits;
     BT_REQUIRE((w + x) * 256 < (1ll << 32), "bt_affine_backward: Mismatched sizes! (%lld tiles)", w + x);
-    const size_t lds_w = 2 * Mm<T, 64, 64, 2, 2, false, false, OUT_W>::BYTES, lds_x = 2 * Mm<T, 64, 64, 2, 2, true, true, OUT_X>::BYTES;
+    const size_t lds_w = 2 * Mm<T, B, B, 2, 2, false, false, OUT_W>::BYTES, lds_x = 2 * Mm<T, B, B, 2, 2, true, true, OUT_X>::BYTES;
     static_assert(lds_w == lds_x, "tiles of one size");
-    BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, OUT_W, OUT_X>), dim3((unsigned)(w + x)), dim3(256), lds_w, W, X, (int)w);
+    BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, B, OUT_W, OUT_X>), dim3((unsigned)(w + x)), dim3(256), lds_w, W, X, (int)w);
     BT_LAUNCH_CHECK();
     return BT_OK;
 }
-template <typename T>
-int both_products(hipStream_t st, Product &W, const Shape &sw, Product &X, const Shape &sx) {
-    set_shape(W, sw), set_shape(X, sx);
-    const bool pw = sw.splits > 1, px = sx.splits > 1;
-    if (int rc = pw ? (px ? both_launch<T, OUT_PART, OUT_PART>(st, W, X) : both_launch<T, OUT_PART, OUT_TYPE>(st, W, X))
-                    : (px ? both_launch<T, OUT_F32, OUT_PART>(st, W, X) : both_launch<T, OUT_F32, OUT_TYPE>(st, W, X)))
+template <typename T, int B>
+int both_of(hipStream_t st, const Product &W, const Product &X) {
+    const bool pw = W.splits > 1, px = X.splits > 1;
+    if (int rc = pw ? (px ? both_launch<T, B, OUT_PART, OUT_PART>(st, W, X) : both_launch<T, B, OUT_PART, OUT_TYPE>(st, W, X))
+                    : (px ? both_launch<T, B, OUT_F32, OUT_PART>(st, W, X) : both_launch<T, B, OUT_F32, OUT_TYPE>(st, W, X)))
         return rc;
     if (pw)
         if (int rc = join_launch<T, OUT_F32>(st, W)) return rc;
     return px ? join_launch<T, OUT_TYPE>(st, X) : BT_OK;
+}
+template <typename T>
+int both_products(hipStream_t st, Product &W, const Shape &sw, Product &X, const Shape &sx) {
+    set_shape(W, sw), set_shape(X, sx);
+    if constexpr (sizeof(T) == 4)
+        if (sw.bm == 32) return both_of<T, 32>(st, W, X);
+    return both_of<T, 64>(st, W, X);
 }
 
 long long padded(int n, size_t es) { return (n + (128 / es) - 1) / (128 / es) * (128 / es); }  // rows on 128 bytes
@@ -1120,11 +1133,19 @@ BackwardPlan backward_plan(const bt_affine_desc *d) {
     p.ranges = bt_div_up(d->batch, p.range);
     p.dw = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift);
     p.dx = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift);
+    if (p.dw.bm <= 64 && p.dx.bm <= 64 && p.dw.bm != p.dx.bm) {  // one launch: tiles of one size, whichever serves both better
+        const Shape w = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift, p.dx.bm);
+        const Shape x = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift, p.dw.bm);
+        if (w.us + p.dx.us < p.dw.us + x.us)
+            p.dw = w;
+        else
+            p.dx = x;
+    }
     p.w_bytes = copy_bytes(copy_w(d), d->in, d->out, es), p.x_bytes = copy_bytes(copy_x(d), d->batch, d->in, es);
     p.gz_bytes = p.gz ? bt_align((size_t)d->batch * padded(d->out, es) * es) : 0;
     p.sum_bytes = bt_align((size_t)p.ranges * d->out * 4);
     const size_t a = p.dw.part_bytes(d->in, d->out), b = p.dx.part_bytes(d->batch, d->in);
-    p.both = p.dw.bm == 64 && p.dx.bm == 64;
+    p.both = p.dw.bm <= 64 && p.dx.bm <= 64;
     p.part_dx = p.both ? a : 0;
     p.part_bytes = p.both ? a + b : a > b ? a : b;
     p.total = p.w_bytes + p.x_bytes + p.gz_bytes * p.np_dw + p.sum_bytes + p.part_bytes;
@@ -1176,7 +1197,7 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
         X.e.out = gx, X.e.ld = d->x_ld, X.e.alpha = p.alpha;
     }
     (dw ? W : X).bias = bias;
-    // one launch where both take the smallest tiles: 200 x 512 -> 333 f32 23 us in two, 14 in one
+    // one launch where both take the smaller tiles (200 x 512 -> 333 f32 with 64 x 64 tiles: 23 us in two, 14 in one)
     if (dw && gx && p.both && W.a.aligned && W.b.aligned && X.a.aligned && X.b.aligned)
         return both_products<T>(st, W, p.dw, X, p.dx);
     if (dw)
