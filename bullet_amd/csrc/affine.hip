@@ -251,12 +251,17 @@ struct Product {
 };
 
 // A chunk straight from memory into LDS, 16 bytes a lane: lane l's lands 16 l bytes behind `lds` (the same in all lanes).
-// Written out, since the compiler lets every LDS read wait for all such loads of its own; wait_loads() is the wait, in
-// front of the barrier behind which the chunk is read. The s_nop is the wait state between m0 and its use.
+// Written out, since the compiler lets every LDS read wait for all such loads of its own; wait_loads() is the wait (for all but
+// the N youngest loads), in front of the barrier behind which the chunk is read. The s_nop is the wait state between m0 and
+// its use.
 __device__ __forceinline__ void to_lds(const char *base, uint32_t offset, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" : : "v"(offset), "s"(lds), "s"(base) : "memory");
 }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+template <int N = 0>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64, "what the counter holds");
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_address(const char *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
 }
@@ -347,7 +352,7 @@ struct Mm {
     typedef Tile<T, BKC, BN> TB;
     typedef Stage<T, AK, BM, NT> SA;
     typedef Stage<T, BKC, BN, NT> SB;
-    static constexpr int BYTES = TA::BYTES + TB::BYTES;  // of one of the two buffers
+    static constexpr int BYTES = TA::BYTES + TB::BYTES;  // of one buffer
     typedef typename Elem<T>::frag frag;
     const Product &P;
     const Operand a, b;
@@ -485,8 +490,8 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 
 // Operands whose chunks start on 16 bytes: tiles go straight into LDS, and three things are under way at any time. While
 // the first half of a tile's k is multiplied the second half's fragments are read; behind the barrier that says that the
-// next tile has arrived its first fragments are read, and the tile after it is sent for into the buffer just left, while
-// the second half is multiplied. Each fragment's products carry their share of those reads and loads.
+// next tile has arrived its first fragments are read, and another tile is sent for into the buffer just left, while the
+// second half is multiplied. Each fragment's products carry their share of those reads and loads.
 // The tiles that k fills come first; the others, one of each summand (the rest of k; the last full one, where its last row
 // must not be read to the end of a chunk), take the same way with a check of every chunk.
 //
@@ -495,7 +500,7 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 // 64 x 64 one 1024. 16384 x 2048 -> 4096 bf16 takes 234 us, 1.17 PFLOP/s (the MFMA units are busy 55 % of the clocks, bank
 // conflicts are few); dW of 16384 x 2048 -> 2048 with 4 workgroups to a tile 113 us and grad_x 109, 1.2 and 1.26 PFLOP/s;
 // 4096 x 1024 -> 1024 f32 with 64 x 64 tiles 65 us, 132 TFLOP/s, 83 % of the rate of f32.
-template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
 __device__ __forceinline__ void mm_direct(const Product &P, int wg, int wgs, char *lds) {
     typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
     typedef typename M::frag frag;
@@ -558,7 +563,7 @@ __device__ __forceinline__ void mm_direct(const Product &P, int wg, int wgs, cha
     const std::integral_constant<int, 1> one;
     if (tiles > 0) {
 #pragma unroll 1
-        for (int t = 0; t < 2 && t < tiles; t++) {
+        for (int t = 0; t < BUFS && t < tiles; t++) {
             if (t < quick) {
 #pragma unroll
                 for (int q = 0; q < NA + NB; q++) send(q, t);
@@ -566,49 +571,51 @@ __device__ __forceinline__ void mm_direct(const Product &P, int wg, int wgs, cha
             } else {
                 careful(t, t);
             }
-            if (t == 0) {
-                wait_loads();
-                __syncthreads();
-            }
         }
+        if (quick >= BUFS)
+            wait_loads<(BUFS - 1) * (NA + NB)>();
+        else
+            wait_loads();
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < FM; j++) fa[j] = mm.read_a(0, j, 0);
 #pragma unroll
         for (int i = 0; i < FN; i++) fb[0][i] = mm.read_b(0, i, 0);
     }
     int t = 0, cur = 0;
-    for (; t + 2 < quick; t++, cur ^= 1) {
+    const auto next = [&]() { return BUFS == 2 ? cur ^ 1 : cur == BUFS - 1 ? 0 : cur + 1; };
+    for (; t + BUFS < quick; t++, cur = next()) {
         half(one, std::false_type(), cur, 0);
-        wait_loads();
+        wait_loads<(BUFS - 2) * (NA + NB)>();
         __syncthreads();  // the next tile is here, and every wave has read this one
-        half(zero, std::true_type(), cur ^ 1, cur);
+        half(zero, std::true_type(), next(), cur);
         advance();
     }
 #pragma unroll 1
-    for (; t < tiles; t++, cur ^= 1) {
+    for (; t < tiles; t++, cur = next()) {
         half(one, std::false_type(), cur, 0);
         wait_loads();
         __syncthreads();
-        if (t + 2 < tiles) careful(t + 2, cur);
-        half(zero, std::false_type(), cur ^ 1, 0);  // (behind the last tile: fragments that nothing uses)
+        if (t + BUFS < tiles) careful(t + BUFS, cur);
+        half(zero, std::false_type(), next(), 0);  // (behind the last tile: fragments that nothing uses)
     }
     mm.finish();
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     extern __shared__ __align__(1024) char lds[];
-    mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT>(P, blockIdx.x, gridDim.x, lds);
+    mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT, BUFS>(P, blockIdx.x, gridDim.x, lds);
 }
 // dW and grad_x of a small layer in one launch: neither has tiles enough to fill the chip, or to hide its own latency
 // (200 x 512 -> 333 f32: 8 us, 288 workgroups of 32 x 32 that each walk their whole k; 76 of 64 x 64: 11)
-template <typename T, int B, int OUT_W, int OUT_X>
+template <typename T, int B, int OUT_W, int OUT_X, int BUFS>
 __global__ __launch_bounds__(256, 2) void affine_mm_both(Product W, Product X, int wgs) {  // wgs: W's
     extern __shared__ __align__(1024) char lds[];
     if ((int)blockIdx.x < wgs)
-        mm_direct<T, B, B, 2, 2, false, false, OUT_W>(W, blockIdx.x, wgs, lds);
+        mm_direct<T, B, B, 2, 2, false, false, OUT_W, BUFS>(W, blockIdx.x, wgs, lds);
     else
-        mm_direct<T, B, B, 2, 2, true, true, OUT_X>(X, blockIdx.x - wgs, gridDim.x - wgs, lds);
+        mm_direct<T, B, B, 2, 2, true, true, OUT_X, BUFS>(X, blockIdx.x - wgs, gridDim.x - wgs, lds);
 }
 
 // The splits' sums added in order, then the epilogue. Memory bound: 4 splits of 2048 x 2048 (67 MB of sums, 8 MB out) 13 us,
@@ -883,19 +890,20 @@ struct Shape {
 // Tile size and number of workgroups that share a tile's k: the pair whose estimate is lowest. Measured, in us for one
 // tile and 128 bytes of k: alone on its CU, and per workgroup where a CU has several (256 x 256: never more than one).
 //            256        128           64            32
-//   16-bit   1.75       0.70, 0.48    0.33, 0.18    (waits for memory, not for the matrix cores: nothing to gain)
-//   f32                 2.30, 2.10    0.53, 0.50    0.26, 0.17    (128: never better than four of 64, so not built)
-// and for sharing k a launch (4 us) and the partial sums' way through memory (7 TB/s). What this decides, measured both ways
-// (bf16): dW of 16384 x 2048 -> 2048 takes 113 us as 256 / 4, 123 as 128 / 2, 151 as 128 / 1; 4096 x 1024 -> 1024 forward
-// 15.3 us as 64 / 1, 24.8 as 128 / 2, 29.1 as 256 / 1; dW of 8192 x 1024 -> 1880 40.5 us as 128 / 4, 85 as 128 / 1. And of f32,
-// forward: 512 x 512 -> 512 7.3 us as 32 / 1, 10.9 as 64 / 2; 4096 x 1024 -> 1024 66 us as 64 / 1, 78 as 32 / 1.
+//   16-bit   1.75       0.58, 0.48    0.22, 0.18    (waits for memory, not for the matrix cores: nothing to gain)
+//   f32                 2.30, 2.10    0.52, 0.50    0.20, 0.17    (128: never better than four of 64, so not built)
+// and for sharing k a launch and the partial sums' way through memory (7 TB/s). What this decides, measured both ways, in us
+// with all launches: bf16 dW of 16384 x 2048 -> 2048 113 as 256 / 4, 123 as 128 / 2, 151 as 128 / 1; bf16 forward 2048 x 2048 ->
+// 2048 21.7 as 128 / 1, 27.3 as 64 / 1, 1024 x 1024 -> 1024 7.4 as 64 / 1, 12.9 as 128 / 4; f32 forward 512 x 512 -> 512 7.1 as
+// 32 / 1, 10.9 as 64 / 2, 4096 x 1024 -> 1024 66 as 64 / 1, 78 as 32 / 1.
+constexpr double LAUNCH_US = 4.0;
 Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false, int only = 0) {
     struct Cost {
         int b;
         double alone, busy;
     };
-    static const Cost of_2[] = {{256, 1.75, 1.75}, {128, 0.70, 0.48}, {64, 0.33, 0.18}};
-    static const Cost of_4[] = {{64, 0.53, 0.50}, {32, 0.26, 0.17}};
+    static const Cost of_2[] = {{256, 1.75, 1.75}, {128, 0.58, 0.48}, {64, 0.22, 0.18}};
+    static const Cost of_4[] = {{64, 0.52, 0.50}, {32, 0.20, 0.17}};
     const long long ktiles = (long long)bt_div_up(k, (int)(128 / es)) * passes;
     Shape best = {};
     for (int i = 0; i < (es == 2 ? 3 : 2); i++) {
@@ -906,7 +914,7 @@ Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false, in
             if (splits > 1 && !lift && ktiles / splits < 2) break;
             const double each = (double)((ktiles + splits - 1) / splits), per_cu = (double)((count * splits + 255) / 256);
             double us = each * (per_cu * t.busy > t.alone ? per_cu * t.busy : t.alone);
-            if (splits > 1) us += 4.0 + splits * (double)m * n * 8.0 / 7.0e6;
+            if (splits > 1) us += LAUNCH_US + splits * (double)m * n * 8.0 / 7.0e6;
             if (best.bm == 0 || us < best.us)
                 best = Shape{t.b, bt_div_up(m, t.b), bt_div_up(n, t.b), splits, us};
         }
@@ -920,24 +928,39 @@ dim3 folded(long long blocks) {
     return dim3((unsigned)(blocks < W ? blocks : W), (unsigned)((blocks + W - 1) / W));
 }
 
+// Buffers for direct loads. A third one keeps two tiles on their way at any time, which a workgroup that is alone on its CU
+// needs: the products of a 64 x 64 tile take a third of a load's latency. Where more workgroups share a CU they hide it from
+// each other, and need the LDS. (bf16 dW of 2048 x 1024 -> 1024, 256 workgroups: 21.5 us with two, 15.7 with three; f32 4096 x
+// 1024 -> 1024, 1024 workgroups: 67 with two, 80 with three.)
+constexpr int three_up_to(int b) { return b == 256 ? 0 : b == 128 ? 256 : 512; }  // workgroups up to which there are three
+
 // the tile sizes shape_of chooses from, with or without direct loads
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
+int direct_launch(hipStream_t st, const Product &P, dim3 grid) {
+    const size_t lds = BUFS * Mm<T, BM, BN, WM, WN, AK, BKC, OUT>::BYTES;
+    const auto kernel = affine_mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT, BUFS>;
+    if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
+    BT_LAUNCH(BTK_AFFINE, st, (affine_mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT, BUFS>), grid, dim3(64 * WM * WN), lds, P);
+    BT_LAUNCH_CHECK();
+    return BT_OK;
+}
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
 int mm_launch(hipStream_t st, const Product &P, bool direct) {
     const long long blocks = (long long)P.tiles_m * P.tiles_n * P.splits;
     BT_REQUIRE((blocks + P.bias.blocks) * 64 * WM * WN < (1ll << 32), "bt_affine: Mismatched sizes! (%lld tiles)", blocks);
-    const size_t lds = 2 * Mm<T, BM, BN, WM, WN, AK, BKC, OUT>::BYTES;
-    const dim3 grid((unsigned)(blocks + P.bias.blocks)), block(64 * WM * WN);
-    if (direct) {
-        const auto kernel = affine_mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT>;
-        if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
-        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT>), grid, block, lds, P);
-    } else if constexpr (BM <= 128) {
-        const auto kernel = affine_mm_any<T, BM, BN, WM, WN, AK, BKC, OUT>;
-        if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
-        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_any<T, BM, BN, WM, WN, AK, BKC, OUT>), grid, block, lds, P);
+    const dim3 grid((unsigned)(blocks + P.bias.blocks));
+    if constexpr (BM <= 128) {
+        if (!direct) {
+            const size_t lds = 2 * Mm<T, BM, BN, WM, WN, AK, BKC, OUT>::BYTES;
+            const auto kernel = affine_mm_any<T, BM, BN, WM, WN, AK, BKC, OUT>;
+            if (int rc = bt_set_max_lds(reinterpret_cast<const void *>(kernel), lds)) return rc;
+            BT_LAUNCH(BTK_AFFINE, st, (affine_mm_any<T, BM, BN, WM, WN, AK, BKC, OUT>), grid, dim3(64 * WM * WN), lds, P);
+            BT_LAUNCH_CHECK();
+            return BT_OK;
+        }
+        if (blocks <= three_up_to(BM)) return direct_launch<T, BM, BN, WM, WN, AK, BKC, OUT, 3>(st, P, grid);
     }
-    BT_LAUNCH_CHECK();
-    return BT_OK;
+    return direct_launch<T, BM, BN, WM, WN, AK, BKC, OUT, 2>(st, P, grid);
 }
 template <typename T, bool AK, bool BKC, int OUT>
 int tile_launch(hipStream_t st, const Product &P, const Shape &s, bool direct) {
@@ -973,9 +996,14 @@ template <typename T, int B, int OUT_W, int OUT_X>
 int both_launch(hipStream_t st, const Product &W, const Product &X) {
     const long long w = (long long)W.tiles_m * W.tiles_n * W.splits + W.bias.blocks, x = (long long)X.tiles_m * X.tiles_n * X.splits;
     BT_REQUIRE((w + x) * 256 < (1ll << 32), "bt_affine_backward: Mismatched sizes! (%lld tiles)", w + x);
-    const size_t lds_w = 2 * Mm<T, B, B, 2, 2, false, false, OUT_W>::BYTES, lds_x = 2 * Mm<T, B, B, 2, 2, true, true, OUT_X>::BYTES;
-    static_assert(lds_w == lds_x, "tiles of one size");
-    BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, B, OUT_W, OUT_X>), dim3((unsigned)(w + x)), dim3(256), lds_w, W, X, (int)w);
+    typedef Mm<T, B, B, 2, 2, false, false, OUT_W> MW;
+    typedef Mm<T, B, B, 2, 2, true, true, OUT_X> MX;
+    static_assert(MW::BYTES == MX::BYTES && 3 * MW::BYTES <= 65536, "tiles of one size, within what needs no attribute");
+    const dim3 grid((unsigned)(w + x)), block(256);
+    if (w + x <= three_up_to(B))
+        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, B, OUT_W, OUT_X, 3>), grid, block, 3 * MW::BYTES, W, X, (int)w);
+    else
+        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, B, OUT_W, OUT_X, 2>), grid, block, 2 * MW::BYTES, W, X, (int)w);
     BT_LAUNCH_CHECK();
     return BT_OK;
 }
@@ -1133,19 +1161,19 @@ BackwardPlan backward_plan(const bt_affine_desc *d) {
     p.ranges = bt_div_up(d->batch, p.range);
     p.dw = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift);
     p.dx = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift);
-    if (p.dw.bm <= 64 && p.dx.bm <= 64 && p.dw.bm != p.dx.bm) {  // one launch: tiles of one size, whichever serves both better
-        const Shape w = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift, p.dx.bm);
-        const Shape x = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift, p.dw.bm);
-        if (w.us + p.dx.us < p.dw.us + x.us)
-            p.dw = w;
-        else
-            p.dx = x;
+    // One launch does both where their tiles are of one size, at most 64 x 64; the size that suits each best, or that. (bf16
+    // 4096 x 1024 -> 1024 37 us in one, 40 in two; 2048 x 2048 -> 2048 57 and 50; f32 200 x 512 -> 333 with 64 x 64 tiles 14 and 23.)
+    double us = p.dw.us + p.dx.us + LAUNCH_US;
+    p.both = false;
+    for (int b = 64; b >= (es == 4 ? 32 : 64); b /= 2) {
+        const Shape w = shape_of(d->in, d->out, d->batch, p.np_dw, es, p.lift, b);
+        const Shape x = shape_of(d->batch, d->in, d->out, p.np_dx, es, p.lift, b);
+        if (w.us + x.us <= us) p.dw = w, p.dx = x, p.both = true, us = w.us + x.us;
     }
     p.w_bytes = copy_bytes(copy_w(d), d->in, d->out, es), p.x_bytes = copy_bytes(copy_x(d), d->batch, d->in, es);
     p.gz_bytes = p.gz ? bt_align((size_t)d->batch * padded(d->out, es) * es) : 0;
     p.sum_bytes = bt_align((size_t)p.ranges * d->out * 4);
     const size_t a = p.dw.part_bytes(d->in, d->out), b = p.dx.part_bytes(d->batch, d->in);
-    p.both = p.dw.bm <= 64 && p.dx.bm <= 64;
     p.part_dx = p.both ? a : 0;
     p.part_bytes = p.both ? a + b : a > b ? a : b;
     p.total = p.w_bytes + p.x_bytes + p.gz_bytes * p.np_dw + p.sum_bytes + p.part_bytes;
@@ -1197,7 +1225,6 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
         X.e.out = gx, X.e.ld = d->x_ld, X.e.alpha = p.alpha;
     }
     (dw ? W : X).bias = bias;
-    // one launch where both take the smaller tiles (200 x 512 -> 333 f32 with 64 x 64 tiles: 23 us in two, 14 in one)
     if (dw && gx && p.both && W.a.aligned && W.b.aligned && X.a.aligned && X.b.aligned)
         return both_products<T>(st, W, p.dw, X, p.dx);
     if (dw)
