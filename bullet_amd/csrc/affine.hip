@@ -499,7 +499,7 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 // the chip is taken: for one product of 16 x 16 x 32 a 256 x 256 tile reads 384 bytes of LDS, a 128 x 128 one 512 and a
 // 64 x 64 one 1024. 16384 x 2048 -> 4096 bf16 takes 234 us, 1.17 PFLOP/s (the MFMA units are busy 55 % of the clocks, bank
 // conflicts are few); dW of 16384 x 2048 -> 2048 with 4 workgroups to a tile 113 us and grad_x 109, 1.2 and 1.26 PFLOP/s;
-// 4096 x 1024 -> 1024 f32 with 64 x 64 tiles 65 us, 132 TFLOP/s, 83 % of the rate of f32.
+// 4096 x 1024 -> 1024 f32 with 64 x 64 tiles 66 us, 130 TFLOP/s, 83 % of the rate of f32.
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
 __device__ __forceinline__ void mm_direct(const Product &P, int wg, int wgs, char *lds) {
     typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
@@ -1080,8 +1080,8 @@ int prepare_launch(hipStream_t st, const Prepare<T> &p, int np) {
     return BT_OK;
 }
 
-// Rows that affine_few takes: 8, but 4 where both weights and rows have 16 bits (2048 -> 4096 bf16: 4 rows 8.9 us against 9.9 on
-// the matrix cores, 8 rows 13.3 against 9.9; f32: 8 rows 11.2 against 16; f32 weights that would have to be rounded into a
+// Rows that affine_few takes: 8, but 4 where both weights and rows have 16 bits (2048 -> 4096 bf16: 4 rows 9.0 us against 10.4 on
+// the matrix cores, 8 rows 13.3 against 9.9; f32: 8 rows 11.1 against 12.6; f32 weights that would have to be rounded into a
 // copy first: 8 rows 16 against 20)
 int few_rows(const bt_affine_desc *d) { return d->w_type == BT_TYPE_F32 ? 8 : 4; }
 template <typename T, typename TW>
