@@ -150,6 +150,28 @@ def test_large_tiles(shape, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("batch,out", [(72, 80), (1160, 1608)])
+def test_sums_of_few_tiles(batch, out, kind):
+    """as many tiles of k as buffers, one less and a few more, whole and not, with few workgroups (three buffers) and many (two)"""
+    tile = 32 if kind == "f32" else 64
+    rng = np.random.default_rng(28)
+    for tiles in (1, 2, 3, 4, 5, 6, 7):
+        for k in (tiles * tile - 8, tiles * tile, tiles * tile + 3):
+            run_forward(rng, batch, k, out, kind, "relu")
+            if batch < 100:
+                run_backward(rng, k, batch, out, kind, "crelu")
+                run_backward(rng, batch, out, k, kind, "identity")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shape", [(1000, 304, 4096), (990, 130, 4001), (2048, 64, 2048), (1030, 448, 4000)])
+def test_tiles_that_just_fill_the_chip(shape, kind):
+    rng = np.random.default_rng(29)
+    run_forward(rng, *shape, kind, "screlu", residual=True)
+    run_backward(rng, *shape, kind, "relu")
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_parts_of_the_gradient(kind):
     for parts in (dict(want_dw=False), dict(want_db=False), dict(want_gx=False), dict(want_dw=False, want_gx=False),
                   dict(want_db=False, want_gx=False), dict(want_dw=False, want_db=False)):
