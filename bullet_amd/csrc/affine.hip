@@ -139,6 +139,7 @@ struct Epilogue {
     long long ld;
     int act;
     float alpha;
+    int past;  // outputs are stored past the caches (see past_caches)
 };
 
 // W neighbouring columns of one row, n of them inside the matrix
@@ -157,11 +158,14 @@ struct Cols {
         }
         return v;
     }
-    static __device__ __forceinline__ void store(T *p, sums v, int n) {
+    static __device__ __forceinline__ void store(T *p, sums v, int n, bool past) {
+        typedef T any __attribute__((ext_vector_type(W), aligned(sizeof(T))));
         vec q;
 #pragma unroll
         for (int j = 0; j < W; j++) q[j] = (T)v[j];
-        if (n >= W) {
+        if (n >= W && past) {
+            __builtin_nontemporal_store((any)q, (any *)p);
+        } else if (n >= W) {
             __builtin_memcpy(p, &q, sizeof(q));
         } else {
 #pragma unroll
@@ -186,9 +190,9 @@ __device__ __forceinline__ void finish_at(const Epilogue &e, int row, int c, int
                                           typename Cols<T, W>::sums bias, typename Cols<T, W>::vec residual) {
     const size_t at = (size_t)row * e.ld + c;
     if constexpr (OUT == OUT_F32) {
-        Cols<float, W>::store((float *)e.out + at, v * e.alpha, n);
+        Cols<float, W>::store((float *)e.out + at, v * e.alpha, n, e.past);
     } else if constexpr (OUT == OUT_TYPE) {
-        Cols<T, W>::store((T *)e.out + at, v * e.alpha, n);
+        Cols<T, W>::store((T *)e.out + at, v * e.alpha, n, e.past);
     } else {
         v += bias;
         // bt_act_fwd without its branches: this is unrolled over a whole tile
@@ -199,12 +203,12 @@ __device__ __forceinline__ void finish_at(const Epilogue &e, int row, int c, int
             const float a = fminf(fmaxf(v[j], 0.0f), top), b = square ? a * a : a;
             v[j] = clamp ? b : v[j];
         }
-        if (e.saved) Cols<T, W>::store((T *)e.saved + at, v, n);
+        if (e.saved) Cols<T, W>::store((T *)e.saved + at, v, n, e.past);
         if (e.residual) {
 #pragma unroll
             for (int j = 0; j < W; j++) v[j] += (float)residual[j];
         }
-        Cols<T, W>::store((T *)e.out + at, v, n);
+        Cols<T, W>::store((T *)e.out + at, v, n, e.past);
     }
 }
 
@@ -497,7 +501,7 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 //
 // Bound by the MFMA units and, close behind, by the LDS bytes that feed them, which is why the largest tile that still fills
 // the chip is taken: for one product of 16 x 16 x 32 a 256 x 256 tile reads 384 bytes of LDS, a 128 x 128 one 512 and a
-// 64 x 64 one 1024. 16384 x 2048 -> 4096 bf16 takes 234 us, 1.17 PFLOP/s (the MFMA units are busy 55 % of the clocks, bank
+// 64 x 64 one 1024. 16384 x 2048 -> 4096 bf16 takes 208 us, 1.32 PFLOP/s (the MFMA units are busy 55 % of the clocks, bank
 // conflicts are few); dW of 16384 x 2048 -> 2048 with 4 workgroups to a tile 113 us and grad_x 109, 1.2 and 1.26 PFLOP/s;
 // 4096 x 1024 -> 1024 f32 with 64 x 64 tiles 66 us, 130 TFLOP/s, 83 % of the rate of f32.
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
@@ -1035,6 +1039,13 @@ Operand matrix(const void *p, long long ld, int rows, int len, size_t es) {
 // one of the workspace's: the zeros behind a row are part of it
 Operand own_matrix(const void *p, int rows, int len, size_t es) { return matrix(p, padded(len, es), rows, whole_chunks(len, es), es); }
 
+// Outputs whose rows start on 16 bytes are stored past the caches, where they would only push out the operands (16384 x 2048 ->
+// 4096 bf16 207 us, 231 through them). Pieces of other rows share lines, which the caches put together (1537 x 1027 -> 1881 f16,
+// rows 3 apart: 20.4 us through them, 22.7 past them).
+bool past_caches(const void *out, const void *saved, long long ld, size_t es) {
+    return ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(saved)) & 15) == 0 && ld * es % 16 == 0;
+}
+
 // Matrices that are copied into the workspace first: those whose rows do not start on 16 bytes (read through registers
 // instead, both operands of 4096 x 1024 -> 1024 make the forward product 38 us of bf16 and 102 of f32; the copies take 8 and
 // 13 us and leave 18 and 73), and f32 weights of a 16-bit layer. One whose first element alone is off is read through registers.
@@ -1119,7 +1130,7 @@ ForwardPlan forward_plan(const bt_affine_desc *d) {
 template <typename T>
 int forward(hipStream_t st, const bt_affine_desc *d, const void *w, const float *bias, const void *x, const void *residual, void *y,
             void *saved, char *ws) {
-    const Epilogue e{bias, residual, y, saved, d->y_ld, d->act, 1.0f};
+    const Epilogue e{bias, residual, y, saved, d->y_ld, d->act, 1.0f, past_caches(y, saved, d->y_ld, sizeof(T))};
     if (d->batch <= few_rows(d))
         return d->w_type == d->type ? few_launch<T, T>(st, d, w, x, e) : few_launch<T, float>(st, d, w, x, e);
     const ForwardPlan p = forward_plan(d);
@@ -1216,13 +1227,13 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
         W.a = ox, W.b = gz_operand(p.np_dw);
         W.m = d->in, W.n = d->out, W.k = d->batch, W.passes = p.np_dw, W.lift = p.lift;
         W.part = (float *)part;
-        W.e.out = dw, W.e.ld = d->w_ld, W.e.alpha = p.alpha;
+        W.e.out = dw, W.e.ld = d->w_ld, W.e.alpha = p.alpha, W.e.past = past_caches(dw, nullptr, d->w_ld, sizeof(float));
     }
     if (gx) {
         X.a = gz_operand(p.np_dx), X.b = ow;
         X.m = d->batch, X.n = d->in, X.k = d->out, X.passes = p.np_dx, X.lift = p.lift;
         X.part = (float *)(part + p.part_dx);
-        X.e.out = gx, X.e.ld = d->x_ld, X.e.alpha = p.alpha;
+        X.e.out = gx, X.e.ld = d->x_ld, X.e.alpha = p.alpha, X.e.past = past_caches(gx, nullptr, d->x_ld, sizeof(T));
     }
     (dw ? W : X).bias = bias;
     if (dw && gx && p.both && W.a.aligned && W.b.aligned && X.a.aligned && X.b.aligned)
