@@ -501,8 +501,8 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 //
 // Bound by the MFMA units and, close behind, by the LDS bytes that feed them, which is why the largest tile that still fills
 // the chip is taken: for one product of 16 x 16 x 32 a 256 x 256 tile reads 384 bytes of LDS, a 128 x 128 one 512 and a
-// 64 x 64 one 1024. 16384 x 2048 -> 4096 bf16 takes 208 us, 1.32 PFLOP/s (the MFMA units are busy 55 % of the clocks, bank
-// conflicts are few); dW of 16384 x 2048 -> 2048 with 4 workgroups to a tile 113 us and grad_x 109, 1.2 and 1.26 PFLOP/s;
+// 64 x 64 one 1024. 16384 x 2048 -> 4096 bf16 takes 207 us, 1.33 PFLOP/s (the MFMA units are busy 59 % of the clocks, bank
+// conflicts are few); dW of 16384 x 2048 -> 2048 with 4 workgroups to a tile 110 us and grad_x 109, 1.25 PFLOP/s;
 // 4096 x 1024 -> 1024 f32 with 64 x 64 tiles 66 us, 130 TFLOP/s, 83 % of the rate of f32.
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
 __device__ __forceinline__ void mm_direct(const Product &P, int wg, int wgs, char *lds) {
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256) void affine_join(Product P) {
 //
 // A copy has rows on 128 bytes (so that a tile's row of k is one line of memory), of the layer's type (f32 weights are
 // rounded), with zeros up to a whole chunk. One chunk a thread. Both the copies and gz are bound by memory: gz of 16384 x 2048
-// bf16 (two reads, one write, 201 MB) 40 us, 5 TB/s.
+// bf16 (two reads, one write, 201 MB) 37 us, 5.4 TB/s.
 template <typename T>
 struct Copy {
     const void *from;

@@ -293,7 +293,7 @@ __device__ __noinline__ double sum_again(const T *z, const uint8_t *mask, int wi
 
 // One group of G lanes per row, at most K chunks a lane, all in registers.
 // Bound by memory where there are many rows: 16384 x 1880 f32 with the full KL (two rows of logits and the mask in, gradient
-// out, 401 MB) 82-84 us, 4.8 TB/s, what a copy reaches; 8192 x 4096 bf16 (134 MB) 34 us, 3.9 TB/s. Few rows: 6-7 us for 64 of
+// out, 401 MB) 82-84 us, 4.8 TB/s, what a copy reaches; 8192 x 4096 bf16 (134 MB) 31 us, 4.3 TB/s. Few rows: 6-7 us for 64 of
 // 1880, the time of a launch and of four loads in turn (mask and logits, the action, its logit, its row's scalars).
 template <typename T, int G, int K, bool FULL>
 __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
@@ -513,7 +513,7 @@ struct PrefArgs {
 __device__ __forceinline__ int pref_offset(const PrefArgs &a, int k) { return min(max(a.offsets[k], 0), a.d.rows); }
 
 // Statistics of one row, as in policy_rows. The rows are read again for the gradient, since a pair's factor needs all
-// rows of both its lines first: 16740 x 1880 bf16 (logits and mask 94 MB) 25 us, 3.8 TB/s.
+// rows of both its lines first: 16740 x 1880 bf16 (logits and mask 94 MB) 21 us, 4.6 TB/s.
 template <typename T, int G, int K>
 __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
     constexpr int V = Row<T>::V;
