@@ -180,9 +180,9 @@ __device__ __forceinline__ void store_chunk(T *row, int e0, int width, typename 
 
 // Softmax statistics of one row, and what the KL over the whole policy needs beside them.
 struct RowStats {
-    float top, sum;       // largest legal logit, sum of exp(z - top)
-    float ref_top, ref_sum;
-    float cross;          // sum of exp(z - top) (z - q)
+    float top, ref_top;   // largest legal logit
+    double sum, ref_sum;  // sum of exp(z - top)
+    double cross;         // sum of exp(z - top) (z - q)
 };
 
 // What a row's element needs for its gradient: with e = exp(z - top), g = ce e (+ a share of its own for the action taken),
@@ -229,12 +229,13 @@ struct PolicyRow {
 __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, const PolicyRow &pr, const RowStats &st, double sum64,
                                                bool full, RowGrad &g, double &logp, double &kl, float &loss, float &grad_taken) {
     const bt_policy_desc &d = a.d;
-    const double logsum = log64(sum64 > 0.0 ? sum64 : (double)st.sum);
+    const double logsum = log64(sum64 > 0.0 ? sum64 : st.sum);
     logp = ((double)pr.za - (double)st.top) - logsum;
     const double adv = a.advantages[row], w = a.weights ? (double)a.weights[row] : 1.0;
     const double r = exp64(logp - (double)a.old_logp[row]);
     const double lo = 1.0 - (double)d.clip_low, hi = 1.0 + (double)d.clip_high;
-    // a 32-bit sum of up to 2^24 terms is off by less than 1e-5 of itself
+    // (sum: 74 roundings of 2^-24 at most, 64 of a lane's own and 10 of the lanes', or 7 where chunks are added in 64 bits;
+    // with its terms' own errors less than 1e-5 of it)
     const bool near = fabs(r - lo) < 1e-5 * lo || fabs(r - hi) < 1e-5 * hi;
     const double free_gain = r * adv, held_gain = fmin(fmax(r, lo), hi) * adv;
     double slope = free_gain <= held_gain || free_gain != free_gain ? -free_gain : 0.0;
@@ -247,14 +248,14 @@ __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, con
         kl = em1 - x;
         slope -= (double)d.kl_weight * em1;
     } else if (full) {
-        const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log64((double)st.ref_sum));
-        kl = (double)st.cross / (double)st.sum - dl;
+        const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log64(st.ref_sum));
+        kl = st.cross / st.sum - dl;
         ck = w * (double)d.kl_weight;
         g.shift = (float)(dl + kl);
     }
     loss = (float)(w * ((double)d.kl_weight * kl - (free_gain != free_gain ? free_gain : fmin(free_gain, held_gain))));
     g.top = st.top == NEG_INF ? 0.0f : st.top;  // (nothing but NaN)
-    const float inv = 1.0f / st.sum;
+    const float inv = 1.0f / (float)st.sum;
     g.ce = -(float)(w * slope) * inv;
     g.ck = (float)ck * inv;
     g.plain = fabsf(g.ce) < __builtin_huge_valf();
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
     st.sum = Group<G>::sum(s, red);
     st.ref_sum = FULL ? Group<G>::sum(sq, red) : 1.0f;
     st.cross = FULL ? Group<G>::sum(cross, red) : 0.0f;
-    const bool counted = pr.counted && st.sum != 0.0f;  // (0: nothing above -infinity; NaN counts)
+    const bool counted = pr.counted && st.sum != 0.0;  // (0: nothing above -infinity; NaN counts)
 
     T *grad = a.grad ? (T *)a.grad + (size_t)row * a.d.ld : nullptr;
     if (!counted) {
@@ -383,6 +384,23 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
     if (lane == (act / V) % G) grad[act] = (T)grad_taken;
 }
 
+// A lane's running maximum and sum of exponentials, for rows too wide for registers. A chunk's terms are added in 32 bits, the
+// chunks in 64: thousands of equal terms (16-bit logits repeat) round the same way every time, and what 32 bits would lose,
+// 6e-5 of the sum of 2^20 of them, is more than a ratio next to a clipping border can bear.
+struct Running {
+    float top = NEG_INF;
+    double sum = 0.0;
+    __device__ __forceinline__ float base() const { return top == NEG_INF ? 0.0f : top; }
+    // what the sums so far are multiplied by
+    __device__ __forceinline__ double raise(float m) {
+        const double f = exp64((double)top - (double)m);
+        sum *= f, top = m;
+        return f;
+    }
+    // this lane's share of the sum beside the row's maximum (without a finite maximum: 0 or NaN)
+    __device__ __forceinline__ double scale(float row_top) const { return top == NEG_INF ? 1.0 : exp64((double)top - (double)row_top); }
+};
+
 // Rows too wide for the registers of a workgroup: running maximum and sums in one pass, the gradient in a second one.
 template <typename T, bool FULL>
 __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
@@ -398,7 +416,8 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
     const T *q = FULL ? (const T *)a.ref + (size_t)row * a.d.ld : nullptr;
     const uint8_t *mask = a.mask ? a.mask + (size_t)row * a.d.mask_ld : nullptr;
     const PolicyRow pr = policy_row_begin(a, z, q, mask, row, FULL);
-    float top = NEG_INF, s = 0.0f, ref_top = NEG_INF, sq = 0.0f, cross = 0.0f;
+    Running z_run, q_run;
+    double cross = 0.0;
     for (long long e0 = (long long)lane * V; e0 < width; e0 += 256 * V) {
         const bytes b = legal_bytes<T>(mask, (int)e0, width);
         vec zc, qc;
@@ -408,35 +427,33 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
             load_chunk<T>(q, (int)e0, width, qc);
             keep_legal<T>(mask, (int)e0, width, b, qc);
         }
-        float m = top, mq = ref_top;
+        float m = z_run.top, mq = q_run.top;
         for (int j = 0; j < V; j++) {
             m = fmaxf(m, (float)zc[j]);
             if (FULL) mq = fmaxf(mq, (float)qc[j]);
         }
-        if (m > top) {
-            const float f = exp_neg(top - m);
-            s *= f, cross *= f, top = m;
-        }
-        if (FULL && mq > ref_top) sq *= exp_neg(ref_top - mq), ref_top = mq;
-        const float base = top == NEG_INF ? 0.0f : top;
+        if (m > z_run.top) cross *= z_run.raise(m);
+        if (FULL && mq > q_run.top) q_run.raise(mq);
+        float s = 0.0f, sq = 0.0f, sc = 0.0f;  // of this chunk
         for (int j = 0; j < V; j++) {
-            const float zv = (float)zc[j], e = exp_neg(zv - base);
+            const float zv = (float)zc[j], e = exp_neg(zv - z_run.base());
             s += e;
             if (FULL) {
                 const float qv = (float)qc[j];
-                sq += exp_neg(qv - (ref_top == NEG_INF ? 0.0f : ref_top));
-                cross += e == 0.0f ? 0.0f : e * (zv - qv);
+                sq += exp_neg(qv - q_run.base());
+                sc += e == 0.0f ? 0.0f : e * (zv - qv);
             }
         }
+        z_run.sum += s, q_run.sum += sq, cross += sc;
     }
     RowStats st;
-    st.top = Group<256>::max(top, red);
-    const float f = top == NEG_INF ? 0.0f : exp_neg(top - st.top);
-    st.sum = Group<256>::sum(top == NEG_INF ? s : s * f, red);  // (s without a finite maximum: 0 or NaN)
-    st.ref_top = FULL ? Group<256>::max(ref_top, red) : 0.0f;
-    st.ref_sum = FULL ? Group<256>::sum(ref_top == NEG_INF ? sq : sq * exp_neg(ref_top - st.ref_top), red) : 1.0f;
-    st.cross = FULL ? Group<256>::sum(top == NEG_INF ? cross : cross * f, red) : 0.0f;
-    const bool counted = pr.counted && st.sum != 0.0f;  // (0: nothing above -infinity; NaN counts)
+    st.top = Group<256>::max(z_run.top, red);
+    const double f = z_run.scale(st.top);
+    st.sum = Group<256>::sum64(z_run.sum * f, red64);
+    st.ref_top = FULL ? Group<256>::max(q_run.top, red) : 0.0f;
+    st.ref_sum = FULL ? Group<256>::sum64(q_run.sum * q_run.scale(st.ref_top), red64) : 1.0;
+    st.cross = FULL ? Group<256>::sum64(cross * f, red64) : 0.0;
+    const bool counted = pr.counted && st.sum != 0.0;  // (0: nothing above -infinity; NaN counts)
     T *grad = a.grad ? (T *)a.grad + (size_t)row * a.d.ld : nullptr;
     RowGrad g;
     double logp = 0.0, kl = 0.0;
@@ -518,6 +535,7 @@ template <typename T, int G, int K>
 __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
     constexpr int V = Row<T>::V;
     __shared__ float red[4];
+    __shared__ double red64[4];
     const int lane = threadIdx.x % G;
     const long long row64 = row_block() * (256 / G) + threadIdx.x / G;
     if (row64 < pref_offset(a, 0) || row64 >= pref_offset(a, 2 * a.d.pairs)) return;
@@ -549,21 +567,22 @@ __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
 #pragma unroll
             for (int j = 0; j < V; j++) s += exp_neg((float)zc[k][j] - base);
         s = Group<G>::sum(s, red);
-    } else {  // any width: running maximum and sum
+    } else {  // any width
+        Running run;
         for (long long e0 = (long long)lane * V; e0 < width; e0 += G * V) {
             const typename Row<T>::bytes b = legal_bytes<T>(mask, (int)e0, width);
             typename Row<T>::vec zc;
             load_chunk<T>(z, (int)e0, width, zc);
             keep_legal<T>(mask, (int)e0, width, b, zc);
-            float m = top;
+            float m = run.top;
             for (int j = 0; j < V; j++) m = fmaxf(m, (float)zc[j]);
-            if (m > top) s *= exp_neg(top - m), top = m;
-            const float base = top == NEG_INF ? 0.0f : top;
-            for (int j = 0; j < V; j++) s += exp_neg((float)zc[j] - base);
+            if (m > run.top) run.raise(m);
+            float c = 0.0f;
+            for (int j = 0; j < V; j++) c += exp_neg((float)zc[j] - run.base());
+            run.sum += c;
         }
-        const float all = Group<G>::max(top, red);
-        s = Group<G>::sum(top == NEG_INF ? s : s * exp_neg(top - all), red);
-        top = all;
+        top = Group<G>::max(run.top, red);
+        s = (float)Group<G>::sum64(run.sum * run.scale(top), red64);
     }
     if (lane == 0) {
         a.za[row] = za;

@@ -1,0 +1,105 @@
+"""-m gpu: how many digits the policy and preference losses keep, and what they make of infinite values: cases whose right answer
+is known beyond the bounds that policy_ref.py allows for rows in general."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs a GPU", allow_module_level=True)
+
+from bullet_amd import lib  # noqa: E402
+import policy_ref as pr  # noqa: E402
+
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+INF = float("inf")
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def dev(a, dtype=np.float32):
+    return torch.from_numpy(np.ascontiguousarray(np.asarray(a).astype(dtype))).cuda()
+
+
+def policy(z, actions, old, adv, kl="none", ref=None, mask=None, klw=0.05):
+    """z: the logits on the device -> loss, grad, row_loss, row_logp, row_kl in float64"""
+    n, width = z.shape
+    kind = {v: k for k, v in DT.items()}[z.dtype]
+    loss, grad = torch.full((1,), float("nan"), device="cuda"), torch.full_like(z, 9.0)
+    rows = [torch.full((n,), float("nan"), device="cuda") for _ in range(3)]
+    # (named: the call only queues work, and what it reads has to outlive it)
+    at, ot, vt, mt = dev(actions, np.int32), dev(old), dev(adv), None if mask is None else dev(mask, np.uint8)
+    pr.call_policy(stream(), pr.policy_desc(n, width, kind, kl=kl, klw=klw), z, mt, at, ot, vt, ref, None, loss, grad, *rows)
+    torch.cuda.synchronize()
+    return [t.double().cpu().numpy() for t in (loss, grad, *rows)]
+
+
+def preference(z, actions, offsets, ref, beta=0.1, smoothing=0.05):
+    """-> loss, grad, pair_loss, line_logp in float64"""
+    n, width = z.shape
+    kind = {v: k for k, v in DT.items()}[z.dtype]
+    pairs = len(ref) // 2
+    d = pr.preference_desc(pairs, n, width, kind, beta=beta, smoothing=smoothing)
+    ws = torch.full((lib.load().bt_preference_loss_workspace_bytes(C.byref(d)),), 0xFF, dtype=torch.uint8, device="cuda")
+    out = [torch.full((1,), float("nan"), device="cuda"), torch.full_like(z, 9.0), torch.full((pairs,), float("nan"), device="cuda"),
+           torch.full((2 * pairs,), float("nan"), device="cuda")]
+    at, ot, rt = dev(actions, np.int32), dev(offsets, np.int32), dev(ref)
+    pr.call_preference(stream(), d, z, None, at, ot, rt, None, *out, ws)
+    torch.cuda.synchronize()
+    return [t.double().cpu().numpy() for t in out]
+
+
+# ---------------------------------------------------------------- sums of long rows
+def repeated(kind, width):
+    """rows of one logit each, all below the taken move's 0: every term of a row's sum is the same number -> logits on the
+    device, the log-probability of move 5"""
+    v = np.concatenate([np.arange(1, 49) / 8.0, np.array([0.15625, 5.09375, 3.65625, 5.40625])])
+    z = torch.empty(len(v), width, dtype=DT[kind], device="cuda")
+    z[:] = dev(-v).to(DT[kind])[:, None]
+    z[:, 5] = 0.0
+    kept = z[:, 0].double().cpu().numpy()
+    return z, -np.log(1.0 + (width - 1) * np.exp(kept))
+
+
+# bound of a log-probability: as policy_ref.row_error without its share for the width, and one rounding to 32 bits
+def logp_bound(lp):
+    return 5e-6 + 2.0 ** -24 * np.abs(lp)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("width", [1 << 18, 1 << 20, (1 << 20) + 77])
+def test_sums_of_long_rows_of_equal_logits(kind, width):
+    z, lp = repeated(kind, width)
+    n = len(lp)
+    got = policy(z, np.full(n, 5), lp, np.ones(n))[3]
+    assert (np.abs(got - lp) <= logp_bound(lp)).all(), np.abs(got - lp).max()
+    offsets = np.arange(n + 1)  # a line for every row
+    line = preference(z, np.full(n, 5), offsets, lp)[3]
+    assert (np.abs(line - lp) <= logp_bound(lp)).all(), np.abs(line - lp).max()
+
+
+@pytest.mark.parametrize("kl", ["none", "full"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_long_rows_next_to_the_clipping_border(kind, kl):
+    """ratios 2e-5 and 4e-5 to either side of a border: the taken move's gradient is 0 on one side and the ratio's on the other"""
+    z, lp = repeated(kind, 1 << 20)
+    n = len(lp)
+    klw = 0.0
+    ref = z.clone() if kl == "full" else None
+    for high, adv in ((True, 1.0), (False, -1.0)):
+        border = 1.0 + np.float64(np.float32(0.28)) if high else 1.0 - np.float64(np.float32(0.2))
+        for off in (2e-5, -2e-5, 4e-5, -4e-5):
+            old = (lp - np.log(border * (1.0 + off))).astype(np.float32)
+            r = np.exp(lp - old.astype(np.float64))  # (a step of old at 14 is 1e-6)
+            assert (np.abs(r / border - 1.0 - off) < 2e-6).all()
+            grad = policy(z, np.full(n, 5), old, np.full(n, adv), kl=kl, ref=ref, klw=klw)[1][:, 5]
+            clipped = (off > 0) == high
+            want = 0.0 if clipped else -r * adv * (1.0 - np.exp(lp))
+            # (the ratio is off by the sum's 5e-6; the gradient is rounded to the logits' type)
+            allow = np.abs(want) * (5e-6 + pr.EPS[kind] * 1.01)
+            assert (np.abs(grad - want) <= allow).all(), (high, off, np.flatnonzero(np.abs(grad - want) > allow))
