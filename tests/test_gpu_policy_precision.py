@@ -56,14 +56,14 @@ def preference(z, actions, offsets, ref, beta=0.1, smoothing=0.05):
 
 # ---------------------------------------------------------------- sums of long rows
 def repeated(kind, width):
-    """rows of one logit each, all below the taken move's 0: every term of a row's sum is the same number -> logits on the
-    device, the log-probability of move 5"""
+    """rows of one logit each below 512 logits of 0 at their front, one in every chunk that a lane reads first: from then on every
+    term of a lane's sum is the same number -> logits on the device, the log-probability of move 4"""
     v = np.concatenate([np.arange(1, 49) / 8.0, np.array([0.15625, 5.09375, 3.65625, 5.40625])])
     z = torch.empty(len(v), width, dtype=DT[kind], device="cuda")
     z[:] = dev(-v).to(DT[kind])[:, None]
-    z[:, 5] = 0.0
-    kept = z[:, 0].double().cpu().numpy()
-    return z, -np.log(1.0 + (width - 1) * np.exp(kept))
+    z[:, :2048:4] = 0.0
+    kept = z[:, 1].double().cpu().numpy()
+    return z, -np.log(512 + (width - 512) * np.exp(kept))
 
 
 # bound of a log-probability: as policy_ref.row_error without its share for the width, and one rounding to 32 bits
@@ -76,10 +76,10 @@ def logp_bound(lp):
 def test_sums_of_long_rows_of_equal_logits(kind, width):
     z, lp = repeated(kind, width)
     n = len(lp)
-    got = policy(z, np.full(n, 5), lp, np.ones(n))[3]
+    got = policy(z, np.full(n, 4), lp, np.ones(n))[3]
     assert (np.abs(got - lp) <= logp_bound(lp)).all(), np.abs(got - lp).max()
     offsets = np.arange(n + 1)  # a line for every row
-    line = preference(z, np.full(n, 5), offsets, lp)[3]
+    line = preference(z, np.full(n, 4), offsets, lp)[3]
     assert (np.abs(line - lp) <= logp_bound(lp)).all(), np.abs(line - lp).max()
 
 
@@ -97,7 +97,7 @@ def test_long_rows_next_to_the_clipping_border(kind, kl):
             old = (lp - np.log(border * (1.0 + off))).astype(np.float32)
             r = np.exp(lp - old.astype(np.float64))  # (a step of old at 14 is 1e-6)
             assert (np.abs(r / border - 1.0 - off) < 2e-6).all()
-            grad = policy(z, np.full(n, 5), old, np.full(n, adv), kl=kl, ref=ref, klw=klw)[1][:, 5]
+            grad = policy(z, np.full(n, 4), old, np.full(n, adv), kl=kl, ref=ref, klw=klw)[1][:, 4]
             clipped = (off > 0) == high
             want = 0.0 if clipped else -r * adv * (1.0 - np.exp(lp))
             # (the ratio is off by the sum's 5e-6; the gradient is rounded to the logits' type)
