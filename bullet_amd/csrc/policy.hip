@@ -20,9 +20,14 @@ struct Row {
     typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint64_t>::type bytes;  // one mask byte per element
 };
 
-// exp(x) for x <= 0 in 32 bits: the rounding of x log2(e) costs 2^-24 |x| of the result, and terms with |x| in the tens have
-// no weight in a sum beside one that is 1. -infinity gives 0, NaN stays.
-__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+// exp(x) for x <= 0 in 32 bits, to 2^-22 of itself: 2^t of the rounded t = x log2(e), and what the rounding left over, x - t ln 2
+// (ln 2 as two numbers), multiplied in; without it the entries of a gradient lose 2^-24 |x|. Below -150 it is 0 in 32 bits; the
+// maximum keeps -infinity out of the differences and lets NaN pass.
+__device__ __forceinline__ float exp_neg(float x) {
+    const float c = __builtin_elementwise_maximum(x, -150.0f), t = c * 1.44269502f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, fmaf(t, 1.90465421e-9f, fmaf(t, -0.693147182f, c)), e);
+}
 
 // The scalars of a row in 64 bits, each computed by all its lanes, so shorter than the library's functions: their arguments
 // are finite sums and differences of logits, and 1e-13 is plenty.

@@ -103,3 +103,22 @@ def test_long_rows_next_to_the_clipping_border(kind, kl):
             # (the ratio is off by the sum's 5e-6; the gradient is rounded to the logits' type)
             allow = np.abs(want) * (5e-6 + pr.EPS[kind] * 1.01)
             assert (np.abs(grad - want) <= allow).all(), (high, off, np.flatnonzero(np.abs(grad - want) > allow))
+
+
+# ---------------------------------------------------------------- exponentials
+@pytest.mark.parametrize("width", [7, 300, 1880, 7000, 20001])
+def test_small_entries_of_a_gradient_keep_their_digits(width):
+    """Beside two logits of 0, moves 0 (taken) and 1, a move of logit x has e^x times move 1's gradient. Move 1's e^0 is exactly 1,
+    so the quotient is off by e^x alone and one rounding of the product: argument and correction together less than 2^-25, exp2 1 ulp
+    (2^-23), the correction's rounding and the product's 2^-24 each."""
+    rng = np.random.default_rng(41)
+    x = -75.0 * rng.random((6, width)).astype(np.float32)
+    x[:, :2] = 0.0
+    z, n = dev(x), len(x)
+    want = np.exp(x[:, 1:].astype(np.float64))
+    bound = (2.0 ** -25 + 2.0 ** -23 + 2 * 2.0 ** -24) * 1.001
+    lp = -np.log(np.exp(x.astype(np.float64)).sum(1))
+    grads = dict(policy=policy(z, np.zeros(n), lp, np.ones(n))[1], preference=preference(z, np.zeros(n), np.arange(n + 1), lp)[1])
+    for name, g in grads.items():
+        off = np.abs(g[:, 1:] / g[:, 1:2] / want - 1.0)
+        assert off.max() <= bound, (name, off.max(), x[:, 1:][off > bound][:3])
