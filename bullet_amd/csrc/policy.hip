@@ -184,10 +184,11 @@ __device__ __forceinline__ void store_chunk(T *row, int e0, int width, typename 
 }
 
 // Softmax statistics of one row, and what the KL over the whole policy needs beside them.
+template <typename S>  // (32 bits where rows fill registers: 64 would cost one of three waves a SIMD, 87 us instead of 83)
 struct RowStats {
-    float top, ref_top;   // largest legal logit
-    double sum, ref_sum;  // sum of exp(z - top)
-    double cross;         // sum of exp(z - top) (z - q)
+    float top, ref_top;  // largest legal logit
+    S sum, ref_sum;      // sum of exp(z - top)
+    S cross;             // sum of exp(z - top) (z - q)
 };
 
 // What a row's element needs for its gradient: with e = exp(z - top), g = ce e (+ a share of its own for the action taken),
@@ -231,10 +232,11 @@ struct PolicyRow {
     float za, qa;    // logit (and reference logit) of the action taken
     bool counted;
 };
-__device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, const PolicyRow &pr, const RowStats &st, double sum64,
-                                               bool full, RowGrad &g, double &logp, double &kl, float &loss, float &grad_taken) {
+template <typename S>
+__device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, const PolicyRow &pr, const RowStats<S> &st,
+                                               double sum64, bool full, RowGrad &g, double &logp, double &kl, float &loss, float &grad_taken) {
     const bt_policy_desc &d = a.d;
-    const double logsum = log64(sum64 > 0.0 ? sum64 : st.sum);
+    const double logsum = log64(sum64 > 0.0 ? sum64 : (double)st.sum);
     logp = ((double)pr.za - (double)st.top) - logsum;
     const double adv = a.advantages[row], w = a.weights ? (double)a.weights[row] : 1.0;
     const double r = exp64(logp - (double)a.old_logp[row]);
@@ -253,8 +255,8 @@ __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, con
         kl = em1 - x;
         slope -= (double)d.kl_weight * em1;
     } else if (full) {
-        const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log64(st.ref_sum));
-        kl = st.cross / st.sum - dl;
+        const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log64((double)st.ref_sum));
+        kl = (double)st.cross / (double)st.sum - dl;
         ck = w * (double)d.kl_weight;
         g.shift = (float)(dl + kl);
     }
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
             for (int j = 0; j < V; j++) ref_top = fmaxf(ref_top, (float)qc[FULL ? k : 0][j]);
         }
     }
-    RowStats st;
+    RowStats<float> st;
     st.top = Group<G>::max(top, red);
     st.ref_top = FULL ? Group<G>::max(ref_top, red) : 0.0f;
     const float base = st.top == NEG_INF ? 0.0f : st.top;  // (nothing left: every term is exp(-infinity) = 0)
@@ -359,7 +361,7 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
     st.sum = Group<G>::sum(s, red);
     st.ref_sum = FULL ? Group<G>::sum(sq, red) : 1.0f;
     st.cross = FULL ? Group<G>::sum(cross, red) : 0.0f;
-    const bool counted = pr.counted && st.sum != 0.0;  // (0: nothing above -infinity; NaN counts)
+    const bool counted = pr.counted && st.sum != 0.0f;  // (0: nothing above -infinity; NaN counts)
 
     T *grad = a.grad ? (T *)a.grad + (size_t)row * a.d.ld : nullptr;
     if (!counted) {
@@ -451,7 +453,7 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
         }
         z_run.sum += s, q_run.sum += sq, cross += sc;
     }
-    RowStats st;
+    RowStats<double> st;
     st.top = Group<256>::max(z_run.top, red);
     const double f = z_run.scale(st.top);
     st.sum = Group<256>::sum64(z_run.sum * f, red64);
