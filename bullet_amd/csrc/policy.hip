@@ -31,11 +31,8 @@ __device__ __forceinline__ float exp_neg(float x) {
 
 // The scalars of a row in 64 bits, each computed by all its lanes, so shorter than the library's functions: their arguments
 // are finite sums and differences of logits, and 1e-13 is plenty.
-// e^x = 2^n e^r, n = round(x log2 e), |r| <= ln 2 / 2, by the Taylor series to r^11 / 11! (remainder below 1e-14).
-__device__ __forceinline__ double exp64(double x) {
-    const double n = rint(x * 1.4426950408889634074);
-    double r = fma(n, -6.93147180369123816490e-1, x);  // ln 2 in two parts, the first with zeros at its end
-    r = fma(n, -1.90821492927058770002e-10, r);
+// (e^r - 1 - r) / r^2 for |r| <= ln 2 / 2, by the Taylor series to r^11 / 11! (remainder below 1e-13)
+__device__ __forceinline__ double exp_rest(double r) {
     double p = 1.0 / 39916800.0;
     p = fma(p, r, 1.0 / 3628800.0);
     p = fma(p, r, 1.0 / 362880.0);
@@ -45,13 +42,29 @@ __device__ __forceinline__ double exp64(double x) {
     p = fma(p, r, 1.0 / 120.0);
     p = fma(p, r, 1.0 / 24.0);
     p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
+    return fma(p, r, 0.5);
+}
+// e^x = 2^n e^r, n = round(x log2 e)
+__device__ __forceinline__ double exp64(double x) {
+    const double n = rint(x * 1.4426950408889634074);
+    double r = fma(n, -6.93147180369123816490e-1, x);  // ln 2 in two parts, the first with zeros at its end
+    r = fma(n, -1.90821492927058770002e-10, r);
+    const double p = fma(fma(exp_rest(r), r, 1.0), r, 1.0);
     const double m = fmin(fmax(n, -1100.0), 1100.0);
     const double v = ldexp(p, (int)m);
     // (beyond the range of r's reduction, and infinities: the limits; NaN goes through)
     return x > 709.0 ? __builtin_huge_val() : x < -745.0 ? 0.0 : v;
+}
+// The estimate exp(x) - 1 - x of a KL and its derivative exp(x) - 1. Near 0 their own series: the difference would leave the
+// rounding of the 1, which is more than x^2 / 2 below |x| = 1e-8 and can be less than 0, what the estimate never is.
+__device__ __forceinline__ double kl_estimate(double x, double &em1) {
+    if (fabs(x) < 0.3) {
+        const double rest = x * x * exp_rest(x);
+        em1 = x + rest;
+        return rest;
+    }
+    em1 = exp64(x) - 1.0;
+    return em1 - x;
 }
 // log s for a normal s > 0: s = 2^n m, m in [sqrt 1/2, sqrt 2), log m = 2 atanh t, t = (m - 1) / (m + 1), |t| <= 0.172, by its
 // series to t^15 / 15 (remainder below 1e-14)
@@ -251,8 +264,8 @@ __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, con
     g.shift = 0.0f;
     if (d.kl == BT_KL_TAKEN) {
         const double x = (double)((const float *)a.ref)[row] - logp;
-        const double em1 = exp64(x) - 1.0;  // (off by 1e-15 of 1: d^2 / 2, what is left of small differences, stands 1e9 above)
-        kl = em1 - x;
+        double em1;
+        kl = kl_estimate(x, em1);
         slope -= (double)d.kl_weight * em1;
     } else if (full) {
         const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log64((double)st.ref_sum));

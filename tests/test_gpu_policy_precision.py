@@ -122,3 +122,35 @@ def test_small_entries_of_a_gradient_keep_their_digits(width):
     for name, g in grads.items():
         off = np.abs(g[:, 1:] / g[:, 1:2] / want - 1.0)
         assert off.max() <= bound, (name, off.max(), x[:, 1:][off > bound][:3])
+
+
+# ---------------------------------------------------------------- KL of the move taken
+def series(x, first):
+    """sum over k >= first of x^k / k!, for |x| <= 1, smallest terms first"""
+    x, term, terms = np.asarray(x, np.longdouble), np.ones_like(x, np.longdouble), []
+    for k in range(1, 30):
+        term = term * x / k
+        if k >= first:
+            terms.append(term)
+    return sum(reversed(terms))
+
+
+def only_move(ref, klw=1.0, adv=None):
+    """rows with one legal move: its log-probability is exactly 0 and its ratio 1, so the KL is that of d = ref"""
+    n = len(ref)
+    z = dev(np.random.default_rng(42).standard_normal((n, 9)))
+    mask = np.zeros((n, 9))
+    mask[:, 3] = 1
+    return policy(z, np.full(n, 3), np.zeros(n), np.zeros(n) if adv is None else adv, kl="taken", ref=dev(ref), mask=mask, klw=klw)
+
+
+def test_the_kl_estimate_is_never_negative_and_keeps_its_digits():
+    """d from 1e-18 to 1 of either sign: KL = exp(d) - d - 1 = d^2 / 2 + ..., off by the output's rounding and 1e-12 (64-bit
+    series and, beyond 0.3, differences of 1e-15 next to 0.04)"""
+    d = np.float32(np.exp(np.random.default_rng(43).uniform(np.log(1e-18), 0.0, 3000)))
+    d = np.concatenate([d, -d, np.float32([0.0, 0.2999999, 0.3, 0.3000001, -0.2999999, -0.3, -0.3000001, 0.34657359, -0.34657359])])
+    _, _, row_loss, logp, kl = only_move(d)
+    want = series(d, 2).astype(np.float64)
+    assert (logp == 0).all() and (kl >= 0).all()
+    assert (np.abs(kl - want) <= want * (2.0 ** -24 * 1.0001 + 1e-12) + 2.0 ** -149).all()
+    assert (row_loss == kl).all()
