@@ -64,7 +64,7 @@ __device__ __forceinline__ double kl_estimate(double x, double &em1) {
         return rest;
     }
     em1 = exp64(x) - 1.0;
-    return em1 - x;
+    return em1 < __builtin_huge_val() ? em1 - x : em1;  // (a move at -infinity, x = infinity: not infinity - infinity)
 }
 // log s for a normal s > 0: s = 2^n m, m in [sqrt 1/2, sqrt 2), log m = 2 atanh t, t = (m - 1) / (m + 1), |t| <= 0.172, by its
 // series to t^15 / 15 (remainder below 1e-14)
@@ -218,7 +218,7 @@ __device__ __forceinline__ typename Row<T>::vec grad_chunk(const float (&e)[Row<
 #pragma unroll
         for (int j = 0; j < Row<T>::V; j++) {
             float g = r.ce * e[j];
-            if (FULL) g = fmaf(r.ck * e[j], ((float)z[j] - (float)q[j]) - r.shift, g);
+            if (FULL && r.ck != 0.0f) g = fmaf(r.ck * e[j], ((float)z[j] - (float)q[j]) - r.shift, g);
             out[j] = (T)(e[j] == 0.0f ? 0.0f : g);
         }
     } else {
@@ -266,14 +266,16 @@ __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, con
         const double x = (double)((const float *)a.ref)[row] - logp;
         double em1;
         kl = kl_estimate(x, em1);
-        slope -= (double)d.kl_weight * em1;
+        if (d.kl_weight != 0.0f) slope -= (double)d.kl_weight * em1;
     } else if (full) {
         const double dl = ((double)st.top + logsum) - ((double)st.ref_top + log64((double)st.ref_sum));
         kl = (double)st.cross / (double)st.sum - dl;
         ck = w * (double)d.kl_weight;
         g.shift = (float)(dl + kl);
     }
-    loss = (float)(w * ((double)d.kl_weight * kl - (free_gain != free_gain ? free_gain : fmin(free_gain, held_gain))));
+    // (no weight: a KL that is infinite is none either; NaN stays)
+    const double held_kl = d.kl_weight != 0.0f || kl != kl ? (double)d.kl_weight * kl : 0.0;
+    loss = (float)(w * (held_kl - (free_gain != free_gain ? free_gain : fmin(free_gain, held_gain))));
     g.top = st.top == NEG_INF ? 0.0f : st.top;  // (nothing but NaN)
     const float inv = 1.0f / (float)st.sum;
     g.ce = -(float)(w * slope) * inv;
@@ -281,7 +283,7 @@ __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, con
     g.plain = fabsf(g.ce) < __builtin_huge_valf();
     const double pa = exp64(logp);
     grad_taken = (float)(w * slope * (1.0 - pa));
-    if (full && pa > 0.0) grad_taken += (float)(ck * pa * (((double)pr.za - (double)pr.qa) - (double)g.shift));
+    if (full && pa > 0.0 && ck != 0.0) grad_taken += (float)(ck * pa * (((double)pr.za - (double)pr.qa) - (double)g.shift));
     return near;
 }
 

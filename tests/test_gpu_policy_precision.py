@@ -154,3 +154,32 @@ def test_the_kl_estimate_is_never_negative_and_keeps_its_digits():
     assert (logp == 0).all() and (kl >= 0).all()
     assert (np.abs(kl - want) <= want * (2.0 ** -24 * 1.0001 + 1e-12) + 2.0 ** -149).all()
     assert (row_loss == kl).all()
+
+
+@pytest.mark.parametrize("width", [40, 3000, 20001])
+def test_a_move_that_has_become_impossible(width):
+    """the move taken stands at -infinity among legal moves: l[a] = -infinity, ratio 0, KL = infinity and with it the loss, which a
+    weight of 0 leaves out"""
+    z = torch.zeros(2, width, device="cuda")
+    z[0, 3] = -INF
+    args = (z, np.full(2, 3), np.full(2, -np.log(width)), np.ones(2))
+    loss, grad, row_loss, logp, kl = policy(*args, kl="taken", ref=dev([-1.0, -np.log(width)]))
+    assert logp[0] == -INF and kl[0] == INF and row_loss[0] == INF and loss[0] == INF
+    assert grad[0, 3] == -INF and (np.delete(grad[0], 3) == INF).all() and np.isfinite(grad[1]).all() and np.isfinite(row_loss[1])
+    loss, grad, row_loss, logp, kl = policy(*args, kl="taken", ref=dev([-1.0, -np.log(width)]), klw=0.0)
+    plain = policy(*args)
+    assert kl[0] == INF and row_loss[0] == 0.0 and np.isfinite(loss).all() and np.isfinite(grad).all()
+    assert np.array_equal(grad, plain[1]) and np.array_equal(row_loss, plain[2])
+
+
+@pytest.mark.parametrize("width", [40, 3000, 20001])
+def test_a_reference_policy_without_a_move_that_has_a_share(width):
+    z = torch.zeros(2, width, device="cuda")
+    ref = z.clone()
+    ref[0, 7] = -INF
+    args = (z, np.full(2, 3), np.full(2, -np.log(width)), np.ones(2))
+    loss, _, row_loss, _, kl = policy(*args, kl="full", ref=ref)
+    assert kl[0] == INF and row_loss[0] == INF and loss[0] == INF and np.isfinite(kl[1])
+    loss, grad, row_loss, _, kl = policy(*args, kl="full", ref=ref, klw=0.0)
+    plain = policy(*args)
+    assert kl[0] == INF and np.array_equal(loss, plain[0]) and np.array_equal(grad, plain[1]) and np.array_equal(row_loss, plain[2])
