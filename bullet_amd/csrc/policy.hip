@@ -66,17 +66,19 @@ __device__ __forceinline__ double kl_estimate(double x, double &em1) {
     em1 = exp64(x) - 1.0;
     return em1 < __builtin_huge_val() ? em1 - x : em1;  // (a move at -infinity, x = infinity: not infinity - infinity)
 }
+// 1 / d: the hardware's estimate, squared twice in its error by Newton's steps
+__device__ __forceinline__ double inverse64(double d) {
+    double i = __builtin_amdgcn_rcp(d);
+    i = i * fma(-d, i, 2.0);
+    return i * fma(-d, i, 2.0);
+}
 // log s for a normal s > 0: s = 2^n m, m in [sqrt 1/2, sqrt 2), log m = 2 atanh t, t = (m - 1) / (m + 1), |t| <= 0.172, by its
 // series to t^15 / 15 (remainder below 1e-14)
 __device__ __forceinline__ double log64(double s) {
     int n;
     double m = frexp(s, &n);  // [1/2, 1)
     if (m < 0.70710678118654752440) m *= 2.0, n -= 1;
-    const double d = m + 1.0;
-    double i = __builtin_amdgcn_rcp(d);
-    i = i * fma(-d, i, 2.0);
-    i = i * fma(-d, i, 2.0);
-    const double t = (m - 1.0) * i, u = t * t;
+    const double t = (m - 1.0) * inverse64(m + 1.0), u = t * t;
     double p = 2.0 / 15.0;
     p = fma(p, u, 2.0 / 13.0);
     p = fma(p, u, 2.0 / 11.0);
@@ -277,9 +279,9 @@ __device__ __forceinline__ bool policy_scalars(const PolicyArgs &a, int row, con
     const double held_kl = d.kl_weight != 0.0f || kl != kl ? (double)d.kl_weight * kl : 0.0;
     loss = (float)(w * (held_kl - (free_gain != free_gain ? free_gain : fmin(free_gain, held_gain))));
     g.top = st.top == NEG_INF ? 0.0f : st.top;  // (nothing but NaN)
-    const float inv = 1.0f / (float)st.sum;
-    g.ce = -(float)(w * slope) * inv;
-    g.ck = (float)ck * inv;
+    const double inv = inverse64((double)st.sum);
+    g.ce = -(float)(w * slope * inv);
+    g.ck = (float)(ck * inv);
     g.plain = fabsf(g.ce) < __builtin_huge_valf();
     const double pa = exp64(logp);
     grad_taken = (float)(w * slope * (1.0 - pa));
@@ -659,7 +661,7 @@ __global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
         const double c = h ? -slope : slope;
         const auto put = [&](long long r, const Entry &e) {
             const bool counted = e.sum != 0.0f;
-            a.ce[r] = counted ? -(float)c * (1.0f / e.sum) : 0.0f;
+            a.ce[r] = counted ? -(float)(c * inverse64((double)e.sum)) : 0.0f;
             a.taken[r] = counted ? (float)(c * (1.0 - exp64(e.logp))) : 0.0f;
         };
         if (r0[h] < r1[h]) put(r0[h], first[h]);

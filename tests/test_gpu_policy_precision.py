@@ -183,3 +183,28 @@ def test_a_reference_policy_without_a_move_that_has_a_share(width):
     loss, grad, row_loss, _, kl = policy(*args, kl="full", ref=ref, klw=0.0)
     plain = policy(*args)
     assert kl[0] == INF and np.array_equal(loss, plain[0]) and np.array_equal(grad, plain[1]) and np.array_equal(row_loss, plain[2])
+
+
+# ---------------------------------------------------------------- what a row's gradient is scaled by
+@pytest.mark.parametrize("width", [3, 7, 100, 1879, 5001, 20001])
+def test_gradients_of_equal_logits_are_rounded_once(width):
+    """p = 1 / width and every exponential is exactly 1, so that a gradient is a 64-bit scalar rounded to 32 bits"""
+    n = 200
+    rng = np.random.default_rng(44)
+    z, actions = torch.zeros(n, width, device="cuda"), np.zeros(n)
+    lp = -np.log(np.float64(width))
+    old = np.float32(lp + 0.1 * rng.standard_normal(n))
+    adv = rng.standard_normal(n).astype(np.float32)
+    r, bound = np.exp(lp - old.astype(np.float64)), 2.0 ** -24 * 1.0001 + 1e-12
+    free = (r * adv <= np.clip(r, 1 - np.float64(np.float32(0.2)), 1 + np.float64(np.float32(0.28))) * adv)
+    want = np.where(free, r * adv / width, 0.0)[:, None]
+    g = policy(z, actions, old, adv)[1][:, 1:]
+    assert (np.abs(g - want) <= np.abs(want) * bound).all(), np.abs(g / want - 1).max()
+
+    ref = np.float32(2.0 * rng.standard_normal(n))
+    beta, eps = np.float64(np.float32(0.1)), np.float64(np.float32(0.05))
+    d = beta * (ref[1::2].astype(np.float64) - ref[0::2])
+    c = beta * (eps - 1.0 / (1.0 + np.exp(d)))
+    want = (np.stack([-c, c], 1).reshape(-1) / width)[:, None]
+    g = preference(z, actions, np.arange(n + 1), ref)[1][:, 1:]
+    assert (np.abs(g - want) <= np.abs(want) * bound).all(), np.abs(g / want - 1).max()
