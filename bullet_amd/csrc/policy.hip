@@ -652,7 +652,8 @@ __global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
     const double slope = w * beta * (eps - 1.0 / (1.0 + exp64(x)));
     if (lane == 0) {
         const double soft = log1p(exp64(-fabs(x)));  // -log sigmoid(x) = soft - min(x, 0)
-        a.pair_loss[p] = (float)(w * ((1.0 - eps) * (soft - fmin(x, 0.0)) + eps * (soft + fmax(x, 0.0))));
+        const double other = eps > 0.0 || x != x ? eps * (soft + fmax(x, 0.0)) : 0.0;  // (an infinite one that has no share is none)
+        a.pair_loss[p] = (float)(w * ((1.0 - eps) * (soft - fmin(x, 0.0)) + other));
         if (a.line_logp) a.line_logp[2 * p] = (float)s[0], a.line_logp[2 * p + 1] = (float)s[1];
     }
     if (!a.grad) return;

@@ -208,3 +208,25 @@ def test_gradients_of_equal_logits_are_rounded_once(width):
     want = (np.stack([-c, c], 1).reshape(-1) / width)[:, None]
     g = preference(z, actions, np.arange(n + 1), ref)[1][:, 1:]
     assert (np.abs(g - want) <= np.abs(want) * bound).all(), np.abs(g / want - 1).max()
+
+
+# ---------------------------------------------------------------- infinite margins
+@pytest.mark.parametrize("smoothing", [0.0, 0.05])
+@pytest.mark.parametrize("line", [0, 1])
+def test_a_line_with_an_impossible_move(line, smoothing):
+    """one line's move stands at -infinity: the margin is infinite. The loss is 0 where the preferred line wins for sure, infinite
+    where the other one does, and with smoothing infinite either way; no gradient is NaN, nor is anything of the other pair"""
+    z = torch.zeros(4, 30, device="cuda")
+    z[line, 5] = -INF
+    loss, grad, pair, lp = preference(z, np.full(4, 5), np.arange(5), np.zeros(4), smoothing=smoothing)
+    assert lp[line] == -INF and np.isfinite(np.delete(lp, line)).all()
+    assert pair[0] == (0.0 if line == 1 and smoothing == 0.0 else INF)
+    log2 = np.log(2.0)
+    assert abs(pair[1] - log2) <= log2 * (2.0 ** -24 * 1.0001 + 1e-12) and loss[0] == pair.sum().astype(np.float32)
+    beta, eps = np.float64(np.float32(0.1)), np.float64(np.float32(smoothing))
+    c = beta * (eps - (1.0 if line == 0 else 0.0))  # the slope at its limits
+    row = [c, -c][line]
+    want = np.full(30, -row / 29)  # the row with the impossible move: p = 1 / 29 for the others
+    want[5] = row
+    assert (np.abs(grad[line] - want) <= np.abs(want) * (2.0 ** -24 * 1.0001 + 1e-12)).all()
+    assert np.isfinite(grad).all()
