@@ -47,8 +47,9 @@ __device__ __forceinline__ double exp_rest(double r) {
 // e^x = 2^n e^r, n = round(x log2 e)
 __device__ __forceinline__ double exp64(double x) {
     const double n = rint(x * 1.4426950408889634074);
-    double r = fma(n, -6.93147180369123816490e-1, x);  // ln 2 in two parts, the first with zeros at its end
-    r = fma(n, -1.90821492927058770002e-10, r);
+    // (x - n ln 2 after Cody and Waite: of ln 2 first its 40 leading bits, whose product with n is exact, then the rest)
+    double r = fma(n, -0x1.62e42fefa2p-1, x);
+    r = fma(n, -0x1.9ef35793c7673p-41, r);
     const double p = fma(fma(exp_rest(r), r, 1.0), r, 1.0);
     const double m = fmin(fmax(n, -1100.0), 1100.0);
     const double v = ldexp(p, (int)m);
