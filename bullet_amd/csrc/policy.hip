@@ -302,6 +302,9 @@ __device__ __forceinline__ PolicyRow policy_row_begin(const PolicyArgs &a, const
     }
     return pr;
 }
+// The gradient may lie where the logits are: the move's logit has to be here in every wave of a row before the barrier behind
+// which another one of them may write there.
+__device__ __forceinline__ void taken_is_here(const PolicyRow &pr) { asm volatile("" : : "v"(pr.za) : "memory"); }
 __device__ __forceinline__ void policy_row_out(const PolicyArgs &a, int row, bool counted, float loss, double logp, double kl) {
     a.row_loss[row] = counted ? loss : 0.0f;
     if (a.row_logp) a.row_logp[row] = counted ? (float)logp : 0.0f;
@@ -376,6 +379,7 @@ __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
                 cross += e[k][j] == 0.0f ? 0.0f : e[k][j] * (zv - qv);
             }
         }
+    if (G > 64) taken_is_here(pr);
     st.sum = Group<G>::sum(s, red);
     st.ref_sum = FULL ? Group<G>::sum(sq, red) : 1.0f;
     st.cross = FULL ? Group<G>::sum(cross, red) : 0.0f;
@@ -473,6 +477,7 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
     }
     RowStats<double> st;
     st.top = Group<256>::max(z_run.top, red);
+    taken_is_here(pr);
     const double f = z_run.scale(st.top);
     st.sum = Group<256>::sum64(z_run.sum * f, red64);
     st.ref_top = FULL ? Group<256>::max(q_run.top, red) : 0.0f;
