@@ -712,7 +712,7 @@ __device__ __forceinline__ void gz_block(const Gz<T> &G, int block) {
     const long long b0 = (long long)by * G.range, b1 = b0 + G.range < G.batch ? b0 + G.range : G.batch;
     const int left = e < G.n ? (int)(G.n - e < V ? G.n - e : V) : 0;
     const bool root = G.act == BT_ACT_SCRELU || G.act == BT_ACT_SQRRELU;
-    const float top = G.act == BT_ACT_CRELU || G.act == BT_ACT_SCRELU ? 1.0f : __builtin_huge_valf();
+    const bool clipped = G.act == BT_ACT_CRELU || G.act == BT_ACT_SCRELU;
     float sum[V];
 #pragma unroll
     for (int j = 0; j < V; j++) sum[j] = 0.0f;
@@ -732,9 +732,10 @@ __device__ __forceinline__ void gz_block(const Gz<T> &G, int block) {
             }
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                // bt_act_deriv, halved where it has a factor 2, without its branches (for every output an activation has)
+                // bt_act_deriv, halved where it has a factor 2, without its branches (for every output an activation has; one that
+                // was too large for the type, infinity, has ReLU's slope 1 and squared ReLU's infinity)
                 const float a = (float)o[j];
-                float slope = a > 0.0f && a < top ? 1.0f : 0.0f;
+                float slope = a > 0.0f && (!clipped || a < 1.0f) ? 1.0f : 0.0f;
                 if (root) slope *= __builtin_amdgcn_sqrtf(a);
                 const float v = po ? (float)g[j] * slope : (float)g[j];
                 sum[j] += v;
