@@ -195,13 +195,13 @@ __device__ __forceinline__ void finish_at(const Epilogue &e, int row, int c, int
         Cols<T, W>::store((T *)e.out + at, v * e.alpha, n, e.past);
     } else {
         v += bias;
-        // bt_act_fwd without its branches: this is unrolled over a whole tile
+        // bt_act_fwd without its branches, but for NaN: this is unrolled over a whole tile
         const float top = e.act == BT_ACT_CRELU || e.act == BT_ACT_SCRELU ? 1.0f : __builtin_huge_valf();
         const bool clamp = e.act != BT_ACT_IDENTITY, square = e.act == BT_ACT_SCRELU || e.act == BT_ACT_SQRRELU;
 #pragma unroll
         for (int j = 0; j < W; j++) {
             const float a = fminf(fmaxf(v[j], 0.0f), top), b = square ? a * a : a;
-            v[j] = clamp ? b : v[j];
+            v[j] = clamp && v[j] == v[j] ? b : v[j];  // (NaN stays: a layer that has diverged shows)
         }
         if (e.saved) Cols<T, W>::store((T *)e.saved + at, v, n, e.past);
         if (e.residual) {

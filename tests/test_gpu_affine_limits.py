@@ -78,3 +78,25 @@ def test_squared_relu_at_infinity(kind):
     backward(kind, "sqrrelu", None, x, o, gy, dw, db, None)
     rest = [c for c in range(24) if c != 7]
     assert db[7] == INF and (dw[:, 7] == INF).all() and (db[rest] == 5).all() and (dw[:, rest] == 5).all()
+
+
+@pytest.mark.parametrize("act", ["identity", "relu", "crelu", "screlu", "sqrrelu"])
+@pytest.mark.parametrize("kind", tg.KINDS)
+def test_nan_shows_behind_every_activation(kind, act):
+    """a NaN input makes its row of outputs NaN, a NaN weight its column; infinities become what the activation makes of them"""
+    for batch, in_, out in ((1, 20, 40), (3, 300, 70), (70, 90, 150), (300, 513, 700)):
+        x, w = torch.full((batch, in_), 0.5, device="cuda", dtype=DT[kind]), torch.zeros(in_, out, device="cuda", dtype=DT[kind])
+        w[3, 7], w[5, 9], w[5, 10] = float("nan"), INF, -INF
+        x[batch // 2, 1] = float("nan") if batch > 1 else 0.5
+        y, res = torch.zeros(batch, out, device="cuda", dtype=DT[kind]), torch.zeros(batch, out, device="cuda", dtype=DT[kind])
+        saved = torch.zeros_like(y)
+        forward(kind, act, w, x, y, saved=saved, residual=res)
+        want = torch.zeros(batch, out)
+        want[:, 9] = 1.0 if act in ("crelu", "screlu") else INF
+        want[:, 10] = -INF if act == "identity" else 0.0
+        want[:, 7] = float("nan")
+        if batch > 1:
+            want[batch // 2] = float("nan")
+        for t in (y, saved):
+            t = t.float().cpu()
+            assert torch.equal(t.isnan(), want.isnan()) and torch.equal(t.nan_to_num(7.0), want.nan_to_num(7.0)), (batch, in_, out)
