@@ -259,7 +259,7 @@ struct Product {
 // the N youngest loads), in front of the barrier behind which the chunk is read. The s_nop is the wait state between m0 and
 // its use.
 __device__ __forceinline__ void to_lds(const char *base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" : : "v"(offset), "s"(lds), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" : : "v"(offset), "s"(lds), "s"(base) : "memory", "m0");
 }
 template <int N = 0>
 __device__ __forceinline__ void wait_loads() {
