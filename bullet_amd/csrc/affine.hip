@@ -214,6 +214,14 @@ __device__ __forceinline__ void finish_at(const Epilogue &e, int row, int c, int
 
 constexpr float F16_LIFT = 2048.0f;  // between the two summands of an f16 gradient (affine_gz)
 
+// a launch holds less than 2^32 threads a dimension: many workgroups fold into the grid's second one (the last of its rows may
+// hold some that have no work)
+__device__ __forceinline__ long long folded_block() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 folded(long long blocks) {
+    constexpr long long W = 1 << 21;
+    return dim3((unsigned)(blocks < W ? blocks : W), (unsigned)((blocks + W - 1) / W));
+}
+
 // dbias from the row ranges' sums that affine_prepare leaves, by workgroups of their own behind a product's
 struct BiasSum {
     const float *part;  // [parts][n]
@@ -224,6 +232,7 @@ struct BiasSum {
 constexpr int BIAS_COLS = 32;
 template <int NT>
 __device__ __forceinline__ void bias_sum(const BiasSum b, int block, float *lds) {  // lds: NT floats
+    if (block >= b.blocks) return;
     const int c = threadIdx.x % BIAS_COLS, r = threadIdx.x / BIAS_COLS, col = block * BIAS_COLS + c;
     float s = 0.0f;
     if (col < b.n)
@@ -237,7 +246,7 @@ __device__ __forceinline__ void bias_sum(const BiasSum b, int block, float *lds)
 }
 __global__ __launch_bounds__(256) void affine_dbias(BiasSum b) {
     __shared__ float lds[256];
-    bias_sum<256>(b, blockIdx.x, lds);
+    bias_sum<256>(b, (int)folded_block(), lds);
 }
 
 struct Product {
@@ -252,8 +261,8 @@ struct Product {
     long long part_ld;
     Epilogue e;
     BiasSum bias;
+    int wgs;             // workgroups of the product; bias.blocks more follow them in its launch
 };
-
 // A chunk straight from memory into LDS, 16 bytes a lane: lane l's lands 16 l bytes behind `lds` (the same in all lanes).
 // Written out, since the compiler lets every LDS read wait for all such loads of its own; wait_loads() is the wait (for all but
 // the N youngest loads), in front of the barrier behind which the chunk is read. The s_nop is the wait state between m0 and
@@ -365,14 +374,14 @@ struct Mm {
     uint32_t at_a, at_b;  // where this lane reads a tile of the first buffer
     v4f acc[FN][FM];
 
-    // workgroup `wg` of the product's `wgs`
-    __device__ __forceinline__ Mm(const Product &P_, char *lds_, int wg, int wgs)
+    // workgroup `wg` of the product's
+    __device__ __forceinline__ Mm(const Product &P_, char *lds_, int wg)
         : P(P_), a(P_.a.pinned()), b(P_.b.pinned()), lds(lds_) {
         tid = threadIdx.x, lane = tid & 63;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         wm = wave / WN, wn = wave % WN;
         int tm, tn;
-        tile_of(wg, wgs, P.tiles_m, P.tiles_n, split, tm, tn);
+        tile_of(wg, P.wgs, P.tiles_m, P.tiles_n, split, tm, tn);
         m0 = tm * BM, n0 = tn * BN;
         at_a = lds_address(lds) + TA::origin(wm * FM, lane), at_b = lds_address(lds) + TA::BYTES + TB::origin(wn * FN, lane);
 #pragma unroll
@@ -468,9 +477,9 @@ template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT
 __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
     typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
     extern __shared__ __align__(1024) char lds[];
-    if (blockIdx.x >= gridDim.x - P.bias.blocks)
-        return bias_sum<M::NT>(P.bias, blockIdx.x - (gridDim.x - P.bias.blocks), (float *)lds);
-    M mm(P, lds, blockIdx.x, gridDim.x - P.bias.blocks);
+    const int wg = (int)folded_block();
+    if (wg >= P.wgs) return bias_sum<M::NT>(P.bias, wg - P.wgs, (float *)lds);
+    M mm(P, lds, wg);
     const int ktiles = (P.k + M::BK - 1) / M::BK;
     int p0, p1, t0, t1;
     mm.share(ktiles, p0, p1, t0, t1);
@@ -505,13 +514,12 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 // conflicts are few); dW of 16384 x 2048 -> 2048 with 4 workgroups to a tile 110 us and grad_x 109, 1.25 PFLOP/s;
 // 4096 x 1024 -> 1024 f32 with 64 x 64 tiles 66 us, 130 TFLOP/s, 83 % of the rate of f32.
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
-__device__ __forceinline__ void mm_direct(const Product &P, int wg, int wgs, char *lds) {
+__device__ __forceinline__ void mm_direct(const Product &P, int wg, char *lds) {
     typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
     typedef typename M::frag frag;
     constexpr int FM = M::FM, FN = M::FN, NA = M::SA::N, NB = M::SB::N;
-    wgs -= P.bias.blocks;
-    if (wg >= wgs) return bias_sum<M::NT>(P.bias, wg - wgs, (float *)lds);
-    M mm(P, lds, wg, wgs);
+    if (wg >= P.wgs) return bias_sum<M::NT>(P.bias, wg - P.wgs, (float *)lds);
+    M mm(P, lds, wg);
     const bool ragged = M::SA::ragged(mm.a, mm.m0) || M::SB::ragged(mm.b, mm.n0);
     const int full = (P.k - ragged) / M::BK;
     int p0, p1, t0, t1;
@@ -609,24 +617,25 @@ __device__ __forceinline__ void mm_direct(const Product &P, int wg, int wgs, cha
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     extern __shared__ __align__(1024) char lds[];
-    mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT, BUFS>(P, blockIdx.x, gridDim.x, lds);
+    mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT, BUFS>(P, (int)folded_block(), lds);
 }
 // dW and grad_x of a small layer in one launch: neither has tiles enough to fill the chip, or to hide its own latency
 // (200 x 512 -> 333 f32: 8 us, 288 workgroups of 32 x 32 that each walk their whole k; 76 of 64 x 64: 11)
 template <typename T, int B, int OUT_W, int OUT_X, int BUFS>
-__global__ __launch_bounds__(256, 2) void affine_mm_both(Product W, Product X, int wgs) {  // wgs: W's
+__global__ __launch_bounds__(256, 2) void affine_mm_both(Product W, Product X) {
     extern __shared__ __align__(1024) char lds[];
-    if ((int)blockIdx.x < wgs)
-        mm_direct<T, B, B, 2, 2, false, false, OUT_W, BUFS>(W, blockIdx.x, wgs, lds);
+    const int wg = (int)folded_block(), first = W.wgs + W.bias.blocks;
+    if (wg < first)
+        mm_direct<T, B, B, 2, 2, false, false, OUT_W, BUFS>(W, wg, lds);
     else
-        mm_direct<T, B, B, 2, 2, true, true, OUT_X, BUFS>(X, blockIdx.x - wgs, gridDim.x - wgs, lds);
+        mm_direct<T, B, B, 2, 2, true, true, OUT_X, BUFS>(X, wg - first, lds);
 }
 
 // The splits' sums added in order, then the epilogue. Memory bound: 4 splits of 2048 x 2048 (67 MB of sums, 8 MB out) 13 us,
 // 5.8 TB/s.
 template <typename T, int OUT>
 __global__ __launch_bounds__(256) void affine_join(Product P) {
-    const long long q = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x, cols = P.part_ld / 4;
+    const long long q = folded_block() * 256 + threadIdx.x, cols = P.part_ld / 4;
     if (q >= cols * P.m) return;
     const int m = (int)(q / cols), n = (int)(q % cols) * 4;
     v4f v = {0, 0, 0, 0};
@@ -773,7 +782,7 @@ struct Prepare {
 };
 template <typename T, int NP>  // NP = 0: copies only
 __global__ __launch_bounds__(256) void affine_prepare(Prepare<T> p) {
-    long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+    long long block = folded_block();
     if constexpr (NP > 0) {
         if (block < p.gz.blocks) return gz_block<T, NP>(p.gz, (int)block);
         block -= p.gz.blocks;
@@ -797,7 +806,9 @@ __global__ __launch_bounds__(few_threads(R)) void affine_few(const TW *__restric
     typedef typename Elem<T>::frag xvec;
     __shared__ __align__(16) float red[NT / 64][R][COLS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = threadIdx.x >> 2;
-    const int chunk = xcd_share(blockIdx.x, gridDim.x);  // (neighbours read halves of the same lines)
+    const int all = (out + COLS - 1) / COLS;
+    if (folded_block() >= all) return;
+    const int chunk = xcd_share((int)folded_block(), all);  // (neighbours read halves of the same lines)
     const int c = chunk * COLS + (threadIdx.x & 3) * V;
     float acc[R][V];
 #pragma unroll
@@ -927,12 +938,6 @@ Shape shape_of(int m, int n, int k, int passes, size_t es, bool lift = false, in
     return best;
 }
 
-// a launch holds less than 2^32 threads a dimension: many workgroups fold into the grid's second one
-dim3 folded(long long blocks) {
-    constexpr long long W = 1 << 22;
-    return dim3((unsigned)(blocks < W ? blocks : W), (unsigned)((blocks + W - 1) / W));
-}
-
 // Buffers for direct loads. A third one keeps two tiles on their way at any time, which a workgroup that is alone on its CU
 // needs: the products of a 64 x 64 tile take a third of a load's latency. Where more workgroups share a CU they hide it from
 // each other, and need the LDS. (bf16 dW of 2048 x 1024 -> 1024, 256 workgroups: 21.5 us with two, 15.7 with three; f32 4096 x
@@ -951,9 +956,7 @@ int direct_launch(hipStream_t st, const Product &P, dim3 grid) {
 }
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT>
 int mm_launch(hipStream_t st, const Product &P, bool direct) {
-    const long long blocks = (long long)P.tiles_m * P.tiles_n * P.splits;
-    BT_REQUIRE((blocks + P.bias.blocks) * 64 * WM * WN < (1ll << 32), "bt_affine: Mismatched sizes! (%lld tiles)", blocks);
-    const dim3 grid((unsigned)(blocks + P.bias.blocks));
+    const dim3 grid = folded((long long)P.wgs + P.bias.blocks);
     if constexpr (BM <= 128) {
         if (!direct) {
             const size_t lds = 2 * Mm<T, BM, BN, WM, WN, AK, BKC, OUT>::BYTES;
@@ -963,7 +966,7 @@ int mm_launch(hipStream_t st, const Product &P, bool direct) {
             BT_LAUNCH_CHECK();
             return BT_OK;
         }
-        if (blocks <= three_up_to(BM)) return direct_launch<T, BM, BN, WM, WN, AK, BKC, OUT, 3>(st, P, grid);
+        if (P.wgs <= three_up_to(BM)) return direct_launch<T, BM, BN, WM, WN, AK, BKC, OUT, 3>(st, P, grid);
     }
     return direct_launch<T, BM, BN, WM, WN, AK, BKC, OUT, 2>(st, P, grid);
 }
@@ -978,7 +981,8 @@ int tile_launch(hipStream_t st, const Product &P, const Shape &s, bool direct) {
     return mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT>(st, P, direct);
 }
 void set_shape(Product &P, const Shape &s) {
-    P.tiles_m = s.tiles_m, P.tiles_n = s.tiles_n, P.splits = s.splits;
+    // (of at most 2^36 outputs, tiles of 64 x 64 are less than 2^26, of 32 x 32 less than 2^28; shared only where they are few)
+    P.tiles_m = s.tiles_m, P.tiles_n = s.tiles_n, P.splits = s.splits, P.wgs = s.tiles_m * s.tiles_n * s.splits;
     P.part_ld = (P.n + 3) / 4 * 4;
 }
 template <typename T, int OUT>
@@ -999,16 +1003,15 @@ int product_launch(hipStream_t st, Product &P, Shape s) {
 // both products of a backward pass, each with its sums in a place of its own
 template <typename T, int B, int OUT_W, int OUT_X>
 int both_launch(hipStream_t st, const Product &W, const Product &X) {
-    const long long w = (long long)W.tiles_m * W.tiles_n * W.splits + W.bias.blocks, x = (long long)X.tiles_m * X.tiles_n * X.splits;
-    BT_REQUIRE((w + x) * 256 < (1ll << 32), "bt_affine_backward: Mismatched sizes! (%lld tiles)", w + x);
+    const long long all = (long long)W.wgs + W.bias.blocks + X.wgs;
     typedef Mm<T, B, B, 2, 2, false, false, OUT_W> MW;
     typedef Mm<T, B, B, 2, 2, true, true, OUT_X> MX;
     static_assert(MW::BYTES == MX::BYTES && 3 * MW::BYTES <= 65536, "tiles of one size, within what needs no attribute");
-    const dim3 grid((unsigned)(w + x)), block(256);
-    if (w + x <= three_up_to(B))
-        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, B, OUT_W, OUT_X, 3>), grid, block, 3 * MW::BYTES, W, X, (int)w);
+    const dim3 grid = folded(all), block(256);
+    if (all <= three_up_to(B))
+        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, B, OUT_W, OUT_X, 3>), grid, block, 3 * MW::BYTES, W, X);
     else
-        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, B, OUT_W, OUT_X, 2>), grid, block, 2 * MW::BYTES, W, X, (int)w);
+        BT_LAUNCH(BTK_AFFINE, st, (affine_mm_both<T, B, OUT_W, OUT_X, 2>), grid, block, 2 * MW::BYTES, W, X);
     BT_LAUNCH_CHECK();
     return BT_OK;
 }
@@ -1098,7 +1101,7 @@ int prepare_launch(hipStream_t st, const Prepare<T> &p, int np) {
 int few_rows(const bt_affine_desc *d) { return d->w_type == BT_TYPE_F32 ? 8 : 4; }
 template <typename T, typename TW>
 int few_launch(hipStream_t st, const bt_affine_desc *d, const void *w, const void *x, const Epilogue &e) {
-    const dim3 grid(bt_div_up(d->out, 4 * Elem<T>::V));
+    const dim3 grid = folded(bt_div_up(d->out, 4 * Elem<T>::V));
 #define FEW_CASE(R)                                                                                                         \
     BT_LAUNCH(BTK_AFFINE, st, (affine_few<T, TW, R>), grid, dim3(few_threads(R)), 0, (const TW *)w, (long long)d->w_ld,     \
               (const T *)x, (long long)d->x_ld, d->batch, d->in, d->out, e)
@@ -1214,7 +1217,7 @@ int backward(hipStream_t st, const bt_affine_desc *d, const void *w, const void 
     BiasSum bias = {};
     if (dbias) bias = BiasSum{(const float *)sums, dbias, p.ranges, d->out, bt_div_up(d->out, BIAS_COLS), p.alpha};
     if (dbias && !dw && !gx) {
-        BT_LAUNCH(BTK_AFFINE, st, affine_dbias, dim3(bias.blocks), dim3(256), 0, bias);
+        BT_LAUNCH(BTK_AFFINE, st, affine_dbias, folded(bias.blocks), dim3(256), 0, bias);
         BT_LAUNCH_CHECK();
     }
     const auto gz_operand = [&](int n) {  // its n largest summands, the smallest of them first

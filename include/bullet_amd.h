@@ -283,7 +283,8 @@ enum { BT_TYPE_F32 = 0, BT_TYPE_BF16 = 1, BT_TYPE_F16 = 2 };
  * optimiser's own copy. bias: F32[out] or NULL. x, grad_x: rows x_ld apart; residual, y, saved, out, grad_y: rows y_ld
  * apart. residual may be NULL, and y may be the residual's own buffer. saved (NULL allowed) receives act(x W^T + bias), what
  * the backward pass needs where a residual was added. Each output is rounded once, from 32 bits. A sum that is NaN stays
- * NaN behind every activation (bt_dense_* make it 0 behind one that clamps). Each matrix has at most 2^36 elements.
+ * NaN behind every activation (bt_dense_* make it 0 behind one that clamps). Each matrix has at most 2^36
+ * elements and 2^30 rows or columns.
  * A workspace is needed for some shapes (bt_affine_forward_workspace_bytes says how much; 0: may be NULL). */
 typedef struct {
     int batch, in, out;

@@ -100,3 +100,74 @@ def test_nan_shows_behind_every_activation(kind, act):
         for t in (y, saved):
             t = t.float().cpu()
             assert torch.equal(t.isnan(), want.isnan()) and torch.equal(t.nan_to_num(7.0), want.nan_to_num(7.0)), (batch, in_, out)
+
+
+# ---------------------------------------------------------------- launches of more than 2^32 threads
+def uniform(rows, cols, kind, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.empty(rows, cols, dtype=DT[kind], device="cuda").uniform_(-1.0, 1.0, generator=g)
+
+
+def compare(got, want, tol, kind, what):
+    """as affine_ref.check, on the device"""
+    allow = tol + ar.EPS[kind] * want.abs() * 1.01 + ar.TINY[kind]
+    bad = int((~((got.double() - want).abs() <= allow)).sum())
+    assert bad == 0, (what, bad)
+
+
+def by_rows(rows, step=1 << 25):
+    for a in range(0, rows, step):
+        yield slice(a, min(rows, a + step))
+
+
+@pytest.mark.parametrize("kind,batch,in_,out", [("f32", 1 << 29, 16, 4), ("bf16", 1 << 30, 8, 8), ("bf16", (1 << 30) - 3, 8, 8)])
+def test_forward_of_more_rows_than_one_dimension_of_a_launch_has_threads(kind, batch, in_, out):
+    x, w = uniform(batch, in_, kind, 1), uniform(in_, out, kind, 2)
+    y = torch.full((batch, out), float("nan"), device="cuda", dtype=DT[kind])
+    forward(kind, "relu", w, x, y)
+    for r in by_rows(batch):
+        a = x[r].double()
+        compare(y[r], (a @ w.double()).clamp(min=0), ar.sums(in_ + 1) * (a.abs() @ w.double().abs()), kind, r)
+    del x, y
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind,batch,in_,out", [("f32", 1 << 29, 16, 4)])
+def test_backward_of_as_many_rows(kind, batch, in_, out):
+    x, w, gy = uniform(batch, in_, kind, 1), uniform(in_, out, kind, 2), uniform(batch, out, kind, 3)
+    dw, db, gx = torch.zeros(in_, out, device="cuda"), torch.zeros(out, device="cuda"), torch.zeros_like(x)
+    backward(kind, "identity", w, x, None, gy, dw, db, gx)
+    sums = dict(dw=0.0, adw=0.0, db=0.0, adb=0.0)
+    for r in by_rows(batch):
+        a, g = x[r].double(), gy[r].double()
+        compare(gx[r], g @ w.double().t(), ar.sums(out) * (g.abs() @ w.double().abs().t()), kind, r)
+        # (column by column: the library's product of 16 x 2^25 and 2^25 x 4 takes seconds)
+        outer = [(a * g[:, o:o + 1]) for o in range(out)]
+        for k, v in (("dw", torch.stack([p.sum(0) for p in outer], 1)), ("adw", torch.stack([p.abs_().sum(0) for p in outer], 1)),
+                     ("db", g.sum(0)), ("adb", g.abs().sum(0))):
+            sums[k] = sums[k] + v
+    compare(dw, sums["dw"], ar.sums(batch) * sums["adw"], "f32", "dw")
+    compare(db, sums["db"], (ar.sums(batch) + 4 * ar.U) * sums["adb"], "f32", "dbias")
+    del x, gy, gx
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_one_row_of_more_outputs_than_a_launch_has_workgroups_for(kind):
+    out = (1 << 29) + 70
+    x, w = uniform(1, 1, kind, 1), uniform(1, out, kind, 2)
+    y = torch.full((1, out), float("nan"), device="cuda", dtype=DT[kind])
+    forward(kind, "identity", w, x, y)
+    want = (x.double() * w.double())
+    compare(y, want, torch.zeros_like(want), kind, "y")
+    db = torch.zeros(out, device="cuda")
+    dw = torch.zeros(1, out, device="cuda")
+    backward(kind, "identity", w, x, None, y, dw, db, None)
+    compare(db, y.double()[0], 0.0, "f32", "dbias")
+    compare(dw, x.double() * y.double(), 0.0, "f32", "dw")
+    db.zero_()
+    backward(kind, "identity", None, x, None, y, None, db, None)  # the column sums in a launch of their own
+    compare(db, y.double()[0], 0.0, "f32", "dbias alone")
+    del w, y, dw, db, want
+    torch.cuda.empty_cache()
