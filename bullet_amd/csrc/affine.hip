@@ -991,10 +991,15 @@ int join_launch(hipStream_t st, const Product &P) {
     BT_LAUNCH_CHECK();
     return BT_OK;
 }
+// (256 x 256 tiles have no registers to spare for operands on their way into LDS)
+Shape fitted(Shape s, int m, int n, bool direct) {
+    if (s.bm == 256 && !direct) s.bm = 128, s.tiles_m = bt_div_up(m, 128), s.tiles_n = bt_div_up(n, 128);
+    return s;
+}
 template <typename T, bool AK, bool BKC, int OUT>
-int product_launch(hipStream_t st, Product &P, Shape s) {
+int product_launch(hipStream_t st, Product &P, const Shape &shape) {
     const bool dma = P.a.aligned && P.b.aligned;
-    if (s.bm == 256 && !dma) s.bm = 128, s.tiles_m = bt_div_up(P.m, 128), s.tiles_n = bt_div_up(P.n, 128);
+    const Shape s = fitted(shape, P.m, P.n, dma);
     set_shape(P, s);
     if (s.splits == 1) return tile_launch<T, AK, BKC, OUT>(st, P, s, dma);
     if (int rc = tile_launch<T, AK, BKC, OUT_PART>(st, P, s, dma)) return rc;
@@ -1303,6 +1308,24 @@ int bt_affine_backward(void *stream, const bt_affine_desc *d, const void *w, con
     if (d->type == BT_TYPE_F32) return backward<float>(s, d, w, x, out, grad_y, dw, dbias, grad_x, ws);
     if (d->type == BT_TYPE_BF16) return backward<__bf16>(s, d, w, x, out, grad_y, dw, dbias, grad_x, ws);
     return backward<_Float16>(s, d, w, x, out, grad_y, dw, dbias, grad_x, ws);
+}
+
+// Tests ask which variant a call takes: the tile, the workgroups that share one, and whether both gradients take one launch
+// (product 0: forward, 1: dw, 2: grad_x; direct: whether the operands' first elements are on 16 bytes). Tile 0: affine_few.
+int bt_internal_affine_variant(const bt_affine_desc *d, int product, int direct, int *tile, int *splits, int *both) {
+    if (int rc = validate(d, "bt_internal_affine_variant")) return rc;
+    BT_REQUIRE(product >= 0 && product <= 2 && tile && splits && both, "bt_internal_affine_variant: no such product");
+    Shape s = {};
+    *both = 0;
+    if (product == 0) {
+        s = fitted(forward_plan(d).s, d->batch, d->out, direct);
+    } else {
+        const BackwardPlan p = backward_plan(d);
+        *both = p.both && direct;
+        s = product == 1 ? fitted(p.dw, d->in, d->out, direct) : fitted(p.dx, d->batch, d->in, direct);
+    }
+    *tile = s.bm, *splits = s.splits;
+    return BT_OK;
 }
 
 }  // extern "C"

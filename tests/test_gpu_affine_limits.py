@@ -171,3 +171,49 @@ def test_one_row_of_more_outputs_than_a_launch_has_workgroups_for(kind):
     compare(db, y.double()[0], 0.0, "f32", "dbias alone")
     del w, y, dw, db, want
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------- every tile size
+def variant(product, shape, kind, act="identity", w32=False, pad=0, direct=True):
+    """tile and workgroups that share one (0 for the forward of few rows), as the library chooses them"""
+    batch, in_, out = shape
+    d = ar.desc(batch, in_, out, kind, act, w32, out + pad, in_ + pad, out + pad)
+    tile, splits, both = C.c_int(), C.c_int(), C.c_int()
+    lib.check(tg.L.bt_internal_affine_variant(C.byref(d), product, int(direct), C.byref(tile), C.byref(splits), C.byref(both)))
+    return tile.value, splits.value
+
+
+# bf16 and f16 shapes whose forward product takes 256 x 256 tiles: whole, with a ragged last tile in every direction, with
+# two, three and many tiles of k, the last one ragged
+FORWARD_256 = [(3841, 70, 4090), (3900, 130, 4000), (4096, 64, 4096), (3850, 448, 4003)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", FORWARD_256)
+def test_forward_in_256_tiles(shape, kind):
+    assert variant(0, shape, kind) == (256, 1)
+    rng = np.random.default_rng(61)
+    tg.run_forward(rng, *shape, kind, "screlu", residual=True)
+    tg.run_forward(rng, *shape, kind, "identity", bias=False, pad=8)
+    tg.run_forward(rng, *shape, kind, "crelu", residual=True, w32=True, pad=1)  # (both operands copied first)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_256_tiles_fall_back_to_128_through_registers(kind):
+    """rows on 16 bytes behind a first element that is not"""
+    for shape in ((3841, 70, 4088), (3904, 136, 4000)):
+        assert variant(0, shape, kind, pad=8) == (256, 1) and variant(0, shape, kind, pad=8, direct=False) == (128, 1)
+        tg.run_forward(np.random.default_rng(62), *shape, kind, "relu", residual=True, pad=8, shift=1)
+
+
+# backward passes with 256 x 256 tiles, in three shares of both gradients or for grad_x alone: one summand of the gradient, two
+# or three, and (f16) two in shares of their own
+BACKWARD_256 = [((4200, 1000, 4200), "crelu", "bf16", (256, 3), (256, 3)), ((4200, 1000, 4200), "identity", "f16", (256, 3), (256, 3)),
+                ((4200, 1000, 4200), "screlu", "bf16", (256, 3), (256, 3)), ((3900, 4000, 300), "relu", "bf16", (64, 1), (256, 1)),
+                ((3900, 4000, 300), "screlu", "bf16", (128, 8), (256, 1)), ((3900, 4000, 300), "screlu", "f16", (64, 4), (256, 2))]
+
+
+@pytest.mark.parametrize("shape,act,kind,dw,dx", BACKWARD_256)
+def test_backward_in_256_tiles(shape, act, kind, dw, dx):
+    assert variant(1, shape, kind, act) == dw and variant(2, shape, kind, act) == dx
+    tg.run_backward(np.random.default_rng(63), *shape, kind, act)
