@@ -267,9 +267,12 @@ struct Product {
 // Written out, since the compiler lets every LDS read wait for all such loads of its own; wait_loads() is the wait (for all but
 // the N youngest loads), in front of the barrier behind which the chunk is read. The s_nop is the wait state between m0 and
 // its use.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (that m0 is a reserved register: it is, and this is where it changes)
 __device__ __forceinline__ void to_lds(const char *base, uint32_t offset, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2" : : "v"(offset), "s"(lds), "s"(base) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int N = 0>
 __device__ __forceinline__ void wait_loads() {
     static_assert(N < 64, "what the counter holds");
