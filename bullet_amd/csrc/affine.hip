@@ -7,6 +7,9 @@
 // A k-contiguous operand is staged in LDS as rows of 128 bytes of k and read 16 bytes a lane; one that is contiguous the
 // other way is staged as it lies and read transposed (ds_read_b64_tr_b16 for 16-bit types, single words for f32), so no
 // operand is ever transposed in memory. f32 goes through v_mfma_f32_16x16x4_f32: exact products, 32-bit sums.
+//
+// Times in this file: of a long run of calls, over operands that the caches do not hold where they are large. The first calls
+// after the card has idled take more, 264 us instead of 218 of the largest product; comparisons of two variants are of one run.
 #include <type_traits>
 
 #include "common.h"
@@ -513,9 +516,9 @@ __global__ __launch_bounds__(64 * WM * WN) void affine_mm_any(Product P) {
 //
 // Bound by the MFMA units and, close behind, by the LDS bytes that feed them, which is why the largest tile that still fills
 // the chip is taken: for one product of 16 x 16 x 32 a 256 x 256 tile reads 384 bytes of LDS, a 128 x 128 one 512 and a
-// 64 x 64 one 1024. 16384 x 2048 -> 4096 bf16 takes 207 us, 1.33 PFLOP/s (the MFMA units are busy 59 % of the clocks, bank
-// conflicts are few); dW of 16384 x 2048 -> 2048 with 4 workgroups to a tile 110 us and grad_x 109, 1.25 PFLOP/s;
-// 4096 x 1024 -> 1024 f32 with 64 x 64 tiles 66 us, 130 TFLOP/s, 83 % of the rate of f32.
+// 64 x 64 one 1024. 16384 x 2048 -> 4096 bf16 takes 218 us, 1.26 PFLOP/s (the MFMA units are busy 58 % of the clocks, bank
+// conflicts are few); dW of 16384 x 2048 -> 2048 with 4 workgroups to a tile 108 us and grad_x 105, 1.27 and 1.32 PFLOP/s;
+// 4096 x 1024 -> 1024 f32 with 64 x 64 tiles, residual and kept activation 71 us, 121 TFLOP/s, 79 % of a large library product's.
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BKC, int OUT, int BUFS>
 __device__ __forceinline__ void mm_direct(const Product &P, int wg, char *lds) {
     typedef Mm<T, BM, BN, WM, WN, AK, BKC, OUT> M;
@@ -623,7 +626,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void affine_mm_direct(Product P) {
     mm_direct<T, BM, BN, WM, WN, AK, BKC, OUT, BUFS>(P, (int)folded_block(), lds);
 }
 // dW and grad_x of a small layer in one launch: neither has tiles enough to fill the chip, or to hide its own latency
-// (200 x 512 -> 333 f32: 8 us, 288 workgroups of 32 x 32 that each walk their whole k; 76 of 64 x 64: 11)
+// (200 x 512 -> 333 f32: 7.2 us, 288 workgroups of 32 x 32 that each walk their whole k; 76 of 64 x 64: 11)
 template <typename T, int B, int OUT_W, int OUT_X, int BUFS>
 __global__ __launch_bounds__(256, 2) void affine_mm_both(Product W, Product X) {
     extern __shared__ __align__(1024) char lds[];
@@ -634,8 +637,8 @@ __global__ __launch_bounds__(256, 2) void affine_mm_both(Product W, Product X) {
         mm_direct<T, B, B, 2, 2, true, true, OUT_X, BUFS>(X, wg - first, lds);
 }
 
-// The splits' sums added in order, then the epilogue. Memory bound: 4 splits of 2048 x 2048 (67 MB of sums, 8 MB out) 13 us,
-// 5.8 TB/s.
+// The splits' sums added in order, then the epilogue. Memory bound: 4 splits of 2048 x 2048 (67 MB of sums, 17 MB out) 13 us,
+// 6.5 TB/s, some of the sums still in the caches.
 template <typename T, int OUT>
 __global__ __launch_bounds__(256) void affine_join(Product P) {
     const long long q = folded_block() * 256 + threadIdx.x, cols = P.part_ld / 4;
@@ -659,7 +662,7 @@ __global__ __launch_bounds__(256) void affine_join(Product P) {
 //
 // A copy has rows on 128 bytes (so that a tile's row of k is one line of memory), of the layer's type (f32 weights are
 // rounded), with zeros up to a whole chunk. One chunk a thread. Both the copies and gz are bound by memory: gz of 16384 x 2048
-// bf16 (two reads, one write, 201 MB) 37 us, 5.4 TB/s.
+// bf16 (two reads, one write, 201 MB) 38 us, 5.3 TB/s.
 template <typename T>
 struct Copy {
     const void *from;
@@ -798,8 +801,9 @@ __global__ __launch_bounds__(256) void affine_prepare(Prepare<T> p) {
 // there is nothing for the matrix cores. A workgroup takes 4 chunks of outputs (64 bytes of every weight column; f32
 // weights of a 16-bit layer: 128) for all inputs: its groups of 4 lanes walk the inputs V at a time with V weight loads in
 // flight each, and their sums meet in DPP, shuffles and LDS, in a fixed order. 1024 threads, or 512 where the sums and
-// loads of more than 2 rows need the registers. 1 x 2048 -> 4096 bf16: 8 us with the weights (16.8 MB) in memory, which a copy
-// would read in 3.5: launch, the first load's latency and the reduction have nothing to hide behind.
+// loads of more than 2 rows need the registers. 1 x 2048 -> 4096 bf16: 7.8 us with the weights (16.8 MB) in memory, which a copy
+// would read in 3.3: 128 workgroups leave half of the CUs idle, and launch, the first load's latency and the reduction have nothing
+// to hide behind. (Long sums into few outputs are one workgroup's: nothing shares k here.)
 constexpr int few_threads(int rows) { return rows > 2 ? 512 : 1024; }
 template <typename T, typename TW, int R>
 __global__ __launch_bounds__(few_threads(R)) void affine_few(const TW *__restrict__ w, long long w_ld, const T *__restrict__ x, long long x_ld,
@@ -984,7 +988,7 @@ int tile_launch(hipStream_t st, const Product &P, const Shape &s, bool direct) {
     return mm_launch<T, 64, 64, 2, 2, AK, BKC, OUT>(st, P, direct);
 }
 void set_shape(Product &P, const Shape &s) {
-    // (of at most 2^36 outputs, tiles of 64 x 64 are less than 2^26, of 32 x 32 less than 2^28; shared only where they are few)
+    // (of at most 2^36 outputs and 2^30 rows there are at most 2^26 tiles of any size; k is shared only where they are few)
     P.tiles_m = s.tiles_m, P.tiles_n = s.tiles_n, P.splits = s.splits, P.wgs = s.tiles_m * s.tiles_n * s.splits;
     P.part_ld = (P.n + 3) / 4 * 4;
 }
@@ -1052,8 +1056,8 @@ Operand matrix(const void *p, long long ld, int rows, int len, size_t es) {
 Operand own_matrix(const void *p, int rows, int len, size_t es) { return matrix(p, padded(len, es), rows, whole_chunks(len, es), es); }
 
 // Outputs whose rows start on 16 bytes are stored past the caches, where they would only push out the operands (16384 x 2048 ->
-// 4096 bf16 207 us, 231 through them). Pieces of other rows share lines, which the caches put together (1537 x 1027 -> 1881 f16,
-// rows 3 apart: 20.4 us through them, 22.7 past them).
+// 4096 bf16 218 us, 229 through them; backward of 2048 -> 2048 263 and 271). Pieces of other rows share lines, which the caches put
+// together (1537 x 1027 -> 1881 f16, rows 3 apart: 21.6 us through them, 22.7 past them).
 bool past_caches(const void *out, const void *saved, long long ld, size_t es) {
     return ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(saved)) & 15) == 0 && ld * es % 16 == 0;
 }

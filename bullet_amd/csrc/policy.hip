@@ -5,6 +5,8 @@
 // statistics and the gradient, and so reads every logit once and writes every gradient once. Per-row scalars (log-sum,
 // log-probability, ratio, losses) are computed in 64 bits from the row's 32-bit sum: they cost one evaluation a row and
 // keep the rounding of values near 7 out of differences that may be near 0.
+//
+// Times in this file: of the last of some thousand launches in a row, over inputs that the caches do not hold.
 #include <type_traits>
 
 #include "common.h"
@@ -183,9 +185,9 @@ __device__ __forceinline__ void keep_legal(const uint8_t *mask, int e0, int widt
         for (int j = 0; j < Row<T>::V; j++) v[j] = legal_at(b, j) ? v[j] : (T)NEG_INF;
     }
 }
-// (Past the caches: nothing here reads it again, and the logits stay where the gradient would push them out. 8192 x 4096 bf16 33
-// us, with ordinary stores 37 to 45; 256 pairs of lines, whose logits are read twice, 50 and 58. Loads past the caches are slower,
-// 112 us instead of 83 for 16384 x 1880 f32.)
+// (Past the caches: nothing here reads it again, and the logits stay where the gradient would push them out. Whole calls: 8192 x
+// 4096 bf16 37 us, with ordinary stores 40; 256 pairs of lines, whose logits are read twice, 54 and 60; 16384 x 1880 f32 83 and 85.
+// Loads past the caches are slower, 112 us instead of 83 for the last.)
 template <typename T>
 __device__ __forceinline__ void store_chunk(T *row, int e0, int width, typename Row<T>::vec v) {
     constexpr int V = Row<T>::V;
@@ -322,7 +324,7 @@ __device__ __noinline__ double sum_again(const T *z, const uint8_t *mask, int wi
 
 // One group of G lanes per row, at most K chunks a lane, all in registers.
 // Bound by memory where there are many rows: 16384 x 1880 f32 with the full KL (two rows of logits and the mask in, gradient
-// out, 401 MB) 82-84 us, 4.8 TB/s, what a copy reaches; 8192 x 4096 bf16 (134 MB) 31 us, 4.3 TB/s. Few rows: 6-7 us for 64 of
+// out, 401 MB) 80 us, 5.0 TB/s, what a copy reaches; 8192 x 4096 bf16 (134 MB) 33 us, 4.0 TB/s. Few rows: 6.7 us for 64 of
 // 1880, the time of a launch and of four loads in turn (mask and logits, the action, its logit, its row's scalars).
 template <typename T, int G, int K, bool FULL>
 __global__ __launch_bounds__(256) void policy_rows(PolicyArgs a) {
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(256) void policy_rows_long(PolicyArgs a) {
     if (counted && lane == (act / V) % 256) grad[act] = (T)grad_taken;
 }
 
-// loss_sum = sum of n losses, in 64 bits and a fixed order, by THREADS threads: a launch's 2 us for 16384 losses. (A launch of
+// loss_sum = sum of n losses, in 64 bits and a fixed order, by THREADS threads: 1.7 us for 64 losses, 4.6 for 16384. (A launch of
 // its own, since the last row kernel's workgroup to finish could only add them up behind an atomic counter, which a captured
 // and an eager call of the same buffers would have to share.)
 template <int THREADS>
@@ -560,7 +562,7 @@ struct PrefArgs {
 __device__ __forceinline__ int pref_offset(const PrefArgs &a, int k) { return min(max(a.offsets[k], 0), a.d.rows); }
 
 // Statistics of one row, as in policy_rows. The rows are read again for the gradient, since a pair's factor needs all
-// rows of both its lines first: 16740 x 1880 bf16 (logits and mask 94 MB) 21 us, 4.6 TB/s.
+// rows of both its lines first: 16740 x 1880 bf16 (logits and mask 94 MB) 22 us, 4.3 TB/s.
 template <typename T, int G, int K>
 __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
     constexpr int V = Row<T>::V;
@@ -622,7 +624,7 @@ __global__ __launch_bounds__(256) void pref_rows(PrefArgs a) {
 }
 
 // One wave per pair, one row a lane: the lines' sums and the pair's loss, then what its rows' gradients need. Loads in turn
-// bound it (the offsets, the rows' numbers, then 64-bit arithmetic on them): 3.6 us for one pair, 5.6 for 256.
+// bound it (the offsets, the rows' numbers, then 64-bit arithmetic on them): 4.4 us for 4 pairs, 5.9 for 256.
 __global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
     const long long p64 = row_block() * 4 + (threadIdx.x >> 6);
     const int p = (int)p64, lane = threadIdx.x & 63;
@@ -676,8 +678,8 @@ __global__ __launch_bounds__(256) void pref_pairs(PrefArgs a) {
     }
 }
 
-// The gradient of one row: its logits once more, the numbers its pair left for it, one write. 16740 x 1880 bf16: 25 us for
-// logits, mask and gradient, 157 MB at 6.3 TB/s, some of it still in the caches. (The first workgroup adds the pairs'
+// The gradient of one row: its logits once more, the numbers its pair left for it, one write. 16740 x 1880 bf16: 26 us for
+// logits, mask and gradient, 157 MB at 6.0 TB/s, some of it still in the caches. (The first workgroup adds the pairs'
 // losses up, the others follow with the rows.)
 template <typename T, int G, int K>
 __global__ __launch_bounds__(256) void pref_grad(PrefArgs a) {

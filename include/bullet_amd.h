@@ -320,7 +320,9 @@ int bt_affine_backward(void *stream, const bt_affine_desc *desc, const void *w, 
  * has no effect. actions: I32[batch]. A row is not counted (loss, gradient, row outputs all exactly 0) if its action is
  * outside [0, width) (-1 marks padding), is masked, or if every legal logit is -infinity. grad of masked places is 0.
  * The gradient passes where r A is not above its clipped value. NaN or +infinity in a legal place makes its row's loss NaN,
- * and so do reference logits that leave a counted row nothing above -infinity.
+ * and so do reference logits that leave a counted row nothing above -infinity. A legal action at -infinity has l = -infinity,
+ * r = 0 and an infinite KL (BT_KL_TAKEN), as has a reference policy without a move that has a share (BT_KL_FULL); kl_weight 0
+ * keeps an infinite KL out of loss and gradient.
  * row_weights F32[batch] or NULL = 1. Outputs: loss_sum F32[1] (overwritten, un-normalised, as bt_loss); grad (type and
  * ld of logits; may be the logits themselves, or NULL = loss only); row_loss F32[batch]; row_logp (l[a]) and row_kl (KL):
  * F32[batch] or NULL. */
@@ -345,6 +347,7 @@ int bt_policy_loss(void *stream, const bt_policy_desc *desc, const void *logits,
  *   d = beta * ((s_2p - ref_2p) - (s_2p+1 - ref_2p+1)),  ref_logp F32[2*pairs]: the lines' s under the reference policy
  *   pair_loss[p] = weight[p] * ( -(1 - smoothing) log sigmoid(d) - smoothing log sigmoid(-d) )
  *   loss_sum[0] = sum of pair_loss;   grad = d loss_sum / d logits
+ * (d may be infinite, where a line holds a legal action at -infinity; smoothing 0 then leaves the second term out.)
  * offsets: I32[2*pairs + 1] on the device, not decreasing, within [0, rows] (values outside are taken as the nearest
  * bound). Rows in front of the first line and behind the last are neither read nor written: `grad` keeps what it held.
  * pair_weights F32[pairs] or NULL = 1; grad may be the logits themselves, or NULL; pair_loss F32[pairs]; line_logp (s):
